@@ -685,6 +685,126 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_batch_matmul_packed_rhs(
     float out_scale, iree_amd_uk_index_t batch, iree_amd_uk_index_t lhs_batch_stride,
     iree_amd_uk_index_t rhs_batch_stride, iree_amd_uk_index_t out_batch_stride, void* stream);
 
+/*===------------------------------------------------------------------------===
+ * The attention block of a language model on a cache held in 4 bits (no
+ * reference ukernel; what runs between the q/k/v projection and the output
+ * projection of a layer whose weights iree_amd_uk_dequant_matmul_i4 multiplies).
+ *
+ * The cache is a pool of pages. A page holds `page_size` tokens (a power of two,
+ * 16 to 256) of every kv head: one block of page_size * (head_dim + 8) bytes per
+ * head, in which lie, one after the other,
+ *   K codes   [page_size][head_dim / 2] bytes, even d in the low nibble
+ *   V codes   [page_size / 4][head_dim / 8][4] dwords: a dword holds 8 consecutive
+ *             d of one token (the lowest d in the lowest nibble), the 4 tokens of a
+ *             group side by side
+ *   K params  [page_size] pairs of f16, scale and offset of the token's K row
+ *   V params  [page_size] pairs of f16 of its V row
+ * A code c stands for c * scale + offset. A row x of head_dim values is stored as
+ *   offset = f16(min x), scale = f16((max x - min x) / 15)   (saturating at 65504)
+ *   c = clamp(rne((x - offset) / scale), 0, 15), 0 where scale = 0
+ * computed without a rounding before the code; a row with a value that is not finite
+ * gets the scale NaN, so that all of it reads as NaN.
+ * head_dim is 64, 128 or 256. Page p begins at byte p * page_stride of the cache
+ * (a multiple of 16, at least iree_amd_uk_kv4_page_bytes: a pool that holds all
+ * layers of a page side by side passes the layer's address and the pool's stride);
+ * the cache is 16-byte aligned. Token t of a sequence lies in page
+ * page_table[t / page_size] at row t % page_size; its slot is
+ * page * page_size + row.
+ *===------------------------------------------------------------------------===*/
+#define IREE_AMD_UK_FLAG_ATTENTION_TYPE_MASK 0xFF
+#define IREE_AMD_UK_FLAG_ATTENTION_TYPE_F16 0x01  /* type of the rows q, k, v, out */
+#define IREE_AMD_UK_FLAG_ATTENTION_TYPE_BF16 0x02
+/* Rotation pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2). */
+#define IREE_AMD_UK_FLAG_ATTENTION_ROPE_INTERLEAVED 0x100
+
+/* Bytes of one page of one layer: kv_heads * page_size * (head_dim + 8). Host only. */
+IREE_AMD_UK_EXPORT int iree_amd_uk_kv4_page_bytes(int32_t page_size, int32_t kv_heads,
+                                                  int32_t head_dim, iree_amd_uk_index_t* out_bytes);
+
+/* RMS norm of every query and key head, their position rotation, and the keys and
+ * values into the cache, in one launch. For each of `tokens` tokens and each head
+ * row x of q ([tokens][heads][head_dim], q_stride0 elements between tokens) and of
+ * k ([tokens][kv_heads][head_dim]):
+ *   y = x / sqrt(mean(x^2) + eps) * weight      (weight null: y = x)
+ *   a' = a cos - b sin, b' = b cos + a sin      (cos_sin null: no rotation)
+ * for the pairs (a, b) of y's first rotary_dim values (a multiple of 8), cos and sin
+ * of pair i at cos_sin[position][i] and cos_sin[position][rotary_dim / 2 + i] of a
+ * table of table_rows rows, positions[token] the position. Computed in 64 bits, rounded
+ * to f32 and that to the rows' type. q goes to q_out, k to k_out (either may be its input's own buffer, with the
+ * same stride; k_out may be null with a cache). With a cache, the rounded k row and
+ * the v row of token t are stored at slots[t]. q, or k and v, may be null: nothing is
+ * done for them. Weights have the rows' type. A token whose position lies outside the
+ * table is padding: nothing is written for it. A slot outside the cache is not
+ * stored. Slots must be distinct: of two tokens with one slot, either may leave each
+ * part of the row. Row buffers 16-byte aligned with strides of whole 8 elements, cos_sin
+ * and weights 16-byte aligned (UNIMPLEMENTED otherwise, and for another head_dim). */
+IREE_AMD_UK_EXPORT int iree_amd_uk_qk_norm_rope(
+    const void* q, iree_amd_uk_index_t q_stride0, const void* k, iree_amd_uk_index_t k_stride0,
+    const void* v, iree_amd_uk_index_t v_stride0, void* q_out, iree_amd_uk_index_t q_out_stride0,
+    void* k_out, iree_amd_uk_index_t k_out_stride0, const void* q_weight, const void* k_weight,
+    float eps, const float* cos_sin, iree_amd_uk_index_t table_rows, int32_t rotary_dim,
+    const int32_t* positions, void* cache, iree_amd_uk_index_t pages,
+    iree_amd_uk_index_t page_stride, int32_t page_size, const int64_t* slots,
+    iree_amd_uk_index_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, uint32_t flags,
+    void* stream);
+
+/* Rows back out of the cache: k_out[i] and v_out[i] ([rows][kv_heads][head_dim], either
+ * may be null) receive what slots[i] holds, rounded once to the rows' type. A row whose
+ * slot lies outside the cache is left as it was. Alignment as above. */
+IREE_AMD_UK_EXPORT int iree_amd_uk_kv4_read(
+    const void* cache, iree_amd_uk_index_t pages, iree_amd_uk_index_t page_stride,
+    int32_t page_size, const int64_t* slots, void* k_out, iree_amd_uk_index_t k_out_stride0,
+    void* v_out, iree_amd_uk_index_t v_out_stride0, iree_amd_uk_index_t rows, int32_t kv_heads,
+    int32_t head_dim, uint32_t flags, void* stream);
+
+/* Attention over the cache. Sequence b of `batch` has the query tokens
+ * [q_starts[b], q_starts[b + 1]) (q_starts does not fall) of q
+ * ([tokens][heads][head_dim]) and kv_lens[b] tokens in the cache, the last of which are
+ * the queries' own: its i-th query stands at position p = kv_lens[b] - queries + i.
+ * Query head h reads kv head h / (heads / kv_heads). Token j is visible to position p
+ * when j <= p and (window == 0 or j > p - window or j < sinks) and its page exists: its
+ * entry of page_table[b] ([batch][max_pages], page_table_stride entries between
+ * sequences) lies in [0, pages) (a program that has freed the pages behind its window
+ * writes -1), and j < max_pages * page_size.
+ *   out = sum_j softmax_j(scale * q . k_j) v_j over the visible tokens
+ * Sums and the softmax in f32, rounded once to the rows' type; zeros where nothing is
+ * visible. Rows of q outside [q_starts[0], q_starts[batch]) are neither read nor
+ * written. What masked tokens and pages hold, NaN among it, changes nothing.
+ *   max_kv_len: the longest of kv_lens as far as the caller knows (it sets how the work is
+ * split, not what is computed; 0: max_pages * page_size).
+ *   workspace: partial results of a long cache that is read by several workgroups, at
+ * least what iree_amd_uk_attention_kv4_workspace says, 16-byte aligned; with less, or
+ * null, the call runs unsplit (slower). The caller's: calls that may overlap, and graphs
+ * whose replays may, need one each.
+ * The library's memory is not used and nothing is allocated. Alignment as above. */
+IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4(
+    const void* q, iree_amd_uk_index_t q_stride0, void* out, iree_amd_uk_index_t out_stride0,
+    const void* cache, iree_amd_uk_index_t pages, iree_amd_uk_index_t page_stride,
+    int32_t page_size, const int32_t* page_table, iree_amd_uk_index_t page_table_stride,
+    iree_amd_uk_index_t max_pages, const int32_t* q_starts, const int32_t* kv_lens,
+    iree_amd_uk_index_t tokens, iree_amd_uk_index_t batch, int32_t heads, int32_t kv_heads,
+    int32_t head_dim, float scale, iree_amd_uk_index_t window, iree_amd_uk_index_t sinks,
+    iree_amd_uk_index_t max_kv_len, void* workspace, uint64_t workspace_bytes, uint32_t flags,
+    void* stream);
+/* Bytes of workspace such a call of these sizes uses on the current device (0: none). */
+IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4_workspace(
+    iree_amd_uk_index_t tokens, iree_amd_uk_index_t batch, int32_t heads, int32_t kv_heads,
+    int32_t head_dim, iree_amd_uk_index_t window, iree_amd_uk_index_t sinks,
+    iree_amd_uk_index_t max_kv_len, uint64_t* out_bytes);
+
+/* Copies `count` pages inside a pool of `pages` pages, page_stride bytes apart: the first
+ * page_bytes bytes of page src[i] to page dst[i] (both multiples of 16, the pool 16-byte
+ * aligned). src and dst are HOST arrays; they are read before the call returns and become
+ * part of the launches (a captured call copies the same pages on every replay). What a
+ * fork (a copy of the last, partly filled page), a compaction or a move needs. Page
+ * numbers outside the pool, a page that is written twice, and a page that is both
+ * written and read are refused. */
+IREE_AMD_UK_EXPORT int iree_amd_uk_copy_pages(void* pool, iree_amd_uk_index_t pages,
+                                              iree_amd_uk_index_t page_bytes,
+                                              iree_amd_uk_index_t page_stride, const int32_t* src,
+                                              const int32_t* dst, iree_amd_uk_index_t count,
+                                              void* stream);
+
 /* buf[i] *= scale over n f32 elements, in place (applies the product of the
  * per-tensor scales to an fp8 matmul result). */
 IREE_AMD_UK_EXPORT int iree_amd_uk_scale_f32(void* buf_f32, iree_amd_uk_index_t n,

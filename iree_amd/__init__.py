@@ -8,6 +8,15 @@ used only to own device memory and streams.
 """
 from . import flags  # noqa: F401
 from ._lib import load_library, library_path  # noqa: F401
+from .attention import (  # noqa: F401
+    Kv4Cache,
+    attention_kv4,
+    attention_kv4_workspace,
+    copy_pages,
+    kv4_page_bytes,
+    kv4_read,
+    qk_norm_rope,
+)
 from .ukernel import (  # noqa: F401
     Fp8Mlp,
     UkError,

@@ -154,6 +154,21 @@ def _declare(lib):
     lib.iree_amd_uk_batch_matmul_packed_rhs.argtypes = [vp, i64, i64, vp, i64, i64, vp, i64, i64,
                                                         i64, i64, i64, C.c_int32, C.c_uint32, C.c_float,
                                                         i64, i64, i64, i64, vp]
+    f32 = C.c_float
+    lib.iree_amd_uk_kv4_page_bytes.restype = C.c_int
+    lib.iree_amd_uk_kv4_page_bytes.argtypes = [i32, i32, i32, C.POINTER(i64)]
+    lib.iree_amd_uk_qk_norm_rope.restype = C.c_int
+    lib.iree_amd_uk_qk_norm_rope.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, f32, vp, i64, i32,
+                                             vp, vp, i64, i64, i32, vp, i64, i32, i32, i32, u32, vp]
+    lib.iree_amd_uk_kv4_read.restype = C.c_int
+    lib.iree_amd_uk_kv4_read.argtypes = [vp, i64, i64, i32, vp, vp, i64, vp, i64, i64, i32, i32, u32, vp]
+    lib.iree_amd_uk_attention_kv4.restype = C.c_int
+    lib.iree_amd_uk_attention_kv4.argtypes = [vp, i64, vp, i64, vp, i64, i64, i32, vp, i64, i64, vp, vp, i64, i64,
+                                              i32, i32, i32, f32, i64, i64, i64, vp, u64, u32, vp]
+    lib.iree_amd_uk_attention_kv4_workspace.restype = C.c_int
+    lib.iree_amd_uk_attention_kv4_workspace.argtypes = [i64, i64, i32, i32, i32, i64, i64, i64, C.POINTER(u64)]
+    lib.iree_amd_uk_copy_pages.restype = C.c_int
+    lib.iree_amd_uk_copy_pages.argtypes = [vp, i64, i64, i64, vp, vp, i64, vp]
     lib.iree_amd_uk_scale_f32.restype = C.c_int
     lib.iree_amd_uk_scale_f32.argtypes = [vp, i64, C.c_float, vp]
     lib.iree_amd_uk_mfma_probe.restype = C.c_int

@@ -3,6 +3,7 @@
 // device ABI and the host-pointer staging variants. No kernels live here.
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include "uk_common.h"
@@ -873,6 +874,235 @@ extern "C" int iree_amd_uk_matmul_data_tiled(
     return launch_matmul_chain(a, b, c, lhs, rhs, out, M, N, K, M0, N0, K0, flags, (hipStream_t)stream);
   note_kernel_path("mmt4d:mfma-one-launch");
   return st;
+}
+
+// ---------------------------------------------------------------------------
+// Attention block on the 4-bit cache
+// ---------------------------------------------------------------------------
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// The flag word and head sizes that all entry points of the block share.
+static int validate_rows(const char* what, uint32_t flags, uint32_t known, int32_t kv_heads, int32_t head_dim) {
+  const uint32_t type = flags & IREE_AMD_UK_FLAG_ATTENTION_TYPE_MASK;
+  if (flags & ~(known | IREE_AMD_UK_FLAG_ATTENTION_TYPE_MASK))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: unknown flag bits 0x%x", what, flags & ~known);
+  if (type != IREE_AMD_UK_FLAG_ATTENTION_TYPE_F16 && type != IREE_AMD_UK_FLAG_ATTENTION_TYPE_BF16)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: unknown type 0x%x", what, type);
+  if (kv_heads < 0 || head_dim < 1) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: negative size", what);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: head_dim %d (64, 128 and 256 are served)", what, head_dim);
+  return 0;
+}
+
+// Rows [tokens][heads][head_dim] with `stride` elements between tokens.
+static int validate_row_buffer(const char* what, const char* name, const void* p, int64_t stride, int64_t tokens,
+                               int64_t heads, int64_t head_dim) {
+  if (!p) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null %s", what, name);
+  if (stride < 0 || (tokens > 1 && stride < heads * head_dim))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: %s stride below a row", what, name);
+  if (!aligned16(p) || stride % 8)
+    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: %s is not 16-byte aligned with a stride of whole 8 elements", what,
+                name);
+  return 0;
+}
+
+static int kv4_block_bytes(const char* what, int32_t page_size, int32_t head_dim, int64_t* out) {
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: page_size %d is not a power of two from 16 to 256", what,
+                page_size);
+  *out = (int64_t)page_size * (head_dim + 8);
+  return 0;
+}
+
+static int make_pool(const char* what, const void* cache, int64_t pages, int64_t page_stride, int32_t page_size,
+                     int32_t kv_heads, int32_t head_dim, Kv4Pool* out) {
+  int64_t block;
+  UK_RETURN_IF_ERROR(kv4_block_bytes(what, page_size, head_dim, &block));
+  if (!cache) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null cache", what);
+  if (pages < 0 || pages > 0x7FFFFFFF)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: pages outside [0, 2^31)", what);
+  if (page_stride < kv_heads * block || page_stride % 16 || !aligned16(cache) ||
+      page_stride > (INT64_MAX >> 1) / (pages + 1))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT,
+                "%s: the cache must be 16-byte aligned with pages whole 16 bytes apart, at least a page's bytes", what);
+  *out = {(char*)cache, pages, page_stride, __builtin_ctz((unsigned)page_size)};
+  return 0;
+}
+
+extern "C" int iree_amd_uk_kv4_page_bytes(int32_t page_size, int32_t kv_heads, int32_t head_dim,
+                                         iree_amd_uk_index_t* out_bytes) {
+  UK_RETURN_IF_ERROR(validate_rows("kv4_page_bytes", IREE_AMD_UK_FLAG_ATTENTION_TYPE_F16, 0, kv_heads, head_dim));
+  if (!out_bytes) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "kv4_page_bytes: null result");
+  int64_t block;
+  UK_RETURN_IF_ERROR(kv4_block_bytes("kv4_page_bytes", page_size, head_dim, &block));
+  *out_bytes = kv_heads * block;
+  return 0;
+}
+
+extern "C" int iree_amd_uk_qk_norm_rope(
+    const void* q, iree_amd_uk_index_t q_stride0, const void* k, iree_amd_uk_index_t k_stride0, const void* v,
+    iree_amd_uk_index_t v_stride0, void* q_out, iree_amd_uk_index_t q_out_stride0, void* k_out,
+    iree_amd_uk_index_t k_out_stride0, const void* q_weight, const void* k_weight, float eps, const float* cos_sin,
+    iree_amd_uk_index_t table_rows, int32_t rotary_dim, const int32_t* positions, void* cache, iree_amd_uk_index_t pages,
+    iree_amd_uk_index_t page_stride, int32_t page_size, const int64_t* slots, iree_amd_uk_index_t tokens, int32_t heads,
+    int32_t kv_heads, int32_t head_dim, uint32_t flags, void* stream) {
+  const char* what = "qk_norm_rope";
+  UK_RETURN_IF_ERROR(validate_rows(what, flags, IREE_AMD_UK_FLAG_ATTENTION_ROPE_INTERLEAVED, kv_heads, head_dim));
+  if (tokens < 0 || tokens > 0x7FFFFFFF || heads < 0)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: tokens or heads outside [0, 2^31)", what);
+  if (!(eps >= 0.f)) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: eps is not at least 0", what);
+  if (cos_sin && (rotary_dim < 8 || rotary_dim > head_dim || rotary_dim % 8 || table_rows < 0))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: rotary_dim must be a multiple of 8, at most head_dim", what);
+  if (heads == 0) q = nullptr;
+  if (kv_heads == 0) k = v = cache = nullptr;
+  QkNormRopeArgs a{};
+  if (cache)
+    UK_RETURN_IF_ERROR(make_pool(what, cache, pages, page_stride, page_size, kv_heads, head_dim, &a.pool));
+  if (tokens == 0 || (!q && !k && !cache)) return 0;
+  if (q) {
+    UK_RETURN_IF_ERROR(validate_row_buffer(what, "q", q, q_stride0, tokens, heads, head_dim));
+    UK_RETURN_IF_ERROR(validate_row_buffer(what, "q_out", q_out, q_out_stride0, tokens, heads, head_dim));
+  }
+  if (k || cache) {
+    UK_RETURN_IF_ERROR(validate_row_buffer(what, "k", k, k_stride0, tokens, kv_heads, head_dim));
+    if (k_out || !cache)
+      UK_RETURN_IF_ERROR(validate_row_buffer(what, "k_out", k_out, k_out_stride0, tokens, kv_heads, head_dim));
+  }
+  if (cache) {
+    UK_RETURN_IF_ERROR(validate_row_buffer(what, "v", v, v_stride0, tokens, kv_heads, head_dim));
+    if (!slots) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null slots", what);
+  } else if (v) {
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: v without a cache", what);
+  }
+  if ((q == q_out && q && q_stride0 != q_out_stride0) || (k == k_out && k && k_stride0 != k_out_stride0))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: in place with another stride", what);
+  if (cos_sin && !positions) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null positions", what);
+  if (!aligned16(q_weight) || !aligned16(k_weight) || !aligned16(cos_sin))
+    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: a weight or the table is not 16-byte aligned", what);
+  a.q = q, a.k = k, a.v = v, a.q_out = q_out, a.k_out = k_out;
+  a.q_stride = q_stride0, a.k_stride = k_stride0, a.v_stride = v_stride0;
+  a.q_out_stride = q_out_stride0, a.k_out_stride = k_out_stride0;
+  a.q_weight = q_weight, a.k_weight = k_weight, a.eps = eps;
+  a.cos_sin = cos_sin, a.table_rows = table_rows, a.rotary = rotary_dim, a.positions = positions, a.slots = slots;
+  a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim;
+  a.interleaved = (flags & IREE_AMD_UK_FLAG_ATTENTION_ROPE_INTERLEAVED) != 0;
+  a.bf16 = (flags & IREE_AMD_UK_FLAG_ATTENTION_TYPE_MASK) == IREE_AMD_UK_FLAG_ATTENTION_TYPE_BF16;
+  return launch_qk_norm_rope(a, (hipStream_t)stream);
+}
+
+extern "C" int iree_amd_uk_kv4_read(const void* cache, iree_amd_uk_index_t pages, iree_amd_uk_index_t page_stride,
+                                   int32_t page_size, const int64_t* slots, void* k_out,
+                                   iree_amd_uk_index_t k_out_stride0, void* v_out, iree_amd_uk_index_t v_out_stride0,
+                                   iree_amd_uk_index_t rows, int32_t kv_heads, int32_t head_dim, uint32_t flags,
+                                   void* stream) {
+  const char* what = "kv4_read";
+  UK_RETURN_IF_ERROR(validate_rows(what, flags, 0, kv_heads, head_dim));
+  if (rows < 0 || rows > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: rows outside [0, 2^31)", what);
+  if (rows == 0 || kv_heads == 0 || (!k_out && !v_out)) return 0;
+  Kv4ReadArgs a{};
+  UK_RETURN_IF_ERROR(make_pool(what, cache, pages, page_stride, page_size, kv_heads, head_dim, &a.pool));
+  if (!slots) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null slots", what);
+  if (k_out) UK_RETURN_IF_ERROR(validate_row_buffer(what, "k_out", k_out, k_out_stride0, rows, kv_heads, head_dim));
+  if (v_out) UK_RETURN_IF_ERROR(validate_row_buffer(what, "v_out", v_out, v_out_stride0, rows, kv_heads, head_dim));
+  a.slots = slots, a.k_out = k_out, a.v_out = v_out, a.k_out_stride = k_out_stride0, a.v_out_stride = v_out_stride0;
+  a.rows = rows, a.kv_heads = kv_heads, a.dim = head_dim;
+  a.bf16 = (flags & IREE_AMD_UK_FLAG_ATTENTION_TYPE_MASK) == IREE_AMD_UK_FLAG_ATTENTION_TYPE_BF16;
+  return launch_kv4_read(a, (hipStream_t)stream);
+}
+
+// Sizes that the call and its workspace query check alike.
+static int validate_attention_sizes(const char* what, int64_t tokens, int64_t batch, int32_t heads, int32_t kv_heads,
+                                    int64_t window, int64_t sinks, int64_t max_kv_len) {
+  if (tokens < 0 || tokens > 0x7FFFFFFF || batch < 0 || batch > 0x7FFFFFFF || heads < 0 || heads > 0xFFFF ||
+      window < 0 || sinks < 0 || max_kv_len < 0)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: a size is negative or too large", what);
+  if (heads && (kv_heads < 1 || heads % kv_heads))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: heads must be a multiple of kv_heads", what);
+  return 0;
+}
+
+extern "C" int iree_amd_uk_attention_kv4(
+    const void* q, iree_amd_uk_index_t q_stride0, void* out, iree_amd_uk_index_t out_stride0, const void* cache,
+    iree_amd_uk_index_t pages, iree_amd_uk_index_t page_stride, int32_t page_size, const int32_t* page_table,
+    iree_amd_uk_index_t page_table_stride, iree_amd_uk_index_t max_pages, const int32_t* q_starts, const int32_t* kv_lens,
+    iree_amd_uk_index_t tokens, iree_amd_uk_index_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale,
+    iree_amd_uk_index_t window, iree_amd_uk_index_t sinks, iree_amd_uk_index_t max_kv_len, void* workspace,
+    uint64_t workspace_bytes, uint32_t flags, void* stream) {
+  const char* what = "attention_kv4";
+  UK_RETURN_IF_ERROR(validate_rows(what, flags, 0, kv_heads, head_dim));
+  UK_RETURN_IF_ERROR(validate_attention_sizes(what, tokens, batch, heads, kv_heads, window, sinks, max_kv_len));
+  if (tokens == 0 || batch == 0 || heads == 0) return 0;
+  AttentionKv4Args a{};
+  UK_RETURN_IF_ERROR(make_pool(what, cache, pages, page_stride, page_size, kv_heads, head_dim, &a.pool));
+  if (max_pages < 0 || max_pages > 0x7FFFFFFF || page_table_stride < 0 || (batch > 1 && page_table_stride < max_pages))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: page table stride below max_pages, or a negative one", what);
+  if ((!page_table && max_pages) || !q_starts || !kv_lens)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null page_table, q_starts or kv_lens", what);
+  if (!(scale - scale == 0.f)) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: scale is not finite", what);
+  UK_RETURN_IF_ERROR(validate_row_buffer(what, "q", q, q_stride0, tokens, heads, head_dim));
+  UK_RETURN_IF_ERROR(validate_row_buffer(what, "out", out, out_stride0, tokens, heads, head_dim));
+  if (workspace_bytes && (!workspace || !aligned16(workspace)))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: the workspace is null or not 16-byte aligned", what);
+  a.q = q, a.out = out, a.q_stride = q_stride0, a.out_stride = out_stride0;
+  a.page_table = page_table, a.page_table_stride = page_table_stride, a.max_pages = max_pages;
+  a.q_starts = q_starts, a.kv_lens = kv_lens, a.tokens = tokens, a.batch = batch;
+  a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
+  // (no key lies past 2^31 pages of 256; the limits keep sums of a position and these in range)
+  a.window = window < (1ll << 40) ? window : 0;
+  a.sinks = sinks < (1ll << 40) ? sinks : 1ll << 40;
+  const int64_t capacity = max_pages << a.pool.page_shift;
+  a.max_kv_len = max_kv_len && max_kv_len < capacity ? max_kv_len : capacity;
+  a.workspace = workspace, a.workspace_bytes = workspace ? workspace_bytes : 0;
+  a.bf16 = (flags & IREE_AMD_UK_FLAG_ATTENTION_TYPE_MASK) == IREE_AMD_UK_FLAG_ATTENTION_TYPE_BF16;
+  return launch_attention_kv4(a, (hipStream_t)stream);
+}
+
+extern "C" int iree_amd_uk_attention_kv4_workspace(iree_amd_uk_index_t tokens, iree_amd_uk_index_t batch, int32_t heads,
+                                                  int32_t kv_heads, int32_t head_dim, iree_amd_uk_index_t window,
+                                                  iree_amd_uk_index_t sinks, iree_amd_uk_index_t max_kv_len,
+                                                  uint64_t* out_bytes) {
+  const char* what = "attention_kv4_workspace";
+  UK_RETURN_IF_ERROR(validate_rows(what, IREE_AMD_UK_FLAG_ATTENTION_TYPE_F16, 0, kv_heads, head_dim));
+  UK_RETURN_IF_ERROR(validate_attention_sizes(what, tokens, batch, heads, kv_heads, window, sinks, max_kv_len));
+  if (!out_bytes) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null result", what);
+  *out_bytes = tokens && batch && heads
+                   ? attention_kv4_workspace(tokens, batch, heads, kv_heads, head_dim, window, sinks, max_kv_len)
+                   : 0;
+  return 0;
+}
+
+extern "C" int iree_amd_uk_copy_pages(void* pool, iree_amd_uk_index_t pages, iree_amd_uk_index_t page_bytes,
+                                     iree_amd_uk_index_t page_stride, const int32_t* src, const int32_t* dst,
+                                     iree_amd_uk_index_t count, void* stream) {
+  const char* what = "copy_pages";
+  if (pages < 0 || pages > 0x7FFFFFFF || page_bytes < 0 || count < 0 || page_stride < page_bytes || page_bytes % 16 ||
+      page_stride % 16 || page_stride > (INT64_MAX >> 1) / (pages + 1))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT,
+                "%s: pages, page_bytes and count are not negative, pages whole 16 bytes long and apart", what);
+  if (count == 0) return 0;
+  if (!src || !dst) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null src or dst", what);
+  for (int64_t i = 0; i < count; ++i)
+    if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages)
+      return fail(IREE_AMD_UK_STATUS_OUT_OF_RANGE, "%s: pair %lld (%d to %d) outside the pool's %lld pages", what,
+                  (long long)i, src[i], dst[i], (long long)pages);
+  // One bit a page: written. (calloc's zero pages cost nothing until they are touched.)
+  uint8_t* written = (uint8_t*)calloc((size_t)(pages / 8 + 1), 1);
+  if (!written) return fail(8, "%s: no host memory for %lld pages", what, (long long)pages);
+  int64_t bad = -1;
+  for (int64_t i = 0; i < count && bad < 0; ++i) {
+    if (written[dst[i] / 8] >> (dst[i] % 8) & 1) bad = i;
+    written[dst[i] / 8] |= (uint8_t)(1 << (dst[i] % 8));
+  }
+  for (int64_t i = 0; i < count && bad < 0; ++i)
+    if (written[src[i] / 8] >> (src[i] % 8) & 1) bad = i;
+  free(written);
+  if (bad >= 0)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: pair %lld (%d to %d): a page is written twice, or written and read",
+                what, (long long)bad, src[bad], dst[bad]);
+  if (page_bytes == 0) return 0;
+  if (!pool || !aligned16(pool)) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: the pool is null or not 16-byte aligned", what);
+  return launch_copy_pages(pool, page_bytes, page_stride, src, dst, count, (hipStream_t)stream);
 }
 
 extern "C" int iree_amd_uk_scale_f32(void* buf_f32, iree_amd_uk_index_t n, float scale,

@@ -270,6 +270,59 @@ int launch_silu_mul_quantize_tiled(const void* acc, int64_t acc_stride0, int64_t
                                    int64_t up_tile0, void* out, int64_t out_stride0, int64_t M1,
                                    int64_t N1, float gate_scale, float up_scale,
                                    float inv_out_scale, hipStream_t s);
+// Geometry of a 4-bit cache (uk_kv4.h) and its operators.
+struct Kv4Pool {
+  char* base;
+  int64_t pages, page_stride;
+  int page_shift;            // log2 of the tokens of a page
+};
+struct QkNormRopeArgs {
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+  const void *q_weight, *k_weight;
+  float eps;
+  const float* cos_sin;
+  int64_t table_rows;
+  int rotary;
+  const int32_t* positions;
+  Kv4Pool pool;              // base null: no cache
+  const int64_t* slots;
+  int64_t tokens;
+  int heads, kv_heads, dim;
+  bool interleaved, bf16;
+};
+int launch_qk_norm_rope(const QkNormRopeArgs& a, hipStream_t s);
+struct Kv4ReadArgs {
+  Kv4Pool pool;
+  const int64_t* slots;
+  void *k_out, *v_out;
+  int64_t k_out_stride, v_out_stride, rows;
+  int kv_heads, dim;
+  bool bf16;
+};
+int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s);
+struct AttentionKv4Args {
+  const void* q;
+  void* out;
+  int64_t q_stride, out_stride;
+  Kv4Pool pool;
+  const int32_t* page_table;
+  int64_t page_table_stride, max_pages;
+  const int32_t *q_starts, *kv_lens;
+  int64_t tokens, batch;
+  int heads, kv_heads, dim;
+  float scale;
+  int64_t window, sinks, max_kv_len;
+  void* workspace;
+  uint64_t workspace_bytes;
+  bool bf16;
+};
+int launch_attention_kv4(const AttentionKv4Args& a, hipStream_t s);
+uint64_t attention_kv4_workspace(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int64_t window,
+                                 int64_t sinks, int64_t max_kv_len);
+int launch_copy_pages(void* pool, int64_t page_bytes, int64_t page_stride, const int32_t* src, const int32_t* dst,
+                      int64_t count, hipStream_t s);
 int launch_scale_f32(void* buf, int64_t n, float scale, hipStream_t s);
 int launch_mfma_probe(uint32_t type_flag, const void* operands, int64_t iters, void* sink,
                       int64_t* out_ops_per_launch, hipStream_t s);

@@ -1,0 +1,64 @@
+// Layout of a block of the 4-bit cache (one kv head of one page, include/iree_amd_uk.h),
+// and conversions between the rows' types and f32. Device code and sizes only.
+#ifndef IREE_AMD_CSRC_UK_KV4_H_
+#define IREE_AMD_CSRC_UK_KV4_H_
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace uk {
+namespace kv4 {
+
+// Byte offsets inside a block of `page` tokens of D values.
+template <int D>
+struct Block {
+  __host__ __device__ static constexpr int64_t bytes(int page) { return (int64_t)page * (D + 8); }
+  __device__ static int k_row(int row) { return row * (D / 2); }
+  // The dword of V that holds d = 8 * i .. 8 * i + 7 of a row.
+  __device__ static int v_dword(int page, int row, int i) {
+    return page * (D / 2) + (((row >> 2) * (D / 8) + i) * 4 + (row & 3)) * 4;
+  }
+  __device__ static int k_params(int page, int row) { return page * D + row * 4; }
+  __device__ static int v_params(int page, int row) { return page * (D + 4) + row * 4; }
+};
+
+// One row value. (bf16 is handled as bits: widening is a shift, narrowing rounds to the
+// nearest, ties to even, and keeps NaN.)
+struct F16 {
+  typedef uint16_t bits;
+  __device__ static float widen(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (uint16_t)b); }
+  __device__ static uint32_t narrow(float f) {
+    // (a value that comes from 64 bits is rounded here from its 32: contracted, the two
+    // roundings would become one, for this type and not for the other)
+#pragma clang fp contract(off)
+    return __builtin_bit_cast(uint16_t, (_Float16)f);
+  }
+};
+struct BF16 {
+  typedef uint16_t bits;
+  __device__ static float widen(uint32_t b) { return __builtin_bit_cast(float, b << 16); }
+  __device__ static uint32_t narrow(float f) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, f);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (u >> 16) | 0x40u;
+    return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+  }
+};
+
+template <typename T>
+__device__ inline void widen4(uint2 w, float* x) {
+  x[0] = T::widen(w.x & 0xFFFFu);
+  x[1] = T::widen(w.x >> 16);
+  x[2] = T::widen(w.y & 0xFFFFu);
+  x[3] = T::widen(w.y >> 16);
+}
+template <typename T>
+__device__ inline uint2 narrow4(const float* x) {
+  return make_uint2(T::narrow(x[0]) | (T::narrow(x[1]) << 16), T::narrow(x[2]) | (T::narrow(x[3]) << 16));
+}
+
+}  // namespace kv4
+}  // namespace uk
+
+#endif  // IREE_AMD_CSRC_UK_KV4_H_

@@ -109,6 +109,10 @@ PyMethodDef g_entries[] = {
     UK_ENTRY(iree_amd_uk_silu_mul_quantize_tiled),
     UK_ENTRY(iree_amd_uk_mmt4d_silu_mul_f8e4m3),
     UK_ENTRY(iree_amd_uk_scale_f32),
+    UK_ENTRY(iree_amd_uk_qk_norm_rope),
+    UK_ENTRY(iree_amd_uk_kv4_read),
+    UK_ENTRY(iree_amd_uk_attention_kv4),
+    UK_ENTRY(iree_amd_uk_copy_pages),
     {"iree_amd_uk_query_matmul_tile_sizes", (PyCFunction)(void (*)(void))query, METH_FASTCALL, nullptr},
 };
 
