@@ -1048,9 +1048,9 @@ extern "C" int iree_amd_uk_attention_kv4(
   a.page_table = page_table, a.page_table_stride = page_table_stride, a.max_pages = max_pages;
   a.q_starts = q_starts, a.kv_lens = kv_lens, a.tokens = tokens, a.batch = batch;
   a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
-  // (no key lies past 2^31 pages of 256; the limits keep sums of a position and these in range)
-  a.window = window < (1ll << 40) ? window : 0;
-  a.sinks = sinks < (1ll << 40) ? sinks : 1ll << 40;
+  // (positions lie below 2^31)
+  a.window = window < 0x7FFFFFFF ? window : 0;
+  a.sinks = sinks < 0x7FFFFFFF ? sinks : 0x7FFFFFFF;
   const int64_t capacity = max_pages << a.pool.page_shift;
   a.max_kv_len = max_kv_len && max_kv_len < capacity ? max_kv_len : capacity;
   a.workspace = workspace, a.workspace_bytes = workspace ? workspace_bytes : 0;
