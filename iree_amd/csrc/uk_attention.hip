@@ -104,7 +104,19 @@ __device__ inline float across_sum(float v) {
 // ---------------------------------------------------------------------------
 
 constexpr int kTile = 32;      // keys a wave takes at a time
-constexpr int kWaves = 4;      // of a workgroup; they take the tiles of its range in turn
+#ifndef WPE
+#define WPE 2
+#endif
+#ifndef NWV
+#define NWV 4
+#endif
+#ifndef WANT
+#define WANT 4
+#endif
+#ifndef MINC
+#define MINC 16
+#endif
+constexpr int kWaves = NWV;      // of a workgroup; they take the tiles of its range in turn
 constexpr int kRows = 16;
 
 // Exponents: weights p = 2^(t) with t <= kLazy above the row's reference, which is only
@@ -138,35 +150,62 @@ struct KvTile {
   uint4 kp[2], vp[2];
 };
 
+// A lane's places in the 16 rows that one half of a tile reads; everything else of an
+// address is the same for the wave.
 template <int D>
-__device__ inline void load_half(KvTile<D>& t, int half, const char* block, int page, int row, int n, int g) {
-  constexpr int S = KvTile<D>::S, C = KvTile<D>::C;
-  const char* k = block + Block<D>::k_row(row + n) + g * (S * 4);
-  if constexpr (S == 2) {
-    const uint2 w = *(const uint2*)k;
-    t.k[half][0] = w.x, t.k[half][1] = w.y;
-  } else {
+struct LaneAt {
+  uint32_t k, v, p;
+  __device__ LaneAt(int n, int g) {
+    k = n * (D / 2) + g * (D / 8);
+    v = g * (D / 8) * 16 + (D >= 128 ? n : n & 7) * 16;
+    p = g * 16;
+  }
+};
+
+// A tile's keys and where its halves, 16 keys apart, lie; pages clamped into the pool.
+struct TileAt {
+  int key;
+  int page[2];           // -1 and others outside the pool: no keys
+  const char* block[2];  // the kv head's block
+  int row[2];
+};
+
+template <int D>
+__device__ inline void load_k(KvTile<D>& t, const TileAt& w, const LaneAt<D>& at) {
 #pragma unroll
-    for (int i = 0; i < S / 4; ++i) {
-      const uint4 w = ((const uint4*)k)[i];
-      t.k[half][4 * i] = w.x, t.k[half][4 * i + 1] = w.y, t.k[half][4 * i + 2] = w.z, t.k[half][4 * i + 3] = w.w;
+  for (int half = 0; half < 2; ++half) {
+    const char* k = w.block[half] + Block<D>::k_row(w.row[half]) + at.k;
+    if constexpr (D == 64) {
+      const uint2 v = *(const uint2*)k;
+      t.k[half][0] = v.x, t.k[half][1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 128; ++i) {
+        const uint4 v = *(const uint4*)(k + 16 * i);
+        t.k[half][4 * i] = v.x, t.k[half][4 * i + 1] = v.y, t.k[half][4 * i + 2] = v.z, t.k[half][4 * i + 3] = v.w;
+      }
     }
   }
-  const char* v = block + page * (D / 2) + ((row >> 2) + g) * (D / 8) * 16;
-#pragma unroll
-  for (int c = 0; c < C; ++c) t.v[half][c] = *(const uint4*)(v + ((D >= 128 ? n : n & 7) + 16 * c) * 16);
-  t.kp[half] = *(const uint4*)(block + Block<D>::k_params(page, row + 4 * g));
-  t.vp[half] = *(const uint4*)(block + Block<D>::v_params(page, row + 4 * g));
 }
-
-// Two halves 16 keys apart; `page0`, `page1`: their pages, clamped into the pool.
 template <int D>
-__device__ inline void load_tile(KvTile<D>& t, const AttentionKv4Args& a, int key, int page0, int page1, int head, int n,
-                                 int g) {
-  const int page = 1 << a.pool.page_shift;
-  const int64_t at = head * Block<D>::bytes(page);
-  load_half<D>(t, 0, a.pool.base + page0 * a.pool.page_stride + at, page, key & (page - 1), n, g);
-  load_half<D>(t, 1, a.pool.base + page1 * a.pool.page_stride + at, page, (key + 16) & (page - 1), n, g);
+__device__ inline void load_kp(KvTile<D>& t, const TileAt& w, const LaneAt<D>& at, int page) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+    t.kp[half] = *(const uint4*)(w.block[half] + Block<D>::k_params(page, w.row[half]) + at.p);
+}
+template <int D>
+__device__ inline void load_vp(KvTile<D>& t, const TileAt& w, const LaneAt<D>& at, int page) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+    t.vp[half] = *(const uint4*)(w.block[half] + Block<D>::v_params(page, w.row[half]) + at.p);
+}
+template <int D>
+__device__ inline void load_v(KvTile<D>& t, const TileAt& w, const LaneAt<D>& at, int page) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int c = 0; c < KvTile<D>::C; ++c)
+      t.v[half][c] = *(const uint4*)(w.block[half] + Block<D>::v_dword(page, w.row[half], 0) + at.v + 256 * c);
 }
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -175,6 +214,8 @@ union Frag {
   half2v h[4];
   half8 f;
 };
+
+__device__ inline half2v as_half2(uint32_t u) { return __builtin_bit_cast(half2v, u); }
 
 // A dword of K codes as 8 f16 subnormals (products and sums are exact all the same): nibbles
 // 0, 4, 1, 5, 2, 6, 3, 7, the odd ones 16 times too large, which the queries take back.
@@ -196,11 +237,11 @@ __device__ inline uint32_t pair_bytes(uint32_t first, uint32_t second) {
 // mantissa, exactly.
 __device__ inline half2v low_codes(uint32_t x) {
   const uint32_t u = (x & 0x000F000Fu) | 0x64006400u;
-  return __builtin_bit_cast(half2v, u) - (half2v)(_Float16)1032.f;
+  return as_half2(u) - (half2v)(_Float16)1032.f;
 }
 __device__ inline half2v high_codes(uint32_t x) {
   const uint32_t u = (x & 0x00F000F0u) | 0x54005400u;
-  return __builtin_bit_cast(half2v, u) - (half2v)(_Float16)72.f;
+  return as_half2(u) - (half2v)(_Float16)72.f;
 }
 
 __device__ inline uint32_t dword(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
@@ -213,7 +254,7 @@ __device__ inline uint32_t dword(const uint4& v, int i) { return i == 0 ? v.x : 
 // with a running softmax of its own; they join through LDS at the end. The next tile is
 // requested before the current one is used.
 template <int D, typename T>
-__global__ __launch_bounds__(64 * kWaves) void attention_kv4_split_kernel(SplitArgs args) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE))) void attention_kv4_split_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
   constexpr int S = KvTile<D>::S, C = KvTile<D>::C;
   constexpr int NI = D / 16;                       // accumulators of O
@@ -225,7 +266,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kv4_split_kernel(SplitA
   const int64_t slot = blockIdx.x / a.kv_heads;
   const Rows rows = find_rows(a, slot, G, kRows);
   if (rows.b < 0) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int last_row = rows.count - 1 < rows.first + kRows - 1 ? rows.count - 1 : rows.first + kRows - 1;
   const int lo_pos = position(rows, rows.first / G), hi_pos = position(rows, last_row / G);
   const Keys<kTile> keys(a, lo_pos, hi_pos);
@@ -282,58 +323,99 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kv4_split_kernel(SplitA
   const int32_t* table = a.page_table + rows.b * a.page_table_stride;
   const int shift = a.pool.page_shift;
 
-  auto page_of = [&](int key) -> int {
-    const int at = key >> shift;
-    return at < a.max_pages ? table[at] : -1;
+  const int page_size = 1 << shift, pages = (int)a.pool.pages, wide = (int)a.max_pages;
+  const char* base = a.pool.base + head * Block<D>::bytes(page_size);
+  // What the lane's row sees: keys up to pos, of them those past `below` and the sinks.
+  const int below = a.window ? pos - (int)a.window : -1, sinks = a.window ? (int)a.sinks : 0;
+  auto locate = [&](int tile) {
+    TileAt w;
+    w.key = keys.key(tile);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int key = w.key + 16 * half, i = key >> shift;
+      w.page[half] = i < wide ? table[i] : -1;
+      w.row[half] = key & (page_size - 1);
+    }
+    return w;
   };
-  auto clamp_page = [&](int p) { return (unsigned)p < (unsigned)a.pool.pages ? p : 0; };
+  // (once the page numbers are needed: they have had a tile's time to arrive)
+  auto resolve = [&](TileAt& w) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int p = (unsigned)w.page[half] < (unsigned)pages ? w.page[half] : 0;
+      w.block[half] = base + p * a.pool.page_stride;
+    }
+  };
 
-  auto use = [&](const KvTile<D>& t, int key, int page0, int page1) {
+  const LaneAt<D> at(n, g);
+  KvTile<D> t;
+  TileAt now, next;
+  int tile = begin + wave;
+  if (tile < end) {
+    now = locate(tile);
+    resolve(now);
+    load_k<D>(t, now, at);
+    load_kp<D>(t, now, at, page_size);
+    load_vp<D>(t, now, at, page_size);
+    load_v<D>(t, now, at, page_size);
+    next = locate(tile + kWaves < end ? tile + kWaves : tile);
+  }
+  // Each part of a tile is requested again, for the wave's next tile, as soon as it has been
+  // used: one tile is in flight at any time, in the registers of one. (The last tile requests
+  // itself once more.)
+  for (; tile < end; tile += kWaves) {
+    const int key = now.key;
+    const bool exist0 = (unsigned)now.page[0] < (unsigned)pages, exist1 = (unsigned)now.page[1] < (unsigned)pages;
+    resolve(next);
     floatx4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       s0 = F16Cfg16::mfma(k_frag(t.k[0][i]), qf[i].f, s0);
       s1 = F16Cfg16::mfma(k_frag(t.k[1][i]), qf[i].f, s1);
     }
-    float w[8], x[8], sv[8], mv[8];
+    load_k<D>(t, next, at);
+    __builtin_amdgcn_sched_barrier(0);
+    float w[8], x[8];
+    uint32_t vp[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t kp = dword(t.kp[j >> 2], j & 3), vp = dword(t.vp[j >> 2], j & 3);
+      const uint32_t kp = dword(t.kp[j >> 2], j & 3);
       w[j] = fmaf(F16::widen(kp & 0xFFFFu), j < 4 ? s0[j & 3] : s1[j & 3], F16::widen(kp >> 16) * qsum);
       x[j] = fmaf(w[j], f, -ref);
-      sv[j] = F16::widen(vp & 0xFFFFu);
-      mv[j] = fmaf(sv[j], 8.f, F16::widen(vp >> 16));
+      vp[j] = dword(t.vp[j >> 2], j & 3);
     }
-    // Every row sees the whole tile, or each looks at each key.
-    const bool exist = (unsigned)page0 < (unsigned)a.pool.pages && (unsigned)page1 < (unsigned)a.pool.pages;
-    const bool whole = exist && key + kTile <= lo_pos + 1 &&
-                       (!a.window || key > hi_pos - a.window || key + kTile <= a.sinks);
+    load_kp<D>(t, next, at, page_size);
+    load_vp<D>(t, next, at, page_size);
+    // Every row sees the whole tile, or each looks at each key: one it does not see has no
+    // weight, and no scale or offset, which may be NaN there.
+    const bool whole = exist0 && exist1 && key + kTile <= lo_pos + 1 &&
+                       (!a.window || key > hi_pos - (int)a.window || key + kTile <= sinks);
     uint32_t seen = 0xFF;
     if (!whole) {
       seen = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = key + 16 * (j >> 2) + 4 * g + (j & 3);
-        const int page = j < 4 ? page0 : page1;
-        const bool yes = k <= pos && (!a.window || k > pos - a.window || k < a.sinks) &&
-                         (unsigned)page < (unsigned)a.pool.pages;
+        const bool yes = (j < 4 ? exist0 : exist1) & (k <= pos) & ((k > below) | (k < sinks));
         seen |= yes ? 1u << j : 0u;
         x[j] = yes ? x[j] : -INFINITY;
-        sv[j] = yes ? sv[j] : 0.f;
-        mv[j] = yes ? mv[j] : 0.f;
+        vp[j] = yes ? vp[j] : 0u;
       }
     }
     const float top = fmaxf(max4(x[0], x[1], x[2], x[3]), max4(x[4], x[5], x[6], x[7]));
-    const float stop = fmaxf(max4(sv[0], sv[1], sv[2], sv[3]), max4(sv[4], sv[5], sv[6], sv[7]));
+    half2v smost = as_half2(vp[0]);                 // (scales are not negative, and the low halves)
+#pragma unroll
+    for (int j = 1; j < 8; ++j) smost = __builtin_elementwise_max(smost, as_half2(vp[j]));
+    const float stop = (float)smost[0];
     if (__ballot(top > kLazy || stop * vscale >= kScaleMost || vscale == 0.f)) {
       float most = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 8; ++j) most = fmaxf(most, seen >> j & 1 ? w[j] * f : -INFINITY);
-      const float now = fmaxf(ref, across_max(most));
-      float factor = exp2f(ref - now);
+      const float raised = fmaxf(ref, across_max(most));
+      float factor = exp2f(ref - raised);
       l *= factor;
       bias *= factor;
-      ref = now;
+      ref = raised;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = seen >> j & 1 ? fmaf(w[j], f, -ref) : -INFINITY;
       float smax = stop;
@@ -349,13 +431,15 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kv4_split_kernel(SplitA
     Frag hi, lo;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
+      const half2v sm = as_half2(vp[j]);
       const float p = __builtin_amdgcn_exp2f(x[j]);
       l += p;
-      bias = fmaf(p, mv[j], bias);
-      const float weight = p * (sv[j] * vscale);
+      bias = fmaf(p, fmaf((float)sm[0], 8.f, (float)sm[1]), bias);
+      const float weight = p * ((float)sm[0] * vscale);
       hi.f[j] = (_Float16)weight;
       if constexpr (kExact) lo.f[j] = (_Float16)(weight - (float)hi.f[j]);
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       uint32_t d[8];
@@ -387,34 +471,9 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kv4_split_kernel(SplitA
       byte(std::integral_constant<int, 2>{});
       byte(std::integral_constant<int, 3>{});
     }
-  };
-
-  // Two tiles in turn: while one is used the next of this wave is on its way.
-  KvTile<D> even, odd;
-  int tile = begin + wave;
-  int key0 = 0, p00 = -1, p01 = -1, key1 = 0, p10 = -1, p11 = -1;
-  if (tile < end) {
-    key0 = keys.key(tile);
-    p00 = page_of(key0), p01 = page_of(key0 + 16);
-    load_tile<D>(even, a, key0, clamp_page(p00), clamp_page(p01), head, n, g);
-  }
-  while (tile < end) {
-    const bool more = tile + kWaves < end;
-    if (more) {
-      key1 = keys.key(tile + kWaves);
-      p10 = page_of(key1), p11 = page_of(key1 + 16);
-      load_tile<D>(odd, a, key1, clamp_page(p10), clamp_page(p11), head, n, g);
-    }
-    use(even, key0, p00, p01);
-    if (!more) break;
-    tile += kWaves;
-    if (tile + kWaves < end) {
-      key0 = keys.key(tile + kWaves);
-      p00 = page_of(key0), p01 = page_of(key0 + 16);
-      load_tile<D>(even, a, key0, clamp_page(p00), clamp_page(p01), head, n, g);
-    }
-    use(odd, key1, p10, p11);
-    tile += kWaves;
+    load_v<D>(t, next, at, page_size);
+    now = next;
+    next = locate(tile + 2 * kWaves < end ? tile + 2 * kWaves : tile);
   }
 
   // Join the waves: everything relative to the largest reference.
@@ -516,9 +575,9 @@ Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int64_t windo
   if (keys > 0x7FFFFFFF) keys = 0x7FFFFFFF;
   const int64_t key_tiles = ceil_div(keys, kTile);
   const int64_t units = (tokens * G / kRows < batch ? batch : tokens * G / kRows) * kv_heads;
-  const int64_t wanted = 4ll * device_cu_count();
+  const int64_t wanted = 1ll * WANT * device_cu_count();
   int64_t chunk = ceil_div(key_tiles * units, wanted);
-  chunk = ceil_div(chunk < 16 ? 16 : chunk, kWaves) * kWaves;
+  chunk = ceil_div(chunk < MINC ? MINC : chunk, kWaves) * kWaves;
   p.chunk = (int)chunk;
   p.splits = (int)ceil_div(key_tiles < 1 ? 1 : key_tiles, chunk);
   if (p.splits > 1024) {
