@@ -7,9 +7,9 @@
 //   sum_j p_j v_j = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (m_j + 8 s_j)
 // so the matrix cores multiply the codes themselves, which f16 holds exactly, and each
 // key costs two multiply-adds for its scale and offset instead of a dequantised row. The
-// codes of V are centred because the sum over a long sequence is small next to its parts:
-// of uncentred codes and offsets the f32 sums would cancel (measured at 131072 keys in one
-// chain: 1.9e-3 of the result).
+// codes of V are centred, because the sum over a long sequence is small next to its parts
+// and the matrix cores cut off what does not fit the sum: 131072 keys, 6.4e-4 of the result
+// with codes from 0, 2.1e-4 (the result's own rounding) with these.
 #include "uk_common.h"
 #include "uk_kv4.h"
 #include "uk_mfma_cfg.h"
@@ -31,41 +31,46 @@ struct Rows {
   int first;         // first row of the tile
   int count;         // rows of the sequence
   int tokens;        // its query tokens
-  int64_t token0;    // its first token
-  int64_t kv_len;
+  int token0;        // its first token
+  int kv_len;
 };
 
 // The sequence of tile `slot`: the last b whose first tile is at most it. 64 lanes look at
-// 64 sequences at a time, so a batch of up to 64 costs one load.
+// 64 sequences at a time, with all that is asked of them, so a batch of up to 64 costs one
+// memory latency.
 __device__ inline Rows find_rows(const AttentionKv4Args& a, int64_t slot, int G, int R) {
   const int lane = threadIdx.x & 63;
   int64_t lo = 0, n = a.batch;                      // candidates [lo, lo + n)
-  while (n > 1) {
+  while (n > 64) {
     const int64_t step = (n + 63) / 64;
     const int64_t b = lo + lane * step;
-    const bool mine = b < lo + n && (int64_t)a.q_starts[b] * G / R + b <= slot;
-    const uint64_t yes = __ballot(mine);
-    const int last = yes ? 63 - __builtin_clzll(yes) : 0;
-    const int64_t from = lo + last * step;
+    const uint64_t yes = __ballot(b < lo + n && (int64_t)a.q_starts[b < lo + n ? b : lo] * G / R + b <= slot);
+    const int64_t from = lo + (yes ? 63 - __builtin_clzll(yes) : 0) * step;
     n = from + step < lo + n ? step : lo + n - from;
     lo = from;
   }
+  const int64_t b = lo + (lane < n ? lane : n - 1);
+  const int start = a.q_starts[b], next = a.q_starts[b + 1], len = a.kv_lens[b];
+  const uint64_t yes = __ballot(lane < n && (int64_t)start * G / R + b <= slot);
+  const int last = yes ? 63 - __builtin_clzll(yes) : 0;
+  const int from = __builtin_amdgcn_readlane(start, last), to = __builtin_amdgcn_readlane(next, last);
+  const int64_t first = (slot - ((int64_t)from * G / R + lo + last)) * R;
+  const int64_t rows = ((int64_t)to - from) * G;
+  const bool mine = from >= 0 && to <= a.tokens && first >= 0 && first < rows;
+  // (the same in all lanes, which the compiler is told: all addresses follow from them)
   Rows r;
-  const int64_t start = a.q_starts[lo], next = a.q_starts[lo + 1];
-  const int64_t first = (slot - (start * G / R + lo)) * R;
-  const int64_t rows = (next - start) * G;
-  r.b = start >= 0 && next <= a.tokens && first >= 0 && first < rows ? (int)lo : -1;
-  r.first = (int)first;
-  r.count = (int)rows;
-  r.tokens = (int)(next - start);
-  r.token0 = start;
-  r.kv_len = a.kv_lens[lo];
+  r.b = __builtin_amdgcn_readfirstlane(mine ? (int)(lo + last) : -1);
+  r.first = __builtin_amdgcn_readfirstlane((int)first);
+  r.count = __builtin_amdgcn_readfirstlane((int)rows);
+  r.tokens = __builtin_amdgcn_readfirstlane(to - from);
+  r.token0 = __builtin_amdgcn_readfirstlane(from);
+  r.kv_len = __builtin_amdgcn_readlane(len, last);
   return r;
 }
 
 // Position of a query token: below 0 where it sees nothing.
 __device__ inline int position(const Rows& r, int token) {
-  const int64_t p = r.kv_len - r.tokens + token;
+  const int64_t p = (int64_t)r.kv_len - r.tokens + token;
   return p < 0 ? -1 : (int)p;
 }
 
@@ -104,27 +109,15 @@ __device__ inline float across_sum(float v) {
 // ---------------------------------------------------------------------------
 
 constexpr int kTile = 32;      // keys a wave takes at a time
-#ifndef WPE
-#define WPE 2
-#endif
-#ifndef NWV
-#define NWV 4
-#endif
-#ifndef WANT
-#define WANT 4
-#endif
-#ifndef MINC
-#define MINC 16
-#endif
-constexpr int kWaves = NWV;      // of a workgroup; they take the tiles of its range in turn
+constexpr int kWaves = 4;      // of a workgroup; they take the tiles of its range in turn
 constexpr int kRows = 16;
+constexpr int kMaxSplits = 1024;
 
-// Exponents: weights p = 2^(t) with t <= kLazy above the row's reference, which is only
-// moved when a score passes that; p s is carried in f16 times 2^-E, E moved when a scale
-// passes 2^kScaleMost of it: p s 2^-E stays below 2^15, and what is dropped at the other end
-// lies 2^-32 below the largest scale.
-constexpr float kLazy = 4.f;
-constexpr float kScaleMost = 2048.f;
+// A row's weights p = 2^(score - ref) are carried against a reference that is only moved
+// when p s leaves the range of f16: it is set so that the largest score and the largest scale
+// of V together give 2^kTarget, and moved when they would give 2^kMost. What is dropped at the
+// other end lies 2^-31 below the largest p s. A scale counts as at least 2^-24 (it may be 0).
+constexpr int kTarget = 7, kMost = 13;
 
 // Partial results of a split: per (tile, kv head, split) O [16][D], reference [16], sum [16].
 template <int D>
@@ -141,73 +134,47 @@ __device__ inline int active_splits(const SplitArgs& s, int total) {
   return n < 1 ? 1 : n < s.splits ? n : s.splits;
 }
 
+// A key tile on its way through LDS, in the order in which the lanes read it: for each of
+// its two halves of 16 keys the K codes [D / 128][64 lanes][16 bytes] (D = 64: [64][8]), the
+// V codes likewise, then K and V parameters [2][16 keys].
 template <int D>
-struct KvTile {
-  static constexpr int S = D / 32;              // dwords of a K row in a lane: MFMA steps
-  static constexpr int C = D >= 128 ? D / 128 : 1;
-  uint32_t k[2][S];
-  uint4 v[2][C];
-  uint4 kp[2], vp[2];
+struct TileLds {
+  static constexpr int kCodes = 8 * D;              // bytes of 16 keys' K (V) codes
+  static constexpr int kHalf = 2 * kCodes + 128;
+  static constexpr int kBytes = 2 * kHalf;
+  static constexpr int kLoads = 2 * (D == 64 ? 2 : 2 * (D / 128) + 1);
 };
 
-// A lane's places in the 16 rows that one half of a tile reads; everything else of an
-// address is the same for the wave.
+// One half straight into LDS: per instruction 64 (params: 8) lanes of 16 bytes.
 template <int D>
-struct LaneAt {
-  uint32_t k, v, p;
-  __device__ LaneAt(int n, int g) {
-    k = n * (D / 2) + g * (D / 8);
-    v = g * (D / 8) * 16 + (D >= 128 ? n : n & 7) * 16;
-    p = g * 16;
+__device__ inline void request_half(char* lds, const char* block, int page, int row, const uint32_t (&k_at)[2],
+                                    uint32_t p_at, int lane) {
+  typedef __attribute__((address_space(3))) void lds_t;
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)block, 0, 0x7FFFFFFF, 0x00020000);
+  const int codes = row * (D / 2), v_codes = codes + page * (D / 2);
+  if constexpr (D == 64) {
+    // (a wave's worth holds K in its first half, V in the second)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)lds, 16, k_at[0], codes, 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 128; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + 1024 * i), 16, k_at[0], codes + 16 * i, 0, 0);
+#pragma unroll
+    for (int i = 0; i < D / 128; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + TileLds<D>::kCodes + 1024 * i), 16, k_at[1],
+                                               v_codes + 256 * i, 0, 0);
   }
-};
-
-// A tile's keys and where its halves, 16 keys apart, lie; pages clamped into the pool.
-struct TileAt {
-  int key;
-  int page[2];           // -1 and others outside the pool: no keys
-  const char* block[2];  // the kv head's block
-  int row[2];
-};
-
-template <int D>
-__device__ inline void load_k(KvTile<D>& t, const TileAt& w, const LaneAt<D>& at) {
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const char* k = w.block[half] + Block<D>::k_row(w.row[half]) + at.k;
-    if constexpr (D == 64) {
-      const uint2 v = *(const uint2*)k;
-      t.k[half][0] = v.x, t.k[half][1] = v.y;
-    } else {
-#pragma unroll
-      for (int i = 0; i < D / 128; ++i) {
-        const uint4 v = *(const uint4*)(k + 16 * i);
-        t.k[half][4 * i] = v.x, t.k[half][4 * i + 1] = v.y, t.k[half][4 * i + 2] = v.z, t.k[half][4 * i + 3] = v.w;
-      }
-    }
-  }
-}
-template <int D>
-__device__ inline void load_kp(KvTile<D>& t, const TileAt& w, const LaneAt<D>& at, int page) {
-#pragma unroll
-  for (int half = 0; half < 2; ++half)
-    t.kp[half] = *(const uint4*)(w.block[half] + Block<D>::k_params(page, w.row[half]) + at.p);
-}
-template <int D>
-__device__ inline void load_vp(KvTile<D>& t, const TileAt& w, const LaneAt<D>& at, int page) {
-#pragma unroll
-  for (int half = 0; half < 2; ++half)
-    t.vp[half] = *(const uint4*)(w.block[half] + Block<D>::v_params(page, w.row[half]) + at.p);
-}
-template <int D>
-__device__ inline void load_v(KvTile<D>& t, const TileAt& w, const LaneAt<D>& at, int page) {
-#pragma unroll
-  for (int half = 0; half < 2; ++half)
-#pragma unroll
-    for (int c = 0; c < KvTile<D>::C; ++c)
-      t.v[half][c] = *(const uint4*)(w.block[half] + Block<D>::v_dword(page, w.row[half], 0) + at.v + 256 * c);
+  if (lane < 8)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + 2 * TileLds<D>::kCodes), 16, p_at, page * D + row * 4, 0, 0);
 }
 
+template <int N>
+__device__ inline void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 union Frag {
   uint32_t u[4];
@@ -217,8 +184,9 @@ union Frag {
 
 __device__ inline half2v as_half2(uint32_t u) { return __builtin_bit_cast(half2v, u); }
 
-// A dword of K codes as 8 f16 subnormals (products and sums are exact all the same): nibbles
-// 0, 4, 1, 5, 2, 6, 3, 7, the odd ones 16 times too large, which the queries take back.
+// A dword of K codes as 8 f16 subnormals, 2^-24 of their values (products and sums are exact
+// all the same): nibbles 0, 4, 1, 5, 2, 6, 3, 7, the odd ones 16 times too large, which the
+// queries take back.
 __device__ inline half8 k_frag(uint32_t w) {
   Frag f;
   f.u[0] = w & 0x000F000Fu;
@@ -233,18 +201,28 @@ template <int b>
 __device__ inline uint32_t pair_bytes(uint32_t first, uint32_t second) {
   return __builtin_amdgcn_perm(second, first, 0x0C040C00u | b | (b << 16));
 }
-// Both low (high) nibbles as centred f16 codes c - 8: 1024 + c (64 + c) by or-ing c into the
-// mantissa, exactly.
-__device__ inline half2v low_codes(uint32_t x) {
-  const uint32_t u = (x & 0x000F000Fu) | 0x64006400u;
-  return as_half2(u) - (half2v)(_Float16)1032.f;
-}
-__device__ inline half2v high_codes(uint32_t x) {
-  const uint32_t u = (x & 0x00F000F0u) | 0x54005400u;
-  return as_half2(u) - (half2v)(_Float16)72.f;
+// Tiles of a wave in LDS: the one in use and the one on its way. (Three, which leave room for
+// three workgroups on a compute unit instead of four: two caches of 131072 keys 58.6 us, with
+// two 56.0.)
+constexpr int kRing = 2;
+
+// LDS of a workgroup: the waves' rings, later their results; behind them the waves'
+// references and sums.
+template <int D>
+constexpr int split_lds_bytes() {
+  constexpr int ring = kWaves * kRing * TileLds<D>::kBytes, join = kWaves * kRows * (D + 4) * 4;
+  return (ring > join ? ring : join) + 2 * kWaves * kRows * 4;
 }
 
-__device__ inline uint32_t dword(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+// The low (high) nibbles of both halves as f16 c - 8: 1024 + c (64 + c) by or-ing c into the
+// mantissa, exactly. The or's constant comes in a register, or the and before it could not
+// be the same instruction.
+__device__ inline half2v low_codes(uint32_t x, uint32_t bias) {
+  return as_half2((x & 0x000F000Fu) | bias) - (half2v)(_Float16)1032.f;
+}
+__device__ inline half2v high_codes(uint32_t x, uint32_t bias) {
+  return as_half2((x & 0x00F000F0u) | bias) - (half2v)(_Float16)72.f;
+}
 
 // One kv head, 16 rows, the key tiles of one split. v_mfma_f32_16x16x32_f16 with the keys
 // as rows of the scores: a lane holds one query row and 8 of the 32 keys, its weights are
@@ -254,17 +232,19 @@ __device__ inline uint32_t dword(const uint4& v, int i) { return i == 0 ? v.x : 
 // with a running softmax of its own; they join through LDS at the end. The next tile is
 // requested before the current one is used.
 template <int D, typename T>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE))) void attention_kv4_split_kernel(SplitArgs args) {
+__global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
-  constexpr int S = KvTile<D>::S, C = KvTile<D>::C;
+  constexpr int S = D / 32;                        // matrix-core steps of a score
+  constexpr int C = D >= 128 ? D / 128 : 1;        // dwords of a V row in a lane
   constexpr int NI = D / 16;                       // accumulators of O
   constexpr bool kExact = __is_same(T, F16);
-  __shared__ float ref_s[kWaves][kRows], sum_s[kWaves][kRows];
-  __shared__ float o_s[kWaves][kRows][D + 4];
+  extern __shared__ __attribute__((aligned(1024))) char memory[];
+  float (*ref_s)[kRows] = (float (*)[kRows])(memory + split_lds_bytes<D>()) - 2 * kWaves;
+  float (*sum_s)[kRows] = ref_s + kWaves;
+  float (*o_s)[kRows][D + 4] = (float (*)[kRows][D + 4])memory;      // (once all tiles are used)
   const int G = args.group;
   const int head = blockIdx.x % a.kv_heads;
-  const int64_t slot = blockIdx.x / a.kv_heads;
-  const Rows rows = find_rows(a, slot, G, kRows);
+  const Rows rows = find_rows(a, blockIdx.x / a.kv_heads, G, kRows);
   if (rows.b < 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int last_row = rows.count - 1 < rows.first + kRows - 1 ? rows.count - 1 : rows.first + kRows - 1;
@@ -279,7 +259,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE
   // The lane's query row (rows past the sequence's last repeat it; they are not written).
   const int row = rows.first + n < last_row ? rows.first + n : last_row;
   const int pos = position(rows, row / G);
-  const uint16_t* q = (const uint16_t*)a.q + (rows.token0 + row / G) * a.q_stride + (int64_t)(head * G + row % G) * D +
+  const uint16_t* q = (const uint16_t*)a.q + (int64_t)(rows.token0 + row / G) * a.q_stride + (int64_t)(head * G + row % G) * D +
                       g * (D / 4);
   Frag qf[S];
   float f, qsum;
@@ -310,16 +290,15 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE
         const int nibble = (j >> 1) + 4 * (j & 1);
         qf[s].f[j] = (_Float16)ldexpf(x[8 * s + nibble], nibble & 1 ? e - 4 : e);
       }
-    // score log2(e) scale = f (s_k S + m_k qsum), S the product with codes of 2^-24
+    // score log2(e) scale = s_k f S + m_k qsum, S the product with codes of 2^-24
     f = ldexpf(fabsf(a.scale) * kLog2e, 24 - e);
-    qsum = ldexpf(sum, e - 24);
+    qsum = sum * (fabsf(a.scale) * kLog2e);
   }
 
   floatx4 o[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   float ref = -1e30f, l = 0.f, bias = 0.f;
-  float vscale = 0.f;             // 2^-E; 0 before the first scale
   const int32_t* table = a.page_table + rows.b * a.page_table_stride;
   const int shift = a.pool.page_shift;
 
@@ -327,65 +306,108 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE
   const char* base = a.pool.base + head * Block<D>::bytes(page_size);
   // What the lane's row sees: keys up to pos, of them those past `below` and the sinks.
   const int below = a.window ? pos - (int)a.window : -1, sinks = a.window ? (int)a.sinks : 0;
-  auto locate = [&](int tile) {
-    TileAt w;
-    w.key = keys.key(tile);
+  // Pages of the wave's next 32 tiles, a lane per half of a tile; -1 and others outside the
+  // pool: no keys. (An entry that is fetched when it is needed costs every tile its latency.)
+  int tile = begin + wave;
+  int pages_from = tile, page_ids = -1;
+  auto fetch_pages = [&](int from) {
+    const int t = from + (lane >> 1) * kWaves;
+    const int i = t < end ? (keys.key(t) + 16 * (lane & 1)) >> shift : wide;
+    pages_from = from;
+    page_ids = i < wide ? table[i] : -1;
+    asm volatile("" : "+v"(page_ids));     // (waited for here, not at each use)
+  };
+  auto page_at = [&](int t, int half) {
+    return __builtin_amdgcn_readlane(page_ids, (t - pages_from) / kWaves * 2 + half);
+  };
+  // Where a lane fetches from, so that what it reads from LDS is its own operand: K row n,
+  // bytes of group g; V dword n of the 4 keys of group g.
+  char* ring = memory + wave * kRing * TileLds<D>::kBytes;
+  uint32_t k_at[2], p_at;
+  if constexpr (D == 64) {
+    // (lanes 0..31 fetch K: chunk c of 16 bytes of row lane / 2; lanes 32.. V: 8 dwords of 4 keys a group)
+    k_at[0] = lane < 32 ? lane * 16 : (lane - 32) * 16 + page_size * (D / 2);
+    k_at[1] = 0;
+  } else {
+    k_at[0] = n * (D / 2) + g * (D / 8);
+    k_at[1] = g * (D / 8) * 16 + n * 16;
+  }
+  p_at = (lane & 3) * 16 + (lane >> 2) * page_size * 4;      // lanes 0..3 the K parameters, 4..7 those of V
+  // What has been requested: its first key, and whether the pages of its halves exist.
+  struct Tile {
+    int key, exist;
+  };
+  auto request = [&](int slot, int t) {
+    char* to = ring + slot * TileLds<D>::kBytes;
+    Tile w{keys.key(t), 0};
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int key = w.key + 16 * half, i = key >> shift;
-      w.page[half] = i < wide ? table[i] : -1;
-      w.row[half] = key & (page_size - 1);
+      const int p = page_at(t, half);
+      const bool ok = (unsigned)p < (unsigned)pages;
+      w.exist |= ok ? 1 << half : 0;
+      request_half<D>(to + half * TileLds<D>::kHalf, base + (ok ? p : 0) * a.pool.page_stride, page_size,
+                      (w.key + 16 * half) & (page_size - 1), k_at, p_at, lane);
     }
     return w;
   };
-  // (once the page numbers are needed: they have had a tile's time to arrive)
-  auto resolve = [&](TileAt& w) {
+  uint32_t bias_low, bias_high;
+  asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(bias_low));
+  asm volatile("v_mov_b32 %0, 0x54005400" : "=v"(bias_high));
+
+  // The next tile of the wave is on its way while one is used. (No other wave reads them, so
+  // the wave's own counter of loads is all there is to wait for.)
+  Tile now{}, next{};
+  if (tile < end) {
+    fetch_pages(tile);
+    next = request(0, tile);
+  }
+  int slot = 0;
+  for (; tile < end; tile += kWaves, slot ^= 1) {
+    now = next;
+    const int ahead = tile + kWaves;
+    if (ahead < end) {
+      if (ahead >= pages_from + 32 * kWaves) fetch_pages(ahead);
+      next = request(slot ^ 1, ahead);
+      wait_loads<TileLds<D>::kLoads>();
+    } else {
+      wait_loads<0>();
+    }
+    const int key = now.key;
+    const bool exist0 = now.exist & 1, exist1 = now.exist >> 1 & 1;
+    const char* mine = ring + slot * TileLds<D>::kBytes;
+    uint32_t kc[2][S], kp[8], vp[8];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int p = (unsigned)w.page[half] < (unsigned)pages ? w.page[half] : 0;
-      w.block[half] = base + p * a.pool.page_stride;
+      const char* at = mine + half * TileLds<D>::kHalf;
+      if constexpr (D == 64) {
+        const u32x2 v = *(const u32x2*)(at + n * 32 + g * 8);
+        kc[half][0] = v[0], kc[half][1] = v[1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+          const u32x4 v = *(const u32x4*)(at + 1024 * i + lane * 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kc[half][4 * i + j] = v[j];
+        }
+      }
+      const u32x4 kv = *(const u32x4*)(at + 2 * TileLds<D>::kCodes + g * 16);
+      const u32x4 vv = *(const u32x4*)(at + 2 * TileLds<D>::kCodes + 64 + g * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kp[4 * half + j] = kv[j], vp[4 * half + j] = vv[j];
     }
-  };
-
-  const LaneAt<D> at(n, g);
-  KvTile<D> t;
-  TileAt now, next;
-  int tile = begin + wave;
-  if (tile < end) {
-    now = locate(tile);
-    resolve(now);
-    load_k<D>(t, now, at);
-    load_kp<D>(t, now, at, page_size);
-    load_vp<D>(t, now, at, page_size);
-    load_v<D>(t, now, at, page_size);
-    next = locate(tile + kWaves < end ? tile + kWaves : tile);
-  }
-  // Each part of a tile is requested again, for the wave's next tile, as soon as it has been
-  // used: one tile is in flight at any time, in the registers of one. (The last tile requests
-  // itself once more.)
-  for (; tile < end; tile += kWaves) {
-    const int key = now.key;
-    const bool exist0 = (unsigned)now.page[0] < (unsigned)pages, exist1 = (unsigned)now.page[1] < (unsigned)pages;
-    resolve(next);
     floatx4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      s0 = F16Cfg16::mfma(k_frag(t.k[0][i]), qf[i].f, s0);
-      s1 = F16Cfg16::mfma(k_frag(t.k[1][i]), qf[i].f, s1);
+      s0 = F16Cfg16::mfma(k_frag(kc[0][i]), qf[i].f, s0);
+      s1 = F16Cfg16::mfma(k_frag(kc[1][i]), qf[i].f, s1);
     }
-    load_k<D>(t, next, at);
-    __builtin_amdgcn_sched_barrier(0);
-    float w[8], x[8];
-    uint32_t vp[8];
+    float x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t kp = dword(t.kp[j >> 2], j & 3);
-      w[j] = fmaf(F16::widen(kp & 0xFFFFu), j < 4 ? s0[j & 3] : s1[j & 3], F16::widen(kp >> 16) * qsum);
-      x[j] = fmaf(w[j], f, -ref);
-      vp[j] = dword(t.vp[j >> 2], j & 3);
+      const half2v sm = as_half2(kp[j]);
+      (j < 4 ? s0 : s1)[j & 3] *= f;
+      x[j] = fmaf((float)sm[0], (j < 4 ? s0 : s1)[j & 3], fmaf((float)sm[1], qsum, -ref));
     }
-    load_kp<D>(t, next, at, page_size);
-    load_vp<D>(t, next, at, page_size);
     // Every row sees the whole tile, or each looks at each key: one it does not see has no
     // weight, and no scale or offset, which may be NaN there.
     const bool whole = exist0 && exist1 && key + kTile <= lo_pos + 1 &&
@@ -406,25 +428,23 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE
     half2v smost = as_half2(vp[0]);                 // (scales are not negative, and the low halves)
 #pragma unroll
     for (int j = 1; j < 8; ++j) smost = __builtin_elementwise_max(smost, as_half2(vp[j]));
-    const float stop = (float)smost[0];
-    if (__ballot(top > kLazy || stop * vscale >= kScaleMost || vscale == 0.f)) {
+    const float stop = fmaxf((float)smost[0], 0x1p-24f);
+    if (__ballot(top > (float)(kMost + 1 - __builtin_amdgcn_frexp_expf(stop)))) {
       float most = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = fmaxf(most, seen >> j & 1 ? w[j] * f : -INFINITY);
-      const float raised = fmaxf(ref, across_max(most));
-      float factor = exp2f(ref - raised);
+      for (int j = 0; j < 8; ++j) {
+        const half2v sm = as_half2(kp[j]);
+        x[j] = fmaf((float)sm[0], (j < 4 ? s0 : s1)[j & 3], (float)sm[1] * qsum);
+        x[j] = seen >> j & 1 ? x[j] : -INFINITY;
+        most = fmaxf(most, x[j]);
+      }
+      const float raised = fmaxf(ref, across_max(most) + (float)(__builtin_amdgcn_frexp_expf(across_max(stop)) - 1 - kTarget));
+      const float factor = __builtin_amdgcn_exp2f(ref - raised);
       l *= factor;
       bias *= factor;
       ref = raised;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = seen >> j & 1 ? fmaf(w[j], f, -ref) : -INFINITY;
-      float smax = stop;
-      for (int m = 1; m < 64; m *= 2) smax = fmaxf(smax, __shfl_xor(smax, m));
-      if (smax * vscale >= kScaleMost || (vscale == 0.f && smax > 0.f)) {
-        const float to = ldexpf(1.f, 7 - ilogbf(smax));
-        factor *= vscale == 0.f ? 0.f : to / vscale;
-        vscale = to;
-      }
+      for (int j = 0; j < 8; ++j) x[j] -= ref;
 #pragma unroll
       for (int i = 0; i < NI; ++i) o[i] *= factor;
     }
@@ -435,16 +455,20 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE
       const float p = __builtin_amdgcn_exp2f(x[j]);
       l += p;
       bias = fmaf(p, fmaf((float)sm[0], 8.f, (float)sm[1]), bias);
-      const float weight = p * ((float)sm[0] * vscale);
-      hi.f[j] = (_Float16)weight;
-      if constexpr (kExact) lo.f[j] = (_Float16)(weight - (float)hi.f[j]);
+      hi.f[j] = (_Float16)(p * (float)sm[0]);
+      if constexpr (kExact) lo.f[j] = (_Float16)fmaf(p, (float)sm[0], -(float)hi.f[j]);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       uint32_t d[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = dword(t.v[j >> 2][c], j & 3);
+      for (int half = 0; half < 2; ++half) {
+        const char* at = mine + half * TileLds<D>::kHalf + TileLds<D>::kCodes;
+        const u32x4 v = *(const u32x4*)(at + (D == 64 ? g * 128 + (n & 7) * 16 : 1024 * c + lane * 16));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[4 * half + j] = v[j];
+      }
       auto add = [&](int i, const Frag& v) {
         o[i] = F16Cfg16::mfma(v.f, hi.f, o[i]);
         if constexpr (kExact) o[i] = F16Cfg16::mfma(v.f, lo.f, o[i]);
@@ -456,8 +480,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE
         for (int p = 0; p < 4; ++p) {
           uint32_t both = pair_bytes<b>(d[2 * p], d[2 * p + 1]);
           if constexpr (D == 64) both >>= (n >> 3) * 4;    // lanes 8.. of 16 take the odd d
-          even.h[p] = low_codes(both);
-          if constexpr (D != 64) odd.h[p] = high_codes(both);
+          even.h[p] = low_codes(both, bias_low);
+          if constexpr (D != 64) odd.h[p] = high_codes(both, bias_high);
         }
         if constexpr (D == 64) {
           add(b, even);
@@ -471,10 +495,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE
       byte(std::integral_constant<int, 2>{});
       byte(std::integral_constant<int, 3>{});
     }
-    load_v<D>(t, next, at, page_size);
-    now = next;
-    next = locate(tile + 2 * kWaves < end ? tile + 2 * kWaves : tile);
   }
+  __syncthreads();           // (the join's memory is the rings')
 
   // Join the waves: everything relative to the largest reference.
   l = across_sum(l);
@@ -487,14 +509,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE
   float top = ref_s[0][n];
   for (int i = 1; i < kWaves; ++i) top = fmaxf(top, ref_s[i][n]);
   const float factor = exp2f(ref - top);
-  const float vfactor = vscale == 0.f ? 0.f : factor / vscale;
 #pragma unroll
   for (int i = 0; i < NI; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int m = 4 * g + r;
       const int d = D == 64 ? 8 * (m & 7) + 2 * i + (m >> 3) : 8 * (m + 16 * (i >> 3)) + (i & 7);
-      o_s[wave][n][d] = fmaf(o[i][r], vfactor, bias * factor);
+      o_s[wave][n][d] = (o[i][r] + bias) * factor;
     }
   __syncthreads();
   float* part = (float*)a.workspace + ((int64_t)blockIdx.x * args.splits + split) * part_floats<D>();
@@ -521,42 +542,69 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = total != 0.f ? v[j] / total : 0.f;
     const uint2 r0 = narrow4<T>(v), r1 = narrow4<T>(v + 4);
-    uint16_t* out = (uint16_t*)a.out + (rows.token0 + mine / G) * a.out_stride + (int64_t)(head * G + mine % G) * D + d;
+    uint16_t* out = (uint16_t*)a.out + (int64_t)(rows.token0 + mine / G) * a.out_stride + (int64_t)(head * G + mine % G) * D + d;
     *(uint4*)out = make_uint4(r0.x, r0.y, r1.x, r1.y);
   }
 }
 
-// Adds the partial results of a tile's splits in order, one workgroup per row.
+// Adds the partial results of the splits. A workgroup takes every gridDim.y-th row of a tile:
+// groups of D / 4 threads a row each, or where there are fewer rows than groups a share of a
+// row's splits, joined in a fixed order.
+constexpr int kJoinThreads = 256;
 template <int D, typename T>
-__global__ __launch_bounds__(D / 2) void attention_kv4_join_kernel(SplitArgs args) {
+__global__ __launch_bounds__(kJoinThreads) void attention_kv4_join_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
+  constexpr int L = D / 4, kGroups = kJoinThreads / L;
+  __shared__ float sum_s[kGroups][D], total_s[kGroups];
   const int head = blockIdx.x % a.kv_heads, G = args.group;
   const Rows rows = find_rows(a, blockIdx.x / a.kv_heads, G, kRows);
   if (rows.b < 0) return;
-  const int row = rows.first + blockIdx.y;
-  if (row >= rows.count) return;
   const int last_row = rows.count - 1 < rows.first + kRows - 1 ? rows.count - 1 : rows.first + kRows - 1;
   const Keys<kTile> keys(a, position(rows, rows.first / G), position(rows, last_row / G));
   const int parts = active_splits(args, keys.total);
   if (parts == 1) return;
   const float* part = (const float*)a.workspace + (int64_t)blockIdx.x * args.splits * part_floats<D>();
-  const int r = blockIdx.y, d = threadIdx.x * 2;
-  float most = -1e30f;
-  for (int i = 0; i < parts; ++i) most = fmaxf(most, part[i * part_floats<D>() + kRows * D + r]);
-  float total = 0.f, x = 0.f, y = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float* p = part + i * part_floats<D>();
-    const float factor = exp2f(p[kRows * D + r] - most);
-    const float2 v = *(const float2*)(p + r * D + d);
-    total = fmaf(p[kRows * (D + 1) + r], factor, total);
-    x = fmaf(v.x, factor, x);
-    y = fmaf(v.y, factor, y);
+  const int Y = gridDim.y, y = blockIdx.y;
+  const int count = (last_row - rows.first - y + Y) / Y;        // rows y, y + Y, ... of the tile
+  if (count <= 0) return;
+  const int share = count < kGroups ? kGroups / count : 1;      // groups of a row
+  const int group = threadIdx.x / L, lane = threadIdx.x % L, d = lane * 4;
+  for (int first = 0; first < count; first += kGroups / share) {
+    const int nth = first + group / share, r = y + nth * Y;
+    if (nth < count && group < kGroups / share * share) {
+      float most = -1e30f;
+      for (int i = lane; i < parts; i += L) most = fmaxf(most, part[i * part_floats<D>() + kRows * D + r]);
+      for (int m = 1; m < L; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float total = 0.f;
+#pragma unroll 8
+      for (int i = group % share; i < parts; i += share) {
+        const float* p = part + i * part_floats<D>();
+        const float factor = __builtin_amdgcn_exp2f(p[kRows * D + r] - most);
+        const float4 v = *(const float4*)(p + r * D + d);
+        total = fmaf(p[kRows * (D + 1) + r], factor, total);
+        sum.x = fmaf(v.x, factor, sum.x), sum.y = fmaf(v.y, factor, sum.y);
+        sum.z = fmaf(v.z, factor, sum.z), sum.w = fmaf(v.w, factor, sum.w);
+      }
+      *(float4*)&sum_s[group][d] = sum;
+      if (lane == 0) total_s[group] = total;
+    }
+    __syncthreads();
+    if (nth < count && group % share == 0 && group < kGroups / share * share) {
+      float v[4] = {}, total = 0.f;
+      for (int i = 0; i < share; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += sum_s[group + i][d + j];
+        total += total_s[group + i];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = total != 0.f ? v[j] / total : 0.f;
+      const int row = rows.first + r;
+      uint16_t* out = (uint16_t*)a.out + (int64_t)(rows.token0 + row / G) * a.out_stride + (int64_t)(head * G + row % G) * D + d;
+      *(uint2*)out = narrow4<T>(v);
+    }
+    __syncthreads();
   }
-  x = total != 0.f ? x / total : 0.f;
-  y = total != 0.f ? y / total : 0.f;
-  uint16_t* out = (uint16_t*)a.out + (rows.token0 + row / G) * a.out_stride + (int64_t)(head * G + row % G) * D + d;
-  *(uint32_t*)out = T::narrow(x) | (T::narrow(y) << 16);
 }
 
 // How many splits of how many key tiles. Of all the tiles of rows the grid can hold, and of
@@ -575,15 +623,20 @@ Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int64_t windo
   if (keys > 0x7FFFFFFF) keys = 0x7FFFFFFF;
   const int64_t key_tiles = ceil_div(keys, kTile);
   const int64_t units = (tokens * G / kRows < batch ? batch : tokens * G / kRows) * kv_heads;
-  const int64_t wanted = 1ll * WANT * device_cu_count();
-  int64_t chunk = ceil_div(key_tiles * units, wanted);
-  chunk = ceil_div(chunk < MINC ? MINC : chunk, kWaves) * kWaves;
-  p.chunk = (int)chunk;
-  p.splits = (int)ceil_div(key_tiles < 1 ? 1 : key_tiles, chunk);
-  if (p.splits > 1024) {
-    p.splits = 1024;
-    p.chunk = (int)ceil_div(key_tiles, 1024);
-  }
+  // Six workgroups to a compute unit, so that lengths that differ even out (32 sequences of
+  // 1000 to 8192 keys: 49 us, two to a unit 59), but no more than 32 splits where fewer fill the
+  // device: the join reads them all (two of 131072 keys: 59 us, with 96 splits 65). A split has
+  // enough tiles to be worth its start and the join, fewer where most of the device is idle; and
+  // at most 512, past which the f32 sums of a wave would show in the result.
+  const int64_t cus = device_cu_count();
+  int64_t splits = ceil_div(6 * cus, units);
+  if (splits > 32) splits = ceil_div(2 * cus, units) > 32 ? ceil_div(2 * cus, units) : 32;
+  const int64_t most = 2 * units <= cus ? ceil_div(key_tiles, 16) : key_tiles / 32;
+  splits = splits < most ? splits : most < 1 ? 1 : most;
+  if (splits < ceil_div(key_tiles, 512)) splits = ceil_div(key_tiles, 512);
+  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
+  p.chunk = (int)(ceil_div(ceil_div(key_tiles < 1 ? 1 : key_tiles, splits), kWaves) * kWaves);
+  p.splits = (int)ceil_div(key_tiles < 1 ? 1 : key_tiles, p.chunk);
   return p;
 }
 
@@ -595,12 +648,26 @@ int launch_split(const AttentionKv4Args& a, hipStream_t s) {
   const uint64_t one = (uint64_t)blocks * part_floats<D>() * 4;
   if (p.splits > 1 && a.workspace_bytes < one * p.splits) p.splits = 1;
   SplitArgs args{a, a.heads / a.kv_heads, p.splits, p.chunk};
-  hipLaunchKernelGGL((attention_kv4_split_kernel<D, T>), dim3((unsigned)blocks, (unsigned)p.splits), dim3(64 * kWaves), 0,
-                     s, args);
+  if (split_lds_bytes<D>() > 65536) {
+    static PerDeviceOnce once;
+    int dev = 0;
+    UK_RETURN_IF_HIP(hipGetDevice(&dev));
+    if (!once.done(dev)) {
+      UK_RETURN_IF_HIP(hipFuncSetAttribute((const void*)attention_kv4_split_kernel<D, T>,
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, split_lds_bytes<D>()));
+      once.mark(dev);
+    }
+  }
+  hipLaunchKernelGGL((attention_kv4_split_kernel<D, T>), dim3((unsigned)blocks, (unsigned)p.splits), dim3(64 * kWaves),
+                     split_lds_bytes<D>(), s, args);
   UK_RETURN_IF_HIP(hipGetLastError());
   if (p.splits == 1) return 0;
-  const int64_t rows = a.tokens * args.group < kRows ? a.tokens * args.group : kRows;
-  hipLaunchKernelGGL((attention_kv4_join_kernel<D, T>), dim3((unsigned)blocks, (unsigned)rows), dim3(D / 2), 0, s, args);
+  // A row a workgroup where the tiles are few, one workgroup a tile where they fill the device
+  // (most rows of a tile are not there in a decode step, and each workgroup has to find that out).
+  int64_t rows = 2ll * device_cu_count() / blocks;
+  rows = rows < 1 ? 1 : rows > kRows ? kRows : rows;
+  hipLaunchKernelGGL((attention_kv4_join_kernel<D, T>), dim3((unsigned)blocks, (unsigned)rows), dim3(kJoinThreads), 0,
+                     s, args);
   return check_hip(hipGetLastError(), "attention_kv4");
 }
 
