@@ -33,6 +33,7 @@ struct Rows {
   int tokens;        // its query tokens
   int token0;        // its first token
   int kv_len;
+  int64_t slot;
 };
 
 // The sequence of tile `slot`: the last b whose first tile is at most it. 64 lanes look at
@@ -65,6 +66,7 @@ __device__ inline Rows find_rows(const AttentionKv4Args& a, int64_t slot, int G,
   r.tokens = __builtin_amdgcn_readfirstlane(to - from);
   r.token0 = __builtin_amdgcn_readfirstlane(from);
   r.kv_len = __builtin_amdgcn_readlane(len, last);
+  r.slot = slot;
   return r;
 }
 
@@ -119,9 +121,9 @@ constexpr int kMaxSplits = 1024;
 // other end lies 2^-31 below the largest p s. A scale counts as at least 2^-24 (it may be 0).
 constexpr int kTarget = 7, kMost = 13;
 
-// Partial results of a split: per (tile, kv head, split) O [16][D], reference [16], sum [16].
-template <int D>
-__host__ __device__ constexpr int64_t part_floats() { return kRows * (D + 2); }
+// Partial results of a split: per (tile, kv head, split) O [R][D], reference [R], sum [R].
+template <int D, int R>
+__host__ __device__ constexpr int64_t part_floats() { return R * (D + 2); }
 
 struct SplitArgs {
   AttentionKv4Args a;
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
       o_s[wave][n][d] = (o[i][r] + bias) * factor;
     }
   __syncthreads();
-  float* part = (float*)a.workspace + ((int64_t)blockIdx.x * args.splits + split) * part_floats<D>();
+  float* part = (float*)a.workspace + ((int64_t)blockIdx.x * args.splits + split) * part_floats<D, kRows>();
   for (int at = threadIdx.x; at < kRows * D / 8; at += 64 * kWaves) {
     const int r = at / (D / 8), d = at % (D / 8) * 8;
     const int mine = rows.first + r;
@@ -551,19 +553,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
 // groups of D / 4 threads a row each, or where there are fewer rows than groups a share of a
 // row's splits, joined in a fixed order.
 constexpr int kJoinThreads = 256;
-template <int D, typename T>
+template <int D, typename T, int R, int kKeys>
 __global__ __launch_bounds__(kJoinThreads) void attention_kv4_join_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
   constexpr int L = D / 4, kGroups = kJoinThreads / L;
   __shared__ float sum_s[kGroups][D], total_s[kGroups];
   const int head = blockIdx.x % a.kv_heads, G = args.group;
-  const Rows rows = find_rows(a, blockIdx.x / a.kv_heads, G, kRows);
+  const Rows rows = find_rows(a, blockIdx.x / a.kv_heads, G, R);
   if (rows.b < 0) return;
-  const int last_row = rows.count - 1 < rows.first + kRows - 1 ? rows.count - 1 : rows.first + kRows - 1;
-  const Keys<kTile> keys(a, position(rows, rows.first / G), position(rows, last_row / G));
+  const int last_row = rows.count - 1 < rows.first + R - 1 ? rows.count - 1 : rows.first + R - 1;
+  const Keys<kKeys> keys(a, position(rows, rows.first / G), position(rows, last_row / G));
   const int parts = active_splits(args, keys.total);
   if (parts == 1) return;
-  const float* part = (const float*)a.workspace + (int64_t)blockIdx.x * args.splits * part_floats<D>();
+  const float* part = (const float*)a.workspace + (int64_t)blockIdx.x * args.splits * part_floats<D, R>();
   const int Y = gridDim.y, y = blockIdx.y;
   const int count = (last_row - rows.first - y + Y) / Y;        // rows y, y + Y, ... of the tile
   if (count <= 0) return;
@@ -573,16 +575,16 @@ __global__ __launch_bounds__(kJoinThreads) void attention_kv4_join_kernel(SplitA
     const int nth = first + group / share, r = y + nth * Y;
     if (nth < count && group < kGroups / share * share) {
       float most = -1e30f;
-      for (int i = lane; i < parts; i += L) most = fmaxf(most, part[i * part_floats<D>() + kRows * D + r]);
+      for (int i = lane; i < parts; i += L) most = fmaxf(most, part[i * part_floats<D, R>() + R * D + r]);
       for (int m = 1; m < L; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       float total = 0.f;
 #pragma unroll 8
       for (int i = group % share; i < parts; i += share) {
-        const float* p = part + i * part_floats<D>();
-        const float factor = __builtin_amdgcn_exp2f(p[kRows * D + r] - most);
+        const float* p = part + i * part_floats<D, R>();
+        const float factor = __builtin_amdgcn_exp2f(p[R * D + r] - most);
         const float4 v = *(const float4*)(p + r * D + d);
-        total = fmaf(p[kRows * (D + 1) + r], factor, total);
+        total = fmaf(p[R * (D + 1) + r], factor, total);
         sum.x = fmaf(v.x, factor, sum.x), sum.y = fmaf(v.y, factor, sum.y);
         sum.z = fmaf(v.z, factor, sum.z), sum.w = fmaf(v.w, factor, sum.w);
       }
@@ -607,67 +609,444 @@ __global__ __launch_bounds__(kJoinThreads) void attention_kv4_join_kernel(SplitA
   }
 }
 
-// How many splits of how many key tiles. Of all the tiles of rows the grid can hold, and of
-// the keys the longest sequence shows them.
+// ---------------------------------------------------------------------------
+// Many rows: prompts
+// ---------------------------------------------------------------------------
+
+constexpr int kPromptRows = 128;      // of a workgroup, 32 of each of its four waves
+template <int D>
+constexpr int prompt_keys() { return D == 256 ? 32 : 64; }
+
+// One of the two buffers of key tiles in LDS: K and V codes as f16 in the order in which the
+// lanes read them, then the keys' parameters, scale and offset (of V: scale and offset + 8
+// scales, rounded to f16, next to which the rounding of the weights is several times as large).
+template <int D>
+struct PromptLds {
+  static constexpr int N = prompt_keys<D>();
+  static constexpr int kV = N * D * 2;                  // K before it: [N / 32][D / 16][64 lanes] of 16 bytes
+  static constexpr int kParams = 2 * kV;                // V: [N / 16][D / 32][64 lanes]
+  static constexpr int kBytes = kParams + N * 8;
+};
+template <int D>
+constexpr int prompt_lds_bytes() { return 2 * PromptLds<D>::kBytes + 64; }
+
+// 128 rows of one kv head against its key tiles. The workgroup turns each tile's codes into f16
+// once, in LDS (centred for V, see above; subnormals for K), while its waves multiply the tile
+// before it: v_mfma_f32_32x32x16_f16 with the keys as rows of the scores, as in the kernel for
+// few rows, 32 rows a wave. Bound by the vector instructions of the softmax: about ten to a
+// score (three for scale and offset, one each for the largest, the sum, the offsets of V and
+// the operand, an exponential at a quarter of the rate).
+template <int D, typename T>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_kernel(SplitArgs args) {
+  const AttentionKv4Args& a = args.a;
+  constexpr int N = prompt_keys<D>(), KB = N / 32, KK = N / 16;     // keys; blocks of 32; steps of 16
+  constexpr int S = D / 16, DB = D / 32;                            // steps of a score; blocks of d
+  constexpr int VU = KK * 2 * (D / 8);                              // units of V: 8 keys of 8 d
+  constexpr int KC = N * D / 32 / 128;                              // chunks of K of 16 bytes to a thread
+  extern __shared__ __attribute__((aligned(1024))) char memory[];
+  const int G = args.group;
+  const int head = blockIdx.x % a.kv_heads;
+  // (the last tiles of a prompt see most keys: they start first)
+  const Rows rows = find_rows(a, gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads, G, kPromptRows);
+  if (rows.b < 0) return;
+  const int last_row = rows.count - 1 < rows.first + kPromptRows - 1 ? rows.count - 1 : rows.first + kPromptRows - 1;
+  const int wg_lo = position(rows, rows.first / G), wg_hi = position(rows, last_row / G);
+  const Keys<N> keys(a, wg_lo, wg_hi);
+  const int parts = active_splits(args, keys.total);
+  const int split = blockIdx.y;
+  if (split >= parts) return;
+  const int begin = split * args.chunk, end = split == parts - 1 ? keys.total : begin + args.chunk;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+
+  // The lane's query row; the rows of its wave.
+  const int wave_first = rows.first + wave * 32 < last_row ? rows.first + wave * 32 : last_row;
+  const int wave_last = wave_first + 31 < last_row ? wave_first + 31 : last_row;
+  const bool idle = rows.first + wave * 32 > last_row;
+  const int row = wave_first + n < wave_last ? wave_first + n : wave_last;
+  const int pos = position(rows, row / G), lo_pos = position(rows, wave_first / G), hi_pos = position(rows, wave_last / G);
+  const uint16_t* q = (const uint16_t*)a.q + (int64_t)(rows.token0 + row / G) * a.q_stride +
+                      (int64_t)(head * G + row % G) * D + h * 8;
+  Frag qf[S];
+  float f, qsum;
+  {
+    float top = 0.f, sum = 0.f;
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const u32x4 w = *(const u32x4*)(q + 16 * s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        qf[s].u[j] = w[j];
+        const float x0 = T::widen(w[j] & 0xFFFFu), x1 = T::widen(w[j] >> 16);
+        top = fmaxf(top, fmaxf(fabsf(x0), fabsf(x1)));
+        sum += x0 + x1;
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 32));
+    sum = (sum + __shfl_xor(sum, 32)) * sign;
+    const int e = top > 0.f && top < INFINITY ? 8 - ilogbf(top) : 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[2 * j] = T::widen(qf[s].u[j] & 0xFFFFu) * sign;
+        x[2 * j + 1] = T::widen(qf[s].u[j] >> 16) * sign;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int nibble = (j >> 1) + 4 * (j & 1);
+        qf[s].f[j] = (_Float16)ldexpf(x[nibble], nibble & 1 ? e - 4 : e);
+      }
+    }
+    f = ldexpf(fabsf(a.scale) * kLog2e, 24 - e);
+    qsum = sum * (fabsf(a.scale) * kLog2e);
+  }
+
+  // Staging: threads 0 .. VU - 1 take a unit of V each, threads 128 .. 255 chunks of K, threads
+  // 128 .. 128 + N - 1 also the parameters of a key.
+  const int shift = a.pool.page_shift, page_size = 1 << shift, pages = (int)a.pool.pages, wide = (int)a.max_pages;
+  const char* base = a.pool.base + head * Block<D>::bytes(page_size);
+  const int32_t* table = a.page_table + rows.b * a.page_table_stride;
+  // (what follows from the thread's number is worked out anew for each tile: kept over the
+  // loop, it would take the registers of the results)
+  auto thread = [&]() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+  };
+  int pages_from = begin, page_ids = -1;
+  auto fetch_pages = [&](int from) {
+    const int t = from + lane / KK;
+    const int i = t < end ? (keys.key(t) + 16 * (lane % KK)) >> shift : wide;
+    pages_from = from;
+    page_ids = i < wide ? table[i] : -1;
+  };
+  u32x4 raw[2];
+  uint32_t raw_kp = 0, raw_vp = 0;
+  int exist_next = 0;           // whether the pages of the fetched tile's groups of 16 keys exist
+  auto fetch = [&](int t) {
+    const int key0 = keys.key(t), tid = thread();
+    const int v_kk = tid / (2 * (D / 8)), v_h = tid / (D / 8) & 1, v_w = tid % (D / 8);
+    exist_next = (int)(__ballot((unsigned)page_ids < (unsigned)pages) >> ((t - pages_from) * KK)) & ((1 << KK) - 1);
+    auto block_of = [&](int group) -> const char* {
+      const int p = __shfl(page_ids, (t - pages_from) * KK + group);
+      return (unsigned)p < (unsigned)pages ? base + p * a.pool.page_stride : nullptr;
+    };
+    if (wave < 2) {
+      const char* block = block_of(v_kk & (KK - 1));
+      const int r = (key0 + 16 * v_kk + 4 * v_h) & (page_size - 1);
+      raw[0] = raw[1] = u32x4{0u, 0u, 0u, 0u};
+      if (block && tid < VU) {
+        raw[0] = *(const u32x4*)(block + Block<D>::v_dword(page_size, r, v_w));
+        raw[1] = *(const u32x4*)(block + Block<D>::v_dword(page_size, r + 8, v_w));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const int chunk = tid - 128 + 128 * i, k = chunk / (D / 32);
+        const char* block = block_of(k / 16);
+        raw[i] = u32x4{0u, 0u, 0u, 0u};
+        if (block)
+          raw[i] = *(const u32x4*)(block + Block<D>::k_row((key0 + k) & (page_size - 1)) + chunk % (D / 32) * 16);
+      }
+      const int k = (tid - 128) & (N - 1);
+      const char* block = block_of(k / 16);
+      // (keys that no row of the workgroup sees count as zeros: what lies there may be NaN)
+      raw_kp = raw_vp = 0;
+      if (block && tid - 128 < N && key0 + k <= wg_hi) {
+        raw_kp = *(const uint32_t*)(block + Block<D>::k_params(page_size, (key0 + k) & (page_size - 1)));
+        raw_vp = *(const uint32_t*)(block + Block<D>::v_params(page_size, (key0 + k) & (page_size - 1)));
+      }
+    }
+  };
+  uint32_t bias_low, bias_high;
+  asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(bias_low));
+  asm volatile("v_mov_b32 %0, 0x54005400" : "=v"(bias_high));
+  float* scales = (float*)(memory + 2 * PromptLds<D>::kBytes);      // the largest scale of V in each buffer
+  auto stage = [&](int buffer) {
+    char* to = memory + buffer * PromptLds<D>::kBytes;
+    const int tid = thread();
+    const int v_kk = tid / (2 * (D / 8)), v_h = tid / (D / 8) & 1, v_w = tid % (D / 8);
+    if (wave < 2) {
+      if (tid < VU) {
+        // 8 d of 8 keys: 16 bytes for each d, those of a thread next to each other. Their place is
+        // turned by the thread's block, or 64 threads would write to an eighth of the banks.
+        char* at = to + PromptLds<D>::kV + ((v_kk * DB + v_w / 4) * 64 + v_h * 32 + v_w % 4 * 8) * 16;
+        const int turn = (v_w & 3) + 4 * v_h;
+        auto byte = [&](auto which) {
+          constexpr int b = decltype(which)::value;
+          Frag even, odd;
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const uint32_t both = pair_bytes<b>(raw[p >> 1][2 * (p & 1)], raw[p >> 1][2 * (p & 1) + 1]);
+            even.h[p] = low_codes(both, bias_low);
+            odd.h[p] = high_codes(both, bias_high);
+          }
+          *(half8*)(at + ((2 * b) ^ turn) * 16) = even.f;
+          *(half8*)(at + ((2 * b + 1) ^ turn) * 16) = odd.f;
+        };
+        byte(std::integral_constant<int, 0>{});
+        byte(std::integral_constant<int, 1>{});
+        byte(std::integral_constant<int, 2>{});
+        byte(std::integral_constant<int, 3>{});
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const int chunk = tid - 128 + 128 * i, k = chunk / (D / 32), c = chunk % (D / 32) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *(half8*)(to + ((k / 32 * S + (c + j) / 2) * 64 + (c + j) % 2 * 32 + k % 32) * 16) = k_frag(raw[i][j]);
+      }
+      if (tid - 128 < N) {
+        const int k = tid - 128;
+        const half2v sm = as_half2(raw_vp);
+        half2v v;
+        v[0] = sm[0];
+        v[1] = (_Float16)fmaf((float)sm[0], 8.f, (float)sm[1]);
+        *(uint32_t*)(to + PromptLds<D>::kParams + k * 4) = raw_kp;
+        *(half2v*)(to + PromptLds<D>::kParams + N * 4 + k * 4) = v;
+        float most = (float)sm[0];
+        for (int m = 1; m < (N < 64 ? N : 64); m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+        if (k == 0) scales[buffer] = most;
+      }
+    }
+  };
+
+  floatx16 o[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) o[i] = floatx16{};
+  float ref = -1e30f, l = 0.f, bias = 0.f;
+  const int below = a.window ? pos - (int)a.window : -1, sinks = a.window ? (int)a.sinks : 0;
+  if (begin < end) {
+    fetch_pages(begin);
+    fetch(begin);
+    stage(0);
+  }
+  __syncthreads();
+  for (int tile = begin; tile < end; ++tile) {
+    const int buffer = (tile - begin) & 1, exist = exist_next;
+    const bool more = tile + 1 < end;
+    if (more) {
+      if (tile + 1 >= pages_from + 64 / KK) fetch_pages(tile + 1);
+      fetch(tile + 1);
+    }
+    const int key = keys.key(tile);
+    // (rows of this wave that see some of the tile: behind its last row there is nothing)
+    if (!idle && key <= hi_pos) {
+      const char* from = memory + buffer * PromptLds<D>::kBytes;
+      const float stop = fmaxf(scales[buffer], 0x1p-24f);
+      const int stop_e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(stop));
+      const bool whole = exist == (1 << KK) - 1 && key + N <= lo_pos + 1 && (!a.window || key > hi_pos - (int)a.window || key + N <= sinks);
+      Frag p[KK];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        floatx16 s = {};
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+          s = F16Cfg::mfma(*(const half8*)(from + ((kb * S + i) * 64 + lane) * 16), qf[i].f, s);
+        __builtin_amdgcn_sched_barrier(0);
+        // Element j of a lane: key 32 kb + 8 (j / 4) + 4 h + j % 4.
+        float x[16];
+        uint32_t kp[16], vp[16];
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const char* at = from + PromptLds<D>::kParams + (32 * kb + 2 * j + 4 * h) * 4;
+          const u32x4 kv = *(const u32x4*)at, vv = *(const u32x4*)(at + N * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) kp[j + i] = kv[i], vp[j + i] = vv[i];
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const half2v sm = as_half2(kp[j]);
+          s[j] *= f;
+          x[j] = fmaf((float)sm[0], s[j], fmaf((float)sm[1], qsum, -ref));
+        }
+        uint32_t seen = 0xFFFF;
+        if (!whole) {
+          seen = 0;
+          const int from_lane = key + 32 * kb + 4 * h;
+          const int up_to = pos - from_lane, past = below - from_lane, sink = sinks - from_lane;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int k = 8 * (j >> 2) + (j & 3);
+            const bool yes = (k <= up_to) & ((k > past) | (k < sink)) & ((exist >> (2 * kb + j / 8) & 1) != 0);
+            seen |= yes ? 1u << j : 0u;
+            x[j] = yes ? x[j] : -INFINITY;
+            vp[j] = yes ? vp[j] : 0u;
+          }
+        }
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
+        if (__ballot(top > (float)(kMost + 1 - stop_e))) {
+          float most = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const half2v sm = as_half2(kp[j]);
+            x[j] = fmaf((float)sm[0], s[j], (float)sm[1] * qsum);
+            x[j] = seen >> j & 1 ? x[j] : -INFINITY;
+            most = fmaxf(most, x[j]);
+          }
+          most = fmaxf(most, __shfl_xor(most, 32));
+          const float raised = fmaxf(ref, most + (float)(stop_e - 1 - kTarget));
+          const float factor = __builtin_amdgcn_exp2f(ref - raised);
+          l *= factor;
+          bias *= factor;
+          ref = raised;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] -= ref;
+#pragma unroll
+          for (int i = 0; i < DB; ++i) o[i] *= factor;
+          if (kb > 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) p[i].f[j] = (_Float16)((float)p[i].f[j] * factor);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const half2v sm = as_half2(vp[j]);
+          const float w = __builtin_amdgcn_exp2f(x[j]);
+          l += w;
+          bias = fmaf(w, (float)sm[1], bias);
+          p[2 * kb + j / 8].f[j % 8] = (_Float16)(w * (float)sm[0]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+          const int at = (kk * DB + i) * 64 + h * 32 + (n & 24) + ((n & 7) ^ ((n >> 3) + 4 * h));
+          o[i] = F16Cfg::mfma(*(const half8*)(from + PromptLds<D>::kV + at * 16), p[kk].f, o[i]);
+        }
+    }
+    if (more) stage(buffer ^ 1);
+    __syncthreads();
+  }
+
+  if (idle) return;
+  l += __shfl_xor(l, 32);
+  bias += __shfl_xor(bias, 32);
+  if (wave_first + n > wave_last) return;
+  if (parts > 1) {
+    float* part = (float*)a.workspace + ((int64_t)(rows.slot * a.kv_heads + head) * args.splits + split) * part_floats<D, kPromptRows>();
+    const int r = wave * 32 + n;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; j += 4)
+        *(float4*)(part + r * D + 32 * i + 2 * j + 4 * h) =
+            make_float4(o[i][j] + bias, o[i][j + 1] + bias, o[i][j + 2] + bias, o[i][j + 3] + bias);
+    if (h == 0) {
+      part[kPromptRows * D + r] = ref;
+      part[kPromptRows * (D + 1) + r] = l;
+    }
+    return;
+  }
+  const float inverse = l != 0.f ? 1.f / l : 0.f;
+  uint16_t* out = (uint16_t*)a.out + (int64_t)(rows.token0 + row / G) * a.out_stride + (int64_t)(head * G + row % G) * D;
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = (o[i][j + k] + bias) * inverse;
+      *(uint2*)(out + 32 * i + 2 * j + 4 * h) = narrow4<T>(v);
+    }
+}
+
+// Which kernel, and how many splits of how many of its key tiles. Of all the tiles of rows the
+// grid can hold, and of the keys the longest sequence shows them.
 struct Split {
+  bool prompt;
   int64_t tiles;       // of rows, with the gaps of their numbering
   int splits, chunk;
 };
 
-Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int64_t window, int64_t sinks, int64_t max_kv_len) {
-  const int64_t G = heads / kv_heads;
+Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int64_t window, int64_t sinks,
+           int64_t max_kv_len) {
+  const int64_t G = heads / kv_heads, rows = tokens * G;
   Split p;
-  p.tiles = tokens * G / kRows + batch;
+  p.prompt = rows >= 64 * batch;
+  const int64_t R = p.prompt ? kPromptRows : kRows, tile = !p.prompt ? kTile : dim == 256 ? 32 : 64;
+  p.tiles = rows / R + batch;
   int64_t keys = max_kv_len;
-  if (window && window + sinks < keys) keys = window + sinks + 2 * kTile;
+  if (window && window + sinks + (p.prompt ? R / G : 0) < keys) keys = window + sinks + (p.prompt ? R / G : 0) + 2 * tile;
   if (keys > 0x7FFFFFFF) keys = 0x7FFFFFFF;
-  const int64_t key_tiles = ceil_div(keys, kTile);
-  const int64_t units = (tokens * G / kRows < batch ? batch : tokens * G / kRows) * kv_heads;
-  // Six workgroups to a compute unit, so that lengths that differ even out (32 sequences of
-  // 1000 to 8192 keys: 49 us, two to a unit 59), but no more than 32 splits where fewer fill the
-  // device: the join reads them all (two of 131072 keys: 59 us, with 96 splits 65). A split has
-  // enough tiles to be worth its start and the join, fewer where most of the device is idle; and
-  // at most 512, past which the f32 sums of a wave would show in the result.
+  const int64_t key_tiles = keys < 1 ? 1 : ceil_div(keys, tile);
+  const int64_t units = (rows / R < batch ? batch : rows / R) * kv_heads;
   const int64_t cus = device_cu_count();
-  int64_t splits = ceil_div(6 * cus, units);
-  if (splits > 32) splits = ceil_div(2 * cus, units) > 32 ? ceil_div(2 * cus, units) : 32;
-  const int64_t most = 2 * units <= cus ? ceil_div(key_tiles, 16) : key_tiles / 32;
-  splits = splits < most ? splits : most < 1 ? 1 : most;
-  if (splits < ceil_div(key_tiles, 512)) splits = ceil_div(key_tiles, 512);
+  int64_t splits;
+  if (p.prompt) {
+    // Two workgroups to a compute unit; the tiles of a prompt see half of its keys on average.
+    splits = ceil_div(2 * cus, units);
+    const int64_t most = key_tiles / 8;
+    splits = units >= cus ? 1 : splits < most ? splits : most;
+  } else {
+    // Six workgroups to a compute unit, so that lengths that differ even out (32 sequences of
+    // 1000 to 8192 keys: 49 us, two to a unit 59), but no more than 32 splits where fewer fill the
+    // device: the join reads them all (two of 131072 keys: 59 us, with 96 splits 65). A split has
+    // enough tiles to be worth its start and the join, fewer where most of the device is idle.
+    splits = ceil_div(6 * cus, units);
+    if (splits > 32) splits = ceil_div(2 * cus, units) > 32 ? ceil_div(2 * cus, units) : 32;
+    const int64_t most = 2 * units <= cus ? ceil_div(key_tiles, 16) : key_tiles / 32;
+    splits = splits < most ? splits : most;
+  }
+  // (past 16384 keys the f32 sums of a wave would begin to show in the result)
+  if (splits < ceil_div(keys, 16384)) splits = ceil_div(keys, 16384);
   splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
-  p.chunk = (int)(ceil_div(ceil_div(key_tiles < 1 ? 1 : key_tiles, splits), kWaves) * kWaves);
-  p.splits = (int)ceil_div(key_tiles < 1 ? 1 : key_tiles, p.chunk);
+  p.chunk = (int)ceil_div(key_tiles, splits);
+  if (!p.prompt) p.chunk = (int)(ceil_div(p.chunk, kWaves) * kWaves);
+  p.splits = (int)ceil_div(key_tiles, p.chunk);
   return p;
+}
+
+template <typename Kernel>
+int allow_lds(Kernel kernel, int bytes, PerDeviceOnce& once) {
+  if (bytes <= 65536) return 0;
+  int dev = 0;
+  UK_RETURN_IF_HIP(hipGetDevice(&dev));
+  if (once.done(dev)) return 0;
+  UK_RETURN_IF_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  once.mark(dev);
+  return 0;
 }
 
 template <int D, typename T>
 int launch_split(const AttentionKv4Args& a, hipStream_t s) {
-  Split p = plan(a.tokens, a.batch, a.heads, a.kv_heads, a.window, a.sinks, a.max_kv_len);
+  Split p = plan(a.tokens, a.batch, a.heads, a.kv_heads, D, a.window, a.sinks, a.max_kv_len);
   const int64_t blocks = p.tiles * a.kv_heads;
   if (blocks > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "attention_kv4: too many rows for one call");
-  const uint64_t one = (uint64_t)blocks * part_floats<D>() * 4;
+  const uint64_t one = (uint64_t)blocks * (p.prompt ? part_floats<D, kPromptRows>() : part_floats<D, kRows>()) * 4;
   if (p.splits > 1 && a.workspace_bytes < one * p.splits) p.splits = 1;
   SplitArgs args{a, a.heads / a.kv_heads, p.splits, p.chunk};
-  if (split_lds_bytes<D>() > 65536) {
-    static PerDeviceOnce once;
-    int dev = 0;
-    UK_RETURN_IF_HIP(hipGetDevice(&dev));
-    if (!once.done(dev)) {
-      UK_RETURN_IF_HIP(hipFuncSetAttribute((const void*)attention_kv4_split_kernel<D, T>,
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, split_lds_bytes<D>()));
-      once.mark(dev);
-    }
+  static PerDeviceOnce once[2];
+  const dim3 grid((unsigned)blocks, (unsigned)p.splits);
+  if (p.prompt) {
+    UK_RETURN_IF_ERROR(allow_lds(attention_kv4_prompt_kernel<D, T>, prompt_lds_bytes<D>(), once[0]));
+    hipLaunchKernelGGL((attention_kv4_prompt_kernel<D, T>), grid, dim3(256), prompt_lds_bytes<D>(), s, args);
+  } else {
+    UK_RETURN_IF_ERROR(allow_lds(attention_kv4_split_kernel<D, T>, split_lds_bytes<D>(), once[1]));
+    hipLaunchKernelGGL((attention_kv4_split_kernel<D, T>), grid, dim3(64 * kWaves), split_lds_bytes<D>(), s, args);
   }
-  hipLaunchKernelGGL((attention_kv4_split_kernel<D, T>), dim3((unsigned)blocks, (unsigned)p.splits), dim3(64 * kWaves),
-                     split_lds_bytes<D>(), s, args);
   UK_RETURN_IF_HIP(hipGetLastError());
   if (p.splits == 1) return 0;
   // A row a workgroup where the tiles are few, one workgroup a tile where they fill the device
   // (most rows of a tile are not there in a decode step, and each workgroup has to find that out).
-  int64_t rows = 2ll * device_cu_count() / blocks;
-  rows = rows < 1 ? 1 : rows > kRows ? kRows : rows;
-  hipLaunchKernelGGL((attention_kv4_join_kernel<D, T>), dim3((unsigned)blocks, (unsigned)rows), dim3(kJoinThreads), 0,
-                     s, args);
+  const int64_t R = p.prompt ? kPromptRows : kRows;
+  int64_t shares = 2ll * device_cu_count() / blocks;
+  shares = shares < 1 ? 1 : shares > R ? R : shares;
+  if (p.prompt && shares < 8) shares = 8;
+  const dim3 join((unsigned)blocks, (unsigned)shares);
+  if (p.prompt)
+    hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kPromptRows, prompt_keys<D>()>), join, dim3(kJoinThreads), 0, s, args);
+  else
+    hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kRows, kTile>), join, dim3(kJoinThreads), 0, s, args);
   return check_hip(hipGetLastError(), "attention_kv4");
 }
 
@@ -675,10 +1054,9 @@ int launch_split(const AttentionKv4Args& a, hipStream_t s) {
 
 uint64_t attention_kv4_workspace(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int64_t window,
                                  int64_t sinks, int64_t max_kv_len) {
-  const Split p = plan(tokens, batch, heads, kv_heads, window, sinks, max_kv_len);
+  const Split p = plan(tokens, batch, heads, kv_heads, dim, window, sinks, max_kv_len);
   if (p.splits == 1) return 0;
-  const int64_t part = dim == 64 ? part_floats<64>() : dim == 128 ? part_floats<128>() : part_floats<256>();
-  return (uint64_t)p.tiles * kv_heads * p.splits * part * 4;
+  return (uint64_t)p.tiles * kv_heads * p.splits * (p.prompt ? kPromptRows : kRows) * (dim + 2) * 4;
 }
 
 int launch_attention_kv4(const AttentionKv4Args& a, hipStream_t s) {
