@@ -641,8 +641,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
   const AttentionKv4Args& a = args.a;
   constexpr int N = prompt_keys<D>(), KB = N / 32, KK = N / 16;     // keys; blocks of 32; steps of 16
   constexpr int S = D / 16, DB = D / 32;                            // steps of a score; blocks of d
-  constexpr int VU = KK * 2 * (D / 8);                              // units of V: 8 keys of 8 d
-  constexpr int KC = N * D / 32 / 128;                              // chunks of K of 16 bytes to a thread
   extern __shared__ __attribute__((aligned(1024))) char memory[];
   const int G = args.group;
   const int head = blockIdx.x % a.kv_heads;
@@ -703,17 +701,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
     qsum = sum * (fabsf(a.scale) * kLog2e);
   }
 
-  // Staging: threads 0 .. VU - 1 take a unit of V each, threads 128 .. 255 chunks of K, threads
-  // 128 .. 128 + N - 1 also the parameters of a key.
+  // Staging. A wave takes a group of 16 keys (D = 256: half of one's bytes), so that their page
+  // is the same for all its lanes: 16 (D = 64: 8) bytes of K codes a lane, and of V the 8 keys
+  // x 8 d of two 16-byte pieces to two (four) lanes, which turn a part of the d each.
   const int shift = a.pool.page_shift, page_size = 1 << shift, pages = (int)a.pool.pages, wide = (int)a.max_pages;
   const char* base = a.pool.base + head * Block<D>::bytes(page_size);
   const int32_t* table = a.page_table + rows.b * a.page_table_stride;
-  // (what follows from the thread's number is worked out anew for each tile: kept over the
-  // loop, it would take the registers of the results)
-  auto thread = [&]() {
-    int t = threadIdx.x;
-    asm volatile("" : "+v"(t));
-    return t;
+  constexpr int KL = D == 64 ? 2 : 4;                    // dwords of K to a lane
+  constexpr int VL = D == 64 ? 4 : 2;                    // lanes to a unit of V
+  const int group = D == 256 ? wave >> 1 : wave, part_of = D == 256 ? wave & 1 : 0;
+  // (a lane's places are worked out anew for each tile: kept over the loop, they would take the
+  // registers of the results)
+  struct Place {
+    int lane, v_h, v_w, k_row, k_c;
+  };
+  auto place = [&]() {
+    Place w;
+    w.lane = lane;
+    asm volatile("" : "+v"(w.lane));
+    const int unit = w.lane / VL + (D == 256 ? 32 * part_of : 0), piece = w.lane + 64 * part_of;
+    w.v_h = unit / (D / 8), w.v_w = unit % (D / 8);
+    w.k_row = piece / (D / 8 / KL), w.k_c = piece % (D / 8 / KL) * KL;
+    return w;
   };
   int pages_from = begin, page_ids = -1;
   auto fetch_pages = [&](int from) {
@@ -721,96 +730,82 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
     const int i = t < end ? (keys.key(t) + 16 * (lane % KK)) >> shift : wide;
     pages_from = from;
     page_ids = i < wide ? table[i] : -1;
+    asm volatile("" : "+v"(page_ids));
   };
-  u32x4 raw[2];
-  uint32_t raw_kp = 0, raw_vp = 0;
+  u32x4 raw_v[2];
+  uint32_t raw_k[KL], raw_p;
   int exist_next = 0;           // whether the pages of the fetched tile's groups of 16 keys exist
   auto fetch = [&](int t) {
-    const int key0 = keys.key(t), tid = thread();
-    const int v_kk = tid / (2 * (D / 8)), v_h = tid / (D / 8) & 1, v_w = tid % (D / 8);
     exist_next = (int)(__ballot((unsigned)page_ids < (unsigned)pages) >> ((t - pages_from) * KK)) & ((1 << KK) - 1);
-    auto block_of = [&](int group) -> const char* {
-      const int p = __shfl(page_ids, (t - pages_from) * KK + group);
-      return (unsigned)p < (unsigned)pages ? base + p * a.pool.page_stride : nullptr;
-    };
-    if (wave < 2) {
-      const char* block = block_of(v_kk & (KK - 1));
-      const int r = (key0 + 16 * v_kk + 4 * v_h) & (page_size - 1);
-      raw[0] = raw[1] = u32x4{0u, 0u, 0u, 0u};
-      if (block && tid < VU) {
-        raw[0] = *(const u32x4*)(block + Block<D>::v_dword(page_size, r, v_w));
-        raw[1] = *(const u32x4*)(block + Block<D>::v_dword(page_size, r + 8, v_w));
-      }
-    } else {
+    const int key = keys.key(t) + 16 * group;
+    // (what does not exist, and parameters that no row of the workgroup sees, count as zeros: what
+    // lies there may be NaN)
+    raw_v[0] = raw_v[1] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const int chunk = tid - 128 + 128 * i, k = chunk / (D / 32);
-        const char* block = block_of(k / 16);
-        raw[i] = u32x4{0u, 0u, 0u, 0u};
-        if (block)
-          raw[i] = *(const u32x4*)(block + Block<D>::k_row((key0 + k) & (page_size - 1)) + chunk % (D / 32) * 16);
+    for (int i = 0; i < KL; ++i) raw_k[i] = 0;
+    raw_p = 0;
+    if (exist_next >> group & 1) {
+      const Place w = place();
+      const int p = __builtin_amdgcn_readlane(page_ids, (t - pages_from) * KK + group);
+      const char* block = base + p * a.pool.page_stride;
+      const int r = key & (page_size - 1);
+      const char* k_at = block + Block<D>::k_row(r) + (w.k_row * (D / 2) + w.k_c * 4);
+      if constexpr (D == 64) {
+        const u32x2 v = *(const u32x2*)k_at;
+        raw_k[0] = v[0], raw_k[1] = v[1];
+      } else {
+        const u32x4 v = *(const u32x4*)k_at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw_k[i] = v[i];
       }
-      const int k = (tid - 128) & (N - 1);
-      const char* block = block_of(k / 16);
-      // (keys that no row of the workgroup sees count as zeros: what lies there may be NaN)
-      raw_kp = raw_vp = 0;
-      if (block && tid - 128 < N && key0 + k <= wg_hi) {
-        raw_kp = *(const uint32_t*)(block + Block<D>::k_params(page_size, (key0 + k) & (page_size - 1)));
-        raw_vp = *(const uint32_t*)(block + Block<D>::v_params(page_size, (key0 + k) & (page_size - 1)));
-      }
+      const char* v_at = block + Block<D>::v_dword(page_size, r, 0) + (w.v_h * (D / 8) * 16 + w.v_w * 16);
+      raw_v[0] = *(const u32x4*)v_at;
+      raw_v[1] = *(const u32x4*)(v_at + D / 8 * 32);
+      // (lanes 0..15: of K, 16..31: of V)
+      if (w.lane < 32 && key + (w.lane & 15) <= wg_hi)
+        raw_p = *(const uint32_t*)(block + Block<D>::k_params(page_size, r) + ((w.lane & 15) + (w.lane >> 4) * page_size) * 4);
     }
   };
   uint32_t bias_low, bias_high;
   asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(bias_low));
   asm volatile("v_mov_b32 %0, 0x54005400" : "=v"(bias_high));
-  float* scales = (float*)(memory + 2 * PromptLds<D>::kBytes);      // the largest scale of V in each buffer
+  float* scales = (float*)(memory + 2 * PromptLds<D>::kBytes);      // per buffer and wave the largest scale of V
+  // In LDS the d of a unit of V lie next to each other, turned by the unit, or the lanes that
+  // write them would meet in an eighth of the banks.
   auto stage = [&](int buffer) {
+    const Place w = place();
     char* to = memory + buffer * PromptLds<D>::kBytes;
-    const int tid = thread();
-    const int v_kk = tid / (2 * (D / 8)), v_h = tid / (D / 8) & 1, v_w = tid % (D / 8);
-    if (wave < 2) {
-      if (tid < VU) {
-        // 8 d of 8 keys: 16 bytes for each d, those of a thread next to each other. Their place is
-        // turned by the thread's block, or 64 threads would write to an eighth of the banks.
-        char* at = to + PromptLds<D>::kV + ((v_kk * DB + v_w / 4) * 64 + v_h * 32 + v_w % 4 * 8) * 16;
-        const int turn = (v_w & 3) + 4 * v_h;
-        auto byte = [&](auto which) {
-          constexpr int b = decltype(which)::value;
-          Frag even, odd;
+    char* k_to = to + ((group >> 1) * S * 64 + w.k_c / 2 * 64 + w.k_c % 2 * 32 + (group & 1) * 16 + w.k_row) * 16;
+    char* v_to = to + PromptLds<D>::kV + ((group * DB + w.v_w / 4) * 64 + w.v_h * 32 + w.v_w % 4 * 8) * 16;
+    const int turn = (w.v_w & 3) + 4 * w.v_h;
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            const uint32_t both = pair_bytes<b>(raw[p >> 1][2 * (p & 1)], raw[p >> 1][2 * (p & 1) + 1]);
-            even.h[p] = low_codes(both, bias_low);
-            odd.h[p] = high_codes(both, bias_high);
-          }
-          *(half8*)(at + ((2 * b) ^ turn) * 16) = even.f;
-          *(half8*)(at + ((2 * b + 1) ^ turn) * 16) = odd.f;
-        };
-        byte(std::integral_constant<int, 0>{});
-        byte(std::integral_constant<int, 1>{});
-        byte(std::integral_constant<int, 2>{});
-        byte(std::integral_constant<int, 3>{});
-      }
-    } else {
+    for (int i = 0; i < KL; ++i)
+      *(half8*)(k_to + (i / 2 * 64 + i % 2 * 32) * 16) = k_frag(raw_k[i]);      // (k_c is even)
 #pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const int chunk = tid - 128 + 128 * i, k = chunk / (D / 32), c = chunk % (D / 32) * 4;
+    for (int i = 0; i < 4 / VL; ++i) {
+      // Byte b of every token's dword: d = 2 b and 2 b + 1.
+      const int b = w.lane % VL * (4 / VL) + i;
+      const uint32_t select = 0x0C040C00u | b | (b << 16);
+      Frag even, odd;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *(half8*)(to + ((k / 32 * S + (c + j) / 2) * 64 + (c + j) % 2 * 32 + k % 32) * 16) = k_frag(raw[i][j]);
+      for (int p = 0; p < 4; ++p) {
+        const uint32_t both =
+            __builtin_amdgcn_perm(raw_v[p >> 1][2 * (p & 1) + 1], raw_v[p >> 1][2 * (p & 1)], select);
+        even.h[p] = low_codes(both, bias_low);
+        odd.h[p] = high_codes(both, bias_high);
       }
-      if (tid - 128 < N) {
-        const int k = tid - 128;
-        const half2v sm = as_half2(raw_vp);
-        half2v v;
-        v[0] = sm[0];
-        v[1] = (_Float16)fmaf((float)sm[0], 8.f, (float)sm[1]);
-        *(uint32_t*)(to + PromptLds<D>::kParams + k * 4) = raw_kp;
-        *(half2v*)(to + PromptLds<D>::kParams + N * 4 + k * 4) = v;
-        float most = (float)sm[0];
-        for (int m = 1; m < (N < 64 ? N : 64); m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-        if (k == 0) scales[buffer] = most;
-      }
+      *(half8*)(v_to + ((2 * b) ^ turn) * 16) = even.f;
+      *(half8*)(v_to + ((2 * b + 1) ^ turn) * 16) = odd.f;
+    }
+    if (part_of == 0) {
+      const half2v sm = as_half2(raw_p);
+      float most = (float)sm[0];
+      for (int m = 1; m < 16; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+      half2v v = sm;
+      if (lane >= 16) v[1] = (_Float16)fmaf((float)sm[0], 8.f, (float)sm[1]);
+      if (lane < 32)
+        *(half2v*)(to + PromptLds<D>::kParams + (lane >= 16 ? N * 4 : 0) + (16 * group + (lane & 15)) * 4) = v;
+      if (lane == 16) scales[4 * buffer + group] = most;
     }
   };
 
@@ -836,7 +831,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
     // (rows of this wave that see some of the tile: behind its last row there is nothing)
     if (!idle && key <= hi_pos) {
       const char* from = memory + buffer * PromptLds<D>::kBytes;
-      const float stop = fmaxf(scales[buffer], 0x1p-24f);
+      float stop = 0x1p-24f;
+#pragma unroll
+      for (int i = 0; i < KK; ++i) stop = fmaxf(stop, scales[4 * buffer + i]);
       const int stop_e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(stop));
       const bool whole = exist == (1 << KK) - 1 && key + N <= lo_pos + 1 && (!a.window || key > hi_pos - (int)a.window || key + N <= sinks);
       Frag p[KK];
