@@ -96,6 +96,18 @@ struct Keys {
 };
 
 __device__ inline float max4(float a, float b, float c, float d) { return fmaxf(fmaxf(a, b), fmaxf(c, d)); }
+// Over 16 lanes next to each other.
+template <int kControl>
+__device__ inline float dpp_max(float v) {
+  const int other = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), kControl, 0xF, 0xF, true);
+  return fmaxf(v, __builtin_bit_cast(float, other));
+}
+__device__ inline float row16_max(float v) {
+  v = dpp_max<0xB1>(v);            // lane ^ 1
+  v = dpp_max<0x4E>(v);            // lane ^ 2
+  v = dpp_max<0x141>(v);           // the other half of 8, mirrored
+  return dpp_max<0x140>(v);        // the other half of 16, mirrored
+}
 // Over the four lanes that share lane % 16.
 __device__ inline float across_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -611,6 +623,12 @@ __global__ __launch_bounds__(kJoinThreads) void attention_kv4_join_kernel(SplitA
 
 // ---------------------------------------------------------------------------
 // Many rows: prompts
+#ifndef PRI
+#define PRI 0
+#endif
+#ifndef OCC
+#define OCC 2
+#endif
 // ---------------------------------------------------------------------------
 
 constexpr int kPromptRows = 128;      // of a workgroup, 32 of each of its four waves
@@ -637,7 +655,7 @@ constexpr int prompt_lds_bytes() { return 2 * PromptLds<D>::kBytes + 64; }
 // score (three for scale and offset, one each for the largest, the sum, the offsets of V and
 // the operand, an exponential at a quarter of the rate).
 template <int D, typename T>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_kernel(SplitArgs args) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : OCC) void attention_kv4_prompt_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
   constexpr int N = prompt_keys<D>(), KB = N / 32, KK = N / 16;     // keys; blocks of 32; steps of 16
   constexpr int S = D / 16, DB = D / 32;                            // steps of a score; blocks of d
@@ -798,13 +816,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
       *(half8*)(v_to + ((2 * b + 1) ^ turn) * 16) = odd.f;
     }
     if (part_of == 0) {
-      const half2v sm = as_half2(raw_p);
+      // A key whose V row is not finite (in scale or offset) gets a K row that is not, and zeros
+      // for V: rows that see it have a NaN for their weight, for all others its weight is 0.
+      const bool broken = (raw_p & 0x7C00u) == 0x7C00u || (raw_p & 0x7C000000u) == 0x7C000000u;
+      const uint32_t all_broken = (uint32_t)__ballot(broken);
+      const half2v sm = as_half2(broken ? 0u : raw_p);
       float most = (float)sm[0];
-      for (int m = 1; m < 16; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-      half2v v = sm;
-      if (lane >= 16) v[1] = (_Float16)fmaf((float)sm[0], 8.f, (float)sm[1]);
+      most = row16_max(most);
+      uint32_t bits;
+      if (lane >= 16) {
+        half2v v = sm;
+        v[1] = (_Float16)fmaf((float)sm[0], 8.f, (float)sm[1]);
+        bits = __builtin_bit_cast(uint32_t, v);
+      } else {
+        bits = (all_broken | all_broken >> 16) >> lane & 1 ? 0x7E007E00u : raw_p;
+      }
       if (lane < 32)
-        *(half2v*)(to + PromptLds<D>::kParams + (lane >= 16 ? N * 4 : 0) + (16 * group + (lane & 15)) * 4) = v;
+        *(uint32_t*)(to + PromptLds<D>::kParams + (lane >= 16 ? N * 4 : 0) + (16 * group + (lane & 15)) * 4) = bits;
       if (lane == 16) scales[4 * buffer + group] = most;
     }
   };
@@ -812,7 +840,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
   floatx16 o[DB];
 #pragma unroll
   for (int i = 0; i < DB; ++i) o[i] = floatx16{};
-  float ref = -1e30f, l = 0.f, bias = 0.f;
+  float ref = 0.f, l = 0.f, bias = 0.f;
+  bool fresh = true;                   // no score yet
+  float limit = -INFINITY;             // what a score and the largest scale may come to
   const int below = a.window ? pos - (int)a.window : -1, sinks = a.window ? (int)a.sinks : 0;
   if (begin < end) {
     fetch_pages(begin);
@@ -829,97 +859,84 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
     }
     const int key = keys.key(tile);
     // (rows of this wave that see some of the tile: behind its last row there is nothing)
-    if (!idle && key <= hi_pos) {
-      const char* from = memory + buffer * PromptLds<D>::kBytes;
+    const bool works = !idle && key <= hi_pos;
+    const bool whole = exist == (1 << KK) - 1 && key + N <= lo_pos + 1 &&
+                       (!a.window || key > hi_pos - (int)a.window || key + N <= sinks);
+    const char* from = memory + buffer * PromptLds<D>::kBytes;
+    if (works) {
       float stop = 0x1p-24f;
 #pragma unroll
       for (int i = 0; i < KK; ++i) stop = fmaxf(stop, scales[4 * buffer + i]);
       const int stop_e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(stop));
-      const bool whole = exist == (1 << KK) - 1 && key + N <= lo_pos + 1 && (!a.window || key > hi_pos - (int)a.window || key + N <= sinks);
-      Frag p[KK];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        floatx16 s = {};
+        // Scores minus the row's reference. Element j of a lane: key 32 kb + 8 (j / 4) + 4 h + j % 4.
+        floatx16 x = {};
+        if (PRI) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < S; ++i)
-          s = F16Cfg::mfma(*(const half8*)(from + ((kb * S + i) * 64 + lane) * 16), qf[i].f, s);
-        __builtin_amdgcn_sched_barrier(0);
-        // Element j of a lane: key 32 kb + 8 (j / 4) + 4 h + j % 4.
-        float x[16];
-        uint32_t kp[16], vp[16];
+          x = F16Cfg::mfma(*(const half8*)(from + ((kb * S + i) * 64 + lane) * 16), qf[i].f, x);
+        if (PRI) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
-          const char* at = from + PromptLds<D>::kParams + (32 * kb + 2 * j + 4 * h) * 4;
-          const u32x4 kv = *(const u32x4*)at, vv = *(const u32x4*)(at + N * 4);
+          const u32x4 kp = *(const u32x4*)(from + PromptLds<D>::kParams + (32 * kb + 2 * j + 4 * h) * 4);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) kp[j + i] = kv[i], vp[j + i] = vv[i];
+          for (int i = 0; i < 4; ++i) {
+            const half2v sm = as_half2(kp[i]);
+            x[j + i] = fmaf((float)sm[0], x[j + i] * f, fmaf((float)sm[1], qsum, -ref));
+          }
         }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const half2v sm = as_half2(kp[j]);
-          s[j] *= f;
-          x[j] = fmaf((float)sm[0], s[j], fmaf((float)sm[1], qsum, -ref));
-        }
-        uint32_t seen = 0xFFFF;
         if (!whole) {
-          seen = 0;
           const int from_lane = key + 32 * kb + 4 * h;
           const int up_to = pos - from_lane, past = below - from_lane, sink = sinks - from_lane;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const int k = 8 * (j >> 2) + (j & 3);
             const bool yes = (k <= up_to) & ((k > past) | (k < sink)) & ((exist >> (2 * kb + j / 8) & 1) != 0);
-            seen |= yes ? 1u << j : 0u;
             x[j] = yes ? x[j] : -INFINITY;
-            vp[j] = yes ? vp[j] : 0u;
           }
         }
         float top = x[0];
 #pragma unroll
         for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
-        if (__ballot(top > (float)(kMost + 1 - stop_e))) {
-          float most = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const half2v sm = as_half2(kp[j]);
-            x[j] = fmaf((float)sm[0], s[j], (float)sm[1] * qsum);
-            x[j] = seen >> j & 1 ? x[j] : -INFINITY;
-            most = fmaxf(most, x[j]);
-          }
-          most = fmaxf(most, __shfl_xor(most, 32));
-          const float raised = fmaxf(ref, most + (float)(stop_e - 1 - kTarget));
-          const float factor = __builtin_amdgcn_exp2f(ref - raised);
+        if (__ballot(top > limit - (float)stop_e)) {
+          const float most = fmaxf(top, __shfl_xor(top, 32));
+          const float over = most + (float)(stop_e - 1 - kTarget);
+          // (a row's first scores set its reference, wherever they lie; later ones only raise it)
+          const float by = fresh ? (over > -INFINITY ? over : 0.f) : fmaxf(over, 0.f);
+          const float factor = fresh ? 1.f : __builtin_amdgcn_exp2f(-by);
+          if (over > -INFINITY) fresh = false, limit = (float)(kMost + 1);
           l *= factor;
           bias *= factor;
-          ref = raised;
+          ref += by;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) x[j] -= ref;
+          for (int j = 0; j < 16; ++j) x[j] -= by;
 #pragma unroll
           for (int i = 0; i < DB; ++i) o[i] *= factor;
-          if (kb > 0) {
+        }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int half = 0; half < 2; ++half) {
+          const int kk = 2 * kb + half;
+          Frag p;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) p[i].f[j] = (_Float16)((float)p[i].f[j] * factor);
+          for (int j = 0; j < 8; j += 4) {
+            const u32x4 vp = *(const u32x4*)(from + PromptLds<D>::kParams + (N + 16 * kk + 2 * j + 4 * h) * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const half2v sm = as_half2(vp[i]);
+              const float w = __builtin_amdgcn_exp2f(x[8 * half + j + i]);
+              l += w;
+              bias = fmaf(w, (float)sm[1], bias);
+              p.f[j + i] = (_Float16)fmaf(w, (float)sm[0], 0.f);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < DB; ++i) {
+            const int at = (kk * DB + i) * 64 + h * 32 + (n & 24) + ((n & 7) ^ ((n >> 3) + 4 * h));
+            o[i] = F16Cfg::mfma(*(const half8*)(from + PromptLds<D>::kV + at * 16), p.f, o[i]);
           }
         }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const half2v sm = as_half2(vp[j]);
-          const float w = __builtin_amdgcn_exp2f(x[j]);
-          l += w;
-          bias = fmaf(w, (float)sm[1], bias);
-          p[2 * kb + j / 8].f[j % 8] = (_Float16)(w * (float)sm[0]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-        for (int i = 0; i < DB; ++i) {
-          const int at = (kk * DB + i) * 64 + h * 32 + (n & 24) + ((n & 7) ^ ((n >> 3) + 4 * h));
-          o[i] = F16Cfg::mfma(*(const half8*)(from + PromptLds<D>::kV + at * 16), p[kk].f, o[i]);
-        }
     }
     if (more) stage(buffer ^ 1);
     __syncthreads();
@@ -939,7 +956,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
         *(float4*)(part + r * D + 32 * i + 2 * j + 4 * h) =
             make_float4(o[i][j] + bias, o[i][j + 1] + bias, o[i][j + 2] + bias, o[i][j + 3] + bias);
     if (h == 0) {
-      part[kPromptRows * D + r] = ref;
+      part[kPromptRows * D + r] = fresh ? -1e30f : ref;
       part[kPromptRows * (D + 1) + r] = l;
     }
     return;

@@ -129,7 +129,12 @@ def attention(q, cache, page, table, starts, kv_lens, kv_heads, scale, window=0,
             p = torch.where(seen[None], p, zero)
             total = p.sum(-1, keepdim=True)
             p = p / torch.where(total == 0, zero + 1, total)
-            out[rows] = (p @ v).transpose(0, 1)
+            # (a value that is not finite reaches the rows that see it, and no others)
+            broken = ~torch.isfinite(v).all(-1)
+            got = p @ torch.where(broken[:, None], zero, v)
+            got[:, (seen & broken[None]).any(-1)] = math.nan
+            out[rows] = got.transpose(0, 1)
+            size_v = torch.where(broken, zero, size_v)
             # scores: a sum of D products and the two terms of a key, each addition within 2^-24
             # of what the sum of all sizes can be
             score_off = (dim + 8) * 2.0**-24 * abs(scale) * x.abs().sum(-1, keepdim=True) * size_k[None]

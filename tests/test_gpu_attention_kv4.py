@@ -304,6 +304,25 @@ def test_sizes_of_values(uk, cuda, q_len):
     case.check(case.run(uk))
 
 
+@pytest.mark.parametrize("which", ["keys", "values"])
+@pytest.mark.parametrize("q_len", [1, 90])
+def test_rows_that_are_not_finite(uk, cuda, q_len, which):
+    """A cached row that was not finite (scale NaN) makes NaN of every query that sees it and of no
+    other: not of earlier ones in its tile, nor of those whose window has passed it."""
+    case = Case(17, F16, 4, 2, 64, 16, [q_len, q_len], [200, 210])
+    view = case.cache.view(case.pages, 2, -1)
+    at = (16 * 64 if which == "keys" else 16 * 68)
+    for token in (150, 197):
+        page = int(case.table[0, token // 16])
+        view[page, 1, at + token % 16 * 4:at + token % 16 * 4 + 4] = torch.tensor([0, 0x7E, 0, 0], dtype=torch.uint8)
+    for window, sinks in ((0, 0), (30, 0), (30, 151)):
+        out = case.run(uk, window=window, sinks=sinks)
+        case.check(out, window=window, sinks=sinks)
+        bad = torch.isnan(out[case.starts[0]:case.starts[1], :4 * 64]).view(q_len, 4, 64)
+        assert bool(bad[-1, 2:].all()) and not bool(bad[:, :2].any())
+    assert not bool(torch.isnan(out[case.starts[1]:case.starts[2]]).any())
+
+
 @pytest.mark.parametrize("heads,kv_heads,dim,kv_lens", [(8, 2, 128, [70001, 5, 20000]), (5, 1, 64, [40003]),
                                                         (2, 2, 256, [9000, 33])])
 def test_long_caches_are_split(uk, cuda, heads, kv_heads, dim, kv_lens):
