@@ -729,8 +729,9 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_kv4_page_bytes(int32_t page_size, int32_t kv_
  *   a' = a cos - b sin, b' = b cos + a sin      (cos_sin null: no rotation)
  * for the pairs (a, b) of y's first rotary_dim values (a multiple of 8), cos and sin
  * of pair i at cos_sin[position][i] and cos_sin[position][rotary_dim / 2 + i] of a
- * table of table_rows rows, positions[token] the position. Computed in 64 bits, rounded
- * to f32 and that to the rows' type. q goes to q_out, k to k_out (either may be its input's own buffer, with the
+ * table of table_rows rows, positions[token] the position. Computed in f32,
+ * and for k with a cache in 64 bits and rounded to f32; that is rounded to the rows'
+ * type. q goes to q_out, k to k_out (either may be its input's own buffer, with the
  * same stride; k_out may be null with a cache). With a cache, the rounded k row and
  * the v row of token t are stored at slots[t]. q, or k and v, may be null: nothing is
  * done for them. Weights have the rows' type. A token whose position lies outside the

@@ -5,6 +5,8 @@
 #include "uk_common.h"
 #include "uk_kv4.h"
 
+#include <type_traits>
+
 namespace uk {
 namespace {
 using namespace kv4;
@@ -15,20 +17,34 @@ constexpr int kBlock = 256;
 // qk_norm_rope
 // ---------------------------------------------------------------------------
 
-// Sums and extrema over the L = D / 8 lanes that hold a row.
-template <int L>
-__device__ inline double row_sum(double v) {
-  for (int m = 1; m < L; m *= 2) v += __shfl_xor(v, m);
-  return v;
+// A value of the lane at the other end of one step of a reduction over L lanes: within 16 lanes
+// through the vector unit's own exchange (lane ^ 1, lane ^ 2, the mirrors of 8 and of 16), the
+// last step of 32 lanes through LDS.
+template <int kStep>
+__device__ inline float other_lane(float v) {
+  if constexpr (kStep == 4) {
+    return __shfl_xor(v, 16);
+  } else {
+    constexpr int control = kStep == 0 ? 0xB1 : kStep == 1 ? 0x4E : kStep == 2 ? 0x141 : 0x140;
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), control, 0xF, 0xF, true));
+  }
 }
-template <int L>
-__device__ inline float row_min(float v) {
-  for (int m = 1; m < L; m *= 2) v = fminf(v, __shfl_xor(v, m));
-  return v;
+template <int kStep>
+__device__ inline double other_lane(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const float lo = other_lane<kStep>(__builtin_bit_cast(float, (uint32_t)u));
+  const float hi = other_lane<kStep>(__builtin_bit_cast(float, (uint32_t)(u >> 32)));
+  return __builtin_bit_cast(double, (uint64_t)__builtin_bit_cast(uint32_t, lo) |
+                                        ((uint64_t)__builtin_bit_cast(uint32_t, hi) << 32));
 }
-template <int L>
-__device__ inline float row_max(float v) {
-  for (int m = 1; m < L; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
+// f over the L = 8, 16 or 32 lanes of a row, the same in all of them.
+template <int L, typename V, typename F>
+__device__ inline V over_row(V v, F f) {
+  v = f(v, other_lane<0>(v));
+  v = f(v, other_lane<1>(v));
+  v = f(v, other_lane<2>(v));
+  if constexpr (L > 8) v = f(v, other_lane<3>(v));
+  if constexpr (L > 16) v = f(v, other_lane<4>(v));
   return v;
 }
 
@@ -37,119 +53,153 @@ struct Params {
   uint32_t code[8];
 };
 
-// Codes of a row, 8 values a lane. A code is decided on x - offset against (code +- 1/2)
-// scale, both exact in 64 bits, so that ties go to the even code and a value next to a
-// border falls on its own side, whatever the estimate in 32 bits said.
+// Codes of a row, 8 values a lane. An estimate in f32 is off by less than 2^-18 of a code; a value
+// that lies within 2^-16 of a border between two codes (one wave in a hundred has one, if values
+// are not on a lattice) is decided by comparing x - offset with (code +- 1/2) scale in 64 bits,
+// which is exact, ties to the even code.
 template <int L>
 __device__ inline Params quantise(const float* x) {
-  float lo = x[0], hi = x[0];
-  bool finite = true;
+  float lo = x[0], hi = x[0], size = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
-    finite = finite && fabsf(x[i]) < INFINITY;
+    size += x[i] * 0.f;            // 0, or NaN where a value is not finite
   }
-  lo = row_min<L>(lo);
-  hi = row_max<L>(hi);
-  const float bad = row_max<L>(finite ? 0.f : 1.f);
+  lo = over_row<L>(lo, [](float a, float b) { return fminf(a, b); });
+  hi = over_row<L>(hi, [](float a, float b) { return fmaxf(a, b); });
+  const float bad = over_row<L>(size == 0.f ? 0.f : 1.f, [](float a, float b) { return fmaxf(a, b); });
   const _Float16 offset = (_Float16)fminf(fmaxf(lo, -65504.f), 65504.f);
   const double range = (double)hi - (double)lo;
   const _Float16 step = (_Float16)fminf((float)(range / 15.0), 65504.f);
   Params p;
   const float s = (float)step, m = (float)offset, inv = s > 0.f ? 1.f / s : 0.f;
+  float c[8];
+  bool near = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float c = fminf(fmaxf(rintf((x[i] - m) * inv), 0.f), 15.f);
-    const double rest = fma(-(double)c, (double)s, (double)x[i] - (double)m), half = 0.5 * (double)s;
-    const bool odd = ((int)c & 1) != 0;
-    if (rest > half || (rest == half && odd)) c += 1.f;
-    if (rest < -half || (rest == -half && odd)) c -= 1.f;
-    p.code[i] = s > 0.f && bad == 0.f ? (uint32_t)fminf(fmaxf(c, 0.f), 15.f) : 0u;
+    const float t = (x[i] - m) * inv;
+    c[i] = rintf(t);
+    near = near || fabsf(fabsf(t - c[i]) - 0.5f) < 0x1p-16f;
+    c[i] = fminf(fmaxf(c[i], 0.f), 15.f);
   }
+  if (near) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double rest = fma(-(double)c[i], (double)s, (double)x[i] - (double)m), half = 0.5 * (double)s;
+      const bool odd = ((int)c[i] & 1) != 0;
+      const float up = rest > half || (rest == half && odd) ? 1.f : 0.f;
+      const float down = rest < -half || (rest == -half && odd) ? 1.f : 0.f;
+      c[i] = fminf(fmaxf(c[i] + up - down, 0.f), 15.f);
+    }
+  }
+  const bool stored = s > 0.f && bad == 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p.code[i] = stored ? (uint32_t)c[i] : 0u;
   p.bits = bad == 0.f ? (uint32_t)__builtin_bit_cast(uint16_t, step) |
                             ((uint32_t)__builtin_bit_cast(uint16_t, offset) << 16)
                       : 0x00007E00u;   // scale NaN, offset 0
   return p;
 }
 
-// A group of L lanes takes `kRows` consecutive head rows of one token (query heads, then
-// key heads, then value heads), so that it reads the token's cosines once. A lane holds two
-// runs of four values: of a rotated row d = 4 i .. and rotary / 2 + 4 i .., the two halves
-// of its pairs, so that the rotation needs no exchange between lanes; else d = 8 i .. + 8.
-// Norm and rotation run in 64 bits: with a cache, the key is about to be compared with the
-// borders between its codes, and the vector unit has the time (the launch is bound by
-// memory either way).
-template <int D, typename T, int kRows>
-__global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(QkNormRopeArgs a, int q_rows, int k_rows, int rows,
-                                                              int chunks) {
+__device__ inline float inverse_root(float v) { return rsqrtf(v); }
+__device__ inline double inverse_root(double v) { return 1.0 / sqrt(v); }
+
+enum RowKind { kQuery, kKey, kCachedKey, kValue };
+
+// A group of L lanes takes kRows consecutive head rows of one token, so that it reads the token's
+// cosines once, and has all of their loads in flight. A lane holds two runs of four values: of a
+// rotated row d = 4 i .. and rotary / 2 + 4 i .., the two halves of its pairs, so that the rotation
+// needs no exchange between lanes; else d = 8 i .. + 8. Norm and rotation run in f32, in 64 bits for
+// a key that goes into the cache: it is about to be compared with the borders between its codes, and
+// which side of one it falls on should not depend on an order of additions.
+template <int D, typename T, RowKind kKind, int kRows>
+__device__ inline void rows_body(const QkNormRopeArgs& a, int64_t block) {
   constexpr int L = D / 8;
+  typedef typename std::conditional<kKind == kCachedKey, double, float>::type Wide;
+  constexpr bool kTurned = kKind != kValue, kStored = kKind == kCachedKey || kKind == kValue;
+  const int heads = kKind == kQuery ? a.heads : a.kv_heads;
+  const int chunks = (heads + kRows - 1) / kRows;
   const int lane = threadIdx.x % L;
-  const int64_t group = (int64_t)blockIdx.x * (kBlock / L) + threadIdx.x / L;
+  const int64_t group = block * (kBlock / L) + threadIdx.x / L;
   const int64_t token = group / chunks;
   if (token >= a.tokens) return;
-  const int first = (int)(group % chunks) * kRows;
+  const int first = (int)(group - token * chunks) * kRows;
+  const bool lane_turns = kTurned && a.cos_sin && lane < a.rotary / 8;
+  const bool halves = lane_turns && !a.interleaved;
+  const int d0 = halves ? lane * 4 : lane * 8, d1 = halves ? a.rotary / 2 + lane * 4 : lane * 8 + 4;
+  const uint16_t* src = kKind == kQuery   ? (const uint16_t*)a.q + token * a.q_stride
+                        : kKind == kValue ? (const uint16_t*)a.v + token * a.v_stride
+                                          : (const uint16_t*)a.k + token * a.k_stride;
+  uint2 raw[kRows][2];
+#pragma unroll
+  for (int j = 0; j < kRows; ++j) {
+    const int head = first + j < heads ? first + j : heads - 1;
+    raw[j][0] = *(const uint2*)(src + (int64_t)head * D + d0);
+    raw[j][1] = *(const uint2*)(src + (int64_t)head * D + d1);
+  }
   float cs[8];
   if (a.cos_sin) {
     const int64_t position = a.positions[token];
     if (position < 0 || position >= a.table_rows) return;
-    if (lane < a.rotary / 8) {
+    if (lane_turns) {
       const float* at = a.cos_sin + position * a.rotary + lane * 4;
       *(float4*)cs = *(const float4*)at;
       const float* sin_at = at + a.rotary / 2;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cs[4 + i] = sin_at[i];
+      *(float4*)(cs + 4) = *(const float4*)sin_at;
     }
   }
-  const bool turns = a.cos_sin && lane < a.rotary / 8;
-  const bool halves = turns && !a.interleaved;
+  const uint16_t* weight = kTurned ? (const uint16_t*)(kKind == kQuery ? a.q_weight : a.k_weight) : nullptr;
+  float w[8];
+  if (weight) {
+    widen4<T>(*(const uint2*)(weight + d0), w);
+    widen4<T>(*(const uint2*)(weight + d1), w + 4);
+  }
+  int64_t slot = 0;
+  if (kStored) slot = a.slots[token];
+  const int page = 1 << a.pool.page_shift, at = (int)(slot & (page - 1));
+  const bool exists = slot >= 0 && (slot >> a.pool.page_shift) < a.pool.pages;
 #pragma unroll
   for (int j = 0; j < kRows; ++j) {
-    const int row = first + j;
-    if (row >= rows) return;
-    const bool is_q = row < q_rows, is_k = !is_q && row < q_rows + k_rows;
-    const int head = is_q ? row : is_k ? row - q_rows : row - q_rows - k_rows;
-    const uint16_t* src = is_q  ? (const uint16_t*)a.q + token * a.q_stride
-                          : is_k ? (const uint16_t*)a.k + token * a.k_stride
-                                 : (const uint16_t*)a.v + token * a.v_stride;
-    src += (int64_t)head * D;
-    const int d0 = halves && (is_q || is_k) ? lane * 4 : lane * 8;
-    const int d1 = halves && (is_q || is_k) ? a.rotary / 2 + lane * 4 : lane * 8 + 4;
+    const int head = first + j;
+    if (head >= heads) return;
     float x[8];
-    widen4<T>(*(const uint2*)(src + d0), x);
-    widen4<T>(*(const uint2*)(src + d1), x + 4);
-    if (is_q || is_k) {
-      double y[8];
+    widen4<T>(raw[j][0], x);
+    widen4<T>(raw[j][1], x + 4);
+    if constexpr (kTurned) {
+      Wide y[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = x[i];
-      const uint16_t* weight = (const uint16_t*)(is_q ? a.q_weight : a.k_weight);
       if (weight) {
-        double sum = 0;
+        Wide sum = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fma(y[i], y[i], sum);
-        sum = row_sum<L>(sum);
-        const double r = 1.0 / sqrt(sum / D + (double)a.eps);
-        float w[8];
-        widen4<T>(*(const uint2*)(weight + d0), w);
-        widen4<T>(*(const uint2*)(weight + d1), w + 4);
+        for (int i = 0; i < 8; ++i) sum = y[i] * y[i] + sum;
+        sum = over_row<L>(sum, [](Wide u, Wide v) { return u + v; });
+        const Wide r = inverse_root(sum * (Wide)(1.0 / D) + (Wide)a.eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] * r * (double)w[i];
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * r * (Wide)w[i];
       }
-      if (turns) {
+      if (lane_turns) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int p = a.interleaved ? 2 * i : i, q = a.interleaved ? 2 * i + 1 : i + 4;
-          const double c = cs[i], s = cs[4 + i], u = y[p], v = y[q];
-          y[p] = u * c - v * s;
-          y[q] = v * c + u * s;
+          const Wide c = cs[i], s = cs[4 + i];
+          if (a.interleaved) {
+            const Wide u = y[2 * i], v = y[2 * i + 1];
+            y[2 * i] = u * c - v * s;
+            y[2 * i + 1] = v * c + u * s;
+          } else {
+            const Wide u = y[i], v = y[i + 4];
+            y[i] = u * c - v * s;
+            y[i + 4] = v * c + u * s;
+          }
         }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = (float)y[i];
       const uint2 r0 = narrow4<T>(x), r1 = narrow4<T>(x + 4);
-      uint16_t* dst = is_q     ? (uint16_t*)a.q_out + token * a.q_out_stride
-                      : a.k_out ? (uint16_t*)a.k_out + token * a.k_out_stride
-                                : nullptr;
+      uint16_t* dst = kKind == kQuery ? (uint16_t*)a.q_out + token * a.q_out_stride
+                      : a.k_out       ? (uint16_t*)a.k_out + token * a.k_out_stride
+                                      : nullptr;
       if (dst) {
         *(uint2*)(dst + (int64_t)head * D + d0) = r0;
         *(uint2*)(dst + (int64_t)head * D + d1) = r1;
@@ -157,38 +207,47 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(QkNormRopeArgs a, 
       widen4<T>(r0, x);
       widen4<T>(r1, x + 4);
     }
-    if (is_q || !a.pool.base) continue;
-    const int64_t slot = a.slots[token];
-    const int page = 1 << a.pool.page_shift, at = (int)(slot & (page - 1));
-    const Params p = quantise<L>(x);
-    if (slot < 0 || (slot >> a.pool.page_shift) >= a.pool.pages) continue;
-    char* block = a.pool.base + (slot >> a.pool.page_shift) * a.pool.page_stride + head * Block<D>::bytes(page);
-    uint32_t low = 0, high = 0;
+    if constexpr (kStored) {
+      const Params p = quantise<L>(x);
+      if (!exists) continue;
+      char* to = a.pool.base + (slot >> a.pool.page_shift) * a.pool.page_stride + head * Block<D>::bytes(page);
+      uint32_t low = 0, high = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      low |= p.code[i] << (4 * i);
-      high |= p.code[4 + i] << (4 * i);
-    }
-    if (is_k) {
-      *(uint16_t*)(block + Block<D>::k_row(at) + d0 / 2) = (uint16_t)low;
-      *(uint16_t*)(block + Block<D>::k_row(at) + d1 / 2) = (uint16_t)high;
-      if (lane == 0) *(uint32_t*)(block + Block<D>::k_params(page, at)) = p.bits;
-    } else {
-      *(uint32_t*)(block + Block<D>::v_dword(page, at, lane)) = low | (high << 16);
-      if (lane == 0) *(uint32_t*)(block + Block<D>::v_params(page, at)) = p.bits;
+      for (int i = 0; i < 4; ++i) {
+        low |= p.code[i] << (4 * i);
+        high |= p.code[4 + i] << (4 * i);
+      }
+      if (kKind == kCachedKey) {
+        *(uint16_t*)(to + Block<D>::k_row(at) + d0 / 2) = (uint16_t)low;
+        *(uint16_t*)(to + Block<D>::k_row(at) + d1 / 2) = (uint16_t)high;
+        if (lane == 0) *(uint32_t*)(to + Block<D>::k_params(page, at)) = p.bits;
+      } else {
+        *(uint32_t*)(to + Block<D>::v_dword(page, at, lane)) = low | (high << 16);
+        if (lane == 0) *(uint32_t*)(to + Block<D>::v_params(page, at)) = p.bits;
+      }
     }
   }
 }
 
+// The first q_blocks workgroups take queries, the next k_blocks keys, the others values.
+template <int D, typename T, int kRows>
+__global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(QkNormRopeArgs a, int64_t q_blocks, int64_t k_blocks) {
+  const int64_t block = blockIdx.x;
+  if (block < q_blocks) rows_body<D, T, kQuery, kRows>(a, block);
+  else if (block >= q_blocks + k_blocks) rows_body<D, T, kValue, kRows>(a, block - q_blocks - k_blocks);
+  else if (a.pool.base) rows_body<D, T, kCachedKey, kRows>(a, block - q_blocks);
+  else rows_body<D, T, kKey, kRows>(a, block - q_blocks);
+}
+
 template <int D, typename T, int kRows>
 int launch_rows(const QkNormRopeArgs& a, hipStream_t s) {
-  const int q_rows = a.q ? a.heads : 0, k_rows = a.k ? a.kv_heads : 0;
-  const int rows = q_rows + k_rows + (a.pool.base ? a.kv_heads : 0);
-  const int chunks = (int)ceil_div(rows, kRows);
-  const int64_t blocks = ceil_div(a.tokens * chunks, kBlock / (D / 8));
+  constexpr int kGroups = kBlock / (D / 8);
+  const int64_t q_blocks = a.q ? ceil_div(a.tokens * ceil_div(a.heads, kRows), kGroups) : 0;
+  const int64_t kv_blocks = ceil_div(a.tokens * ceil_div(a.kv_heads, kRows), kGroups);
+  const int64_t blocks = q_blocks + (a.k ? kv_blocks : 0) + (a.pool.base ? kv_blocks : 0);
   if (blocks > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "qk_norm_rope: too many rows for one call");
-  hipLaunchKernelGGL((qk_norm_rope_kernel<D, T, kRows>), dim3((unsigned)blocks), dim3(kBlock), 0, s, a, q_rows, k_rows,
-                     rows, chunks);
+  hipLaunchKernelGGL((qk_norm_rope_kernel<D, T, kRows>), dim3((unsigned)blocks), dim3(kBlock), 0, s, a, q_blocks,
+                     a.k ? kv_blocks : 0);
   return check_hip(hipGetLastError(), "qk_norm_rope");
 }
 
