@@ -7,6 +7,7 @@ device memory, sizes are given, strides default to tight, and work is enqueued o
 torch's current stream; every tensor lies on the current device.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -17,13 +18,25 @@ from .ukernel import _check, _stream
 _ROW_TYPES = {F.ATTENTION_TYPE_F16: torch.float16, F.ATTENTION_TYPE_BF16: torch.bfloat16}
 
 
-def _tensor(t, dtype, name):
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _device():
+    # (-1 is what a CPU tensor says: it matches no device)
+    try:
+        return _get_device()
+    except RuntimeError:
+        return -2
+
+
+def _tensor(t, dtype, name, device):
     """Address of a tensor of that type on the current device; None stays None."""
     if t is None:
         return None
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+    where = t.get_device()
+    if where != device or where < 0:
         raise ValueError(f"{name} must be a tensor on the current CUDA (HIP) device")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
     return t.data_ptr()
 
@@ -46,32 +59,34 @@ def qk_norm_rope(q, k, q_out, k_out, tokens, heads, kv_heads, head_dim, flags, *
     """RMS norm and rotation of every query and key head; with ``cache``, keys and values
     go into the 4-bit cache at ``slots`` in the same launch. ``q``, or ``k`` and ``v``, may
     be None, and with a cache ``k_out`` too."""
-    rows = _row_type(flags)
-    if cache is not None and page_stride is None:
-        page_stride = kv4_page_bytes(page_size, kv_heads, head_dim)
+    rows, device = _row_type(flags), _device()
+    if page_stride is None:
+        page_stride = kv_heads * page_size * (head_dim + 8)
     q_row, kv_row = heads * head_dim, kv_heads * head_dim
     _check(load_library().iree_amd_uk_qk_norm_rope(
-        _tensor(q, rows, "q"), q_row if q_stride0 is None else q_stride0,
-        _tensor(k, rows, "k"), kv_row if k_stride0 is None else k_stride0,
-        _tensor(v, rows, "v"), kv_row if v_stride0 is None else v_stride0,
-        _tensor(q_out, rows, "q_out"), q_row if q_out_stride0 is None else q_out_stride0,
-        _tensor(k_out, rows, "k_out"), kv_row if k_out_stride0 is None else k_out_stride0,
-        _tensor(q_weight, rows, "q_weight"), _tensor(k_weight, rows, "k_weight"), eps,
-        _tensor(cos_sin, torch.float32, "cos_sin"), table_rows, rotary_dim,
-        _tensor(positions, torch.int32, "positions"), _tensor(cache, None, "cache"), pages, page_stride or 0,
-        page_size, _tensor(slots, torch.int64, "slots"), tokens, heads, kv_heads, head_dim, flags, _stream(stream)))
+        _tensor(q, rows, "q", device), q_row if q_stride0 is None else q_stride0,
+        _tensor(k, rows, "k", device), kv_row if k_stride0 is None else k_stride0,
+        _tensor(v, rows, "v", device), kv_row if v_stride0 is None else v_stride0,
+        _tensor(q_out, rows, "q_out", device), q_row if q_out_stride0 is None else q_out_stride0,
+        _tensor(k_out, rows, "k_out", device), kv_row if k_out_stride0 is None else k_out_stride0,
+        _tensor(q_weight, rows, "q_weight", device), _tensor(k_weight, rows, "k_weight", device), eps,
+        _tensor(cos_sin, torch.float32, "cos_sin", device), table_rows, rotary_dim,
+        _tensor(positions, torch.int32, "positions", device), _tensor(cache, None, "cache", device), pages,
+        page_stride, page_size, _tensor(slots, torch.int64, "slots", device), tokens, heads, kv_heads, head_dim, flags,
+        _stream(stream)))
 
 
 def kv4_read(cache, pages, page_size, slots, k_out, v_out, rows, kv_heads, head_dim, flags, *, page_stride=None,
              k_out_stride0=None, v_out_stride0=None, stream=None):
     """The K and V rows that the cache holds at ``slots``; ``k_out`` or ``v_out`` may be None."""
-    kind, row = _row_type(flags), kv_heads * head_dim
+    kind, row, device = _row_type(flags), kv_heads * head_dim, _device()
     if page_stride is None:
-        page_stride = kv4_page_bytes(page_size, kv_heads, head_dim)
+        page_stride = kv_heads * page_size * (head_dim + 8)
     _check(load_library().iree_amd_uk_kv4_read(
-        _tensor(cache, None, "cache"), pages, page_stride, page_size, _tensor(slots, torch.int64, "slots"),
-        _tensor(k_out, kind, "k_out"), row if k_out_stride0 is None else k_out_stride0,
-        _tensor(v_out, kind, "v_out"), row if v_out_stride0 is None else v_out_stride0, rows, kv_heads, head_dim,
+        _tensor(cache, None, "cache", device), pages, page_stride, page_size,
+        _tensor(slots, torch.int64, "slots", device),
+        _tensor(k_out, kind, "k_out", device), row if k_out_stride0 is None else k_out_stride0,
+        _tensor(v_out, kind, "v_out", device), row if v_out_stride0 is None else v_out_stride0, rows, kv_heads, head_dim,
         flags, _stream(stream)))
 
 
@@ -83,6 +98,13 @@ def attention_kv4_workspace(tokens, batch, heads, kv_heads, head_dim, *, max_kv_
     return out.value
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(device, tokens, batch, heads, kv_heads, head_dim, window, sinks, max_kv_len):
+    # (it follows from the sizes and the device alone, and a decode step asks again and again)
+    return attention_kv4_workspace(tokens, batch, heads, kv_heads, head_dim, max_kv_len=max_kv_len, window=window,
+                                   sinks=sinks)
+
+
 def attention_kv4(q, out, cache, pages, page_size, page_table, q_starts, kv_lens, tokens, batch, heads, kv_heads,
                   head_dim, max_pages, flags, *, scale, window=0, sinks=0, max_kv_len=None, page_stride=None,
                   page_table_stride=None, q_stride0=None, out_stride0=None, workspace=None, stream=None):
@@ -90,25 +112,26 @@ def attention_kv4(q, out, cache, pages, page_size, page_table, q_starts, kv_lens
     causal, optionally with a sliding window and ``sinks`` first tokens that stay visible.
     ``max_kv_len``: the longest of ``kv_lens`` as far as the caller knows. Without a
     ``workspace`` the call takes one from torch's allocator for its own duration."""
-    kind, row = _row_type(flags), heads * head_dim
+    kind, row, device = _row_type(flags), heads * head_dim, _device()
     if page_stride is None:
-        page_stride = kv4_page_bytes(page_size, kv_heads, head_dim)
-    if max_kv_len is None:
-        max_kv_len = max_pages * page_size
-    where = _tensor(q, kind, "q")
+        page_stride = kv_heads * page_size * (head_dim + 8)
+    capacity = max_pages * page_size
+    max_kv_len = capacity if max_kv_len is None else min(max_kv_len, capacity)
+    where = _tensor(q, kind, "q", device)
     if workspace is None:
-        nbytes = attention_kv4_workspace(tokens, batch, heads, kv_heads, head_dim, max_kv_len=max_kv_len,
-                                         window=window, sinks=sinks)
+        nbytes = _workspace_bytes(device, tokens, batch, heads, kv_heads, head_dim, window, sinks, max_kv_len)
         if nbytes:
             workspace = _workspace(nbytes, stream)
     _check(load_library().iree_amd_uk_attention_kv4(
         where, row if q_stride0 is None else q_stride0,
-        _tensor(out, kind, "out"), row if out_stride0 is None else out_stride0,
-        _tensor(cache, None, "cache"), pages, page_stride, page_size,
-        _tensor(page_table, torch.int32, "page_table"), max_pages if page_table_stride is None else page_table_stride,
-        max_pages, _tensor(q_starts, torch.int32, "q_starts"), _tensor(kv_lens, torch.int32, "kv_lens"), tokens, batch,
-        heads, kv_heads, head_dim, scale, window, sinks, max_kv_len, _tensor(workspace, None, "workspace"),
-        0 if workspace is None else workspace.numel() * workspace.element_size(), flags, _stream(stream)))
+        _tensor(out, kind, "out", device), row if out_stride0 is None else out_stride0,
+        _tensor(cache, None, "cache", device), pages, page_stride, page_size,
+        _tensor(page_table, torch.int32, "page_table", device),
+        max_pages if page_table_stride is None else page_table_stride, max_pages,
+        _tensor(q_starts, torch.int32, "q_starts", device), _tensor(kv_lens, torch.int32, "kv_lens", device), tokens,
+        batch, heads, kv_heads, head_dim, scale, window, sinks, max_kv_len,
+        _tensor(workspace, None, "workspace", device), 0 if workspace is None else workspace.nbytes, flags,
+        _stream(stream)))
 
 
 def _workspace(nbytes, stream):
@@ -124,11 +147,11 @@ def _workspace(nbytes, stream):
 def copy_pages(pool, pages, page_bytes, src, dst, *, page_stride=None, stream=None):
     """Page ``src[i]`` to page ``dst[i]`` inside a pool; ``src`` and ``dst`` are page
     numbers on the host (int32 CPU tensors, or sequences)."""
-    src, dst = _host_pages(src), _host_pages(dst)
+    src, dst, device = _host_pages(src), _host_pages(dst), _device()
     if src.numel() != dst.numel():
         raise ValueError("src and dst must have as many pages")
     _check(load_library().iree_amd_uk_copy_pages(
-        _tensor(pool, None, "pool"), pages, page_bytes, page_bytes if page_stride is None else page_stride,
+        _tensor(pool, None, "pool", device), pages, page_bytes, page_bytes if page_stride is None else page_stride,
         src.data_ptr(), dst.data_ptr(), src.numel(), _stream(stream)))
 
 

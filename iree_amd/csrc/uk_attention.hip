@@ -187,8 +187,6 @@ __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 union Frag {
   uint32_t u[4];
@@ -281,9 +279,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
     float x[D / 4], top = 0.f, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 4; i += 8) {
-      const uint4 w = *(const uint4*)(q + i);
-      widen4<T>(make_uint2(w.x, w.y), x + i);
-      widen4<T>(make_uint2(w.z, w.w), x + i + 4);
+      const u32x4 w = *(const u32x4*)(q + i);
+      widen4<T>(u32x2{w.x, w.y}, x + i);
+      widen4<T>(u32x2{w.z, w.w}, x + i + 4);
     }
     const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
@@ -555,9 +553,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = total != 0.f ? v[j] / total : 0.f;
-    const uint2 r0 = narrow4<T>(v), r1 = narrow4<T>(v + 4);
+    const u32x2 r0 = narrow4<T>(v), r1 = narrow4<T>(v + 4);
     uint16_t* out = (uint16_t*)a.out + (int64_t)(rows.token0 + mine / G) * a.out_stride + (int64_t)(head * G + mine % G) * D + d;
-    *(uint4*)out = make_uint4(r0.x, r0.y, r1.x, r1.y);
+    *(u32x4*)out = u32x4{r0.x, r0.y, r1.x, r1.y};
   }
 }
 
@@ -615,7 +613,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_kv4_join_kernel(SplitA
       for (int j = 0; j < 4; ++j) v[j] = total != 0.f ? v[j] / total : 0.f;
       const int row = rows.first + r;
       uint16_t* out = (uint16_t*)a.out + (int64_t)(rows.token0 + row / G) * a.out_stride + (int64_t)(head * G + row % G) * D + d;
-      *(uint2*)out = narrow4<T>(v);
+      *(u32x2*)out = narrow4<T>(v);
     }
     __syncthreads();
   }
@@ -970,7 +968,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : OCC) void attention_kv4_prompt_
       float v[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = (o[i][j + k] + bias) * inverse;
-      *(uint2*)(out + 32 * i + 2 * j + 4 * h) = narrow4<T>(v);
+      *(u32x2*)(out + 32 * i + 2 * j + 4 * h) = narrow4<T>(v);
     }
 }
 

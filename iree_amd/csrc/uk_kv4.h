@@ -24,6 +24,11 @@ struct Block {
   __device__ static int v_params(int page, int row) { return page * (D + 4) + row * 4; }
 };
 
+// (Not HIP's structs of the same sizes: arrays of those do not stay in registers, and the
+// compiler takes reads of them from LDS for possible readers of every load into LDS on its way.)
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // One row value. (bf16 is handled as bits: widening is a shift, narrowing rounds to the
 // nearest, ties to even, and keeps NaN.)
 struct F16 {
@@ -47,15 +52,15 @@ struct BF16 {
 };
 
 template <typename T>
-__device__ inline void widen4(uint2 w, float* x) {
+__device__ inline void widen4(u32x2 w, float* x) {
   x[0] = T::widen(w.x & 0xFFFFu);
   x[1] = T::widen(w.x >> 16);
   x[2] = T::widen(w.y & 0xFFFFu);
   x[3] = T::widen(w.y >> 16);
 }
 template <typename T>
-__device__ inline uint2 narrow4(const float* x) {
-  return make_uint2(T::narrow(x[0]) | (T::narrow(x[1]) << 16), T::narrow(x[2]) | (T::narrow(x[3]) << 16));
+__device__ inline u32x2 narrow4(const float* x) {
+  return u32x2{T::narrow(x[0]) | (T::narrow(x[1]) << 16), T::narrow(x[2]) | (T::narrow(x[3]) << 16)};
 }
 
 }  // namespace kv4

@@ -131,12 +131,12 @@ __device__ inline void rows_body(const QkNormRopeArgs& a, int64_t block) {
   const uint16_t* src = kKind == kQuery   ? (const uint16_t*)a.q + token * a.q_stride
                         : kKind == kValue ? (const uint16_t*)a.v + token * a.v_stride
                                           : (const uint16_t*)a.k + token * a.k_stride;
-  uint2 raw[kRows][2];
+  u32x2 raw[kRows][2];
 #pragma unroll
   for (int j = 0; j < kRows; ++j) {
     const int head = first + j < heads ? first + j : heads - 1;
-    raw[j][0] = *(const uint2*)(src + (int64_t)head * D + d0);
-    raw[j][1] = *(const uint2*)(src + (int64_t)head * D + d1);
+    raw[j][0] = *(const u32x2*)(src + (int64_t)head * D + d0);
+    raw[j][1] = *(const u32x2*)(src + (int64_t)head * D + d1);
   }
   float cs[8];
   if (a.cos_sin) {
@@ -152,8 +152,8 @@ __device__ inline void rows_body(const QkNormRopeArgs& a, int64_t block) {
   const uint16_t* weight = kTurned ? (const uint16_t*)(kKind == kQuery ? a.q_weight : a.k_weight) : nullptr;
   float w[8];
   if (weight) {
-    widen4<T>(*(const uint2*)(weight + d0), w);
-    widen4<T>(*(const uint2*)(weight + d1), w + 4);
+    widen4<T>(*(const u32x2*)(weight + d0), w);
+    widen4<T>(*(const u32x2*)(weight + d1), w + 4);
   }
   int64_t slot = 0;
   if (kStored) slot = a.slots[token];
@@ -196,13 +196,13 @@ __device__ inline void rows_body(const QkNormRopeArgs& a, int64_t block) {
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = (float)y[i];
-      const uint2 r0 = narrow4<T>(x), r1 = narrow4<T>(x + 4);
+      const u32x2 r0 = narrow4<T>(x), r1 = narrow4<T>(x + 4);
       uint16_t* dst = kKind == kQuery ? (uint16_t*)a.q_out + token * a.q_out_stride
                       : a.k_out       ? (uint16_t*)a.k_out + token * a.k_out_stride
                                       : nullptr;
       if (dst) {
-        *(uint2*)(dst + (int64_t)head * D + d0) = r0;
-        *(uint2*)(dst + (int64_t)head * D + d1) = r1;
+        *(u32x2*)(dst + (int64_t)head * D + d0) = r0;
+        *(u32x2*)(dst + (int64_t)head * D + d1) = r1;
       }
       widen4<T>(r0, x);
       widen4<T>(r1, x + 4);
@@ -286,9 +286,9 @@ __global__ __launch_bounds__(kBlock) void kv4_read_kernel(Kv4ReadArgs a) {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((codes >> (4 * i)) & 15u), s, m);
-    const uint2 r0 = narrow4<T>(x), r1 = narrow4<T>(x + 4);
+    const u32x2 r0 = narrow4<T>(x), r1 = narrow4<T>(x + 4);
     out += row * (which ? a.v_out_stride : a.k_out_stride) + (int64_t)head * D + lane * 8;
-    *(uint4*)out = make_uint4(r0.x, r0.y, r1.x, r1.y);
+    *(u32x4*)out = u32x4{r0.x, r0.y, r1.x, r1.y};
   }
 }
 
@@ -311,19 +311,20 @@ struct PagePairs {
   int32_t src[kPairs], dst[kPairs];
 };
 
-// A workgroup copies kBlock * kCopies * 16 bytes of one page.
-constexpr int kCopies = 4;
+// A workgroup copies kBlock * kCopies * 16 bytes of one page, past the caches: 600 pages of 544 KiB
+// in 125 us (5.3 TB/s), through them 135, with four pieces to a thread 131.
+constexpr int kCopies = 2;
 __global__ __launch_bounds__(kBlock) void copy_pages_kernel(char* pool, int64_t chunks, int64_t stride, PagePairs pairs) {
-  const uint4* src = (const uint4*)(pool + pairs.src[blockIdx.y] * stride);
-  uint4* dst = (uint4*)(pool + pairs.dst[blockIdx.y] * stride);
+  const u32x4* src = (const u32x4*)(pool + pairs.src[blockIdx.y] * stride);
+  u32x4* dst = (u32x4*)(pool + pairs.dst[blockIdx.y] * stride);
   const int64_t at = (int64_t)blockIdx.x * (kBlock * kCopies) + threadIdx.x;
-  uint4 v[kCopies];
+  u32x4 v[kCopies];
 #pragma unroll
   for (int i = 0; i < kCopies; ++i)
-    if (at + i * kBlock < chunks) v[i] = src[at + i * kBlock];
+    if (at + i * kBlock < chunks) v[i] = __builtin_nontemporal_load(src + at + i * kBlock);
 #pragma unroll
   for (int i = 0; i < kCopies; ++i)
-    if (at + i * kBlock < chunks) dst[at + i * kBlock] = v[i];
+    if (at + i * kBlock < chunks) __builtin_nontemporal_store(v[i], dst + at + i * kBlock);
 }
 
 }  // namespace
