@@ -29,25 +29,23 @@ struct Block {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// One row value. (bf16 is handled as bits: widening is a shift, narrowing rounds to the
-// nearest, ties to even, and keeps NaN.)
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+
+// Row values as bits. (A value that comes from 64 bits is rounded from its 32: contracted, the
+// two roundings would become one for f16 and not for bf16.)
 struct F16 {
-  typedef uint16_t bits;
   __device__ static float widen(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (uint16_t)b); }
-  __device__ static uint32_t narrow(float f) {
-    // (a value that comes from 64 bits is rounded here from its 32: contracted, the two
-    // roundings would become one, for this type and not for the other)
+  __device__ static uint32_t narrow2(float a, float b) {
 #pragma clang fp contract(off)
-    return __builtin_bit_cast(uint16_t, (_Float16)f);
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{a, b}), pair));
   }
 };
 struct BF16 {
-  typedef uint16_t bits;
   __device__ static float widen(uint32_t b) { return __builtin_bit_cast(float, b << 16); }
-  __device__ static uint32_t narrow(float f) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, f);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (u >> 16) | 0x40u;
-    return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+  __device__ static uint32_t narrow2(float a, float b) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{a, b}), pair));
   }
 };
 
@@ -60,7 +58,7 @@ __device__ inline void widen4(u32x2 w, float* x) {
 }
 template <typename T>
 __device__ inline u32x2 narrow4(const float* x) {
-  return u32x2{T::narrow(x[0]) | (T::narrow(x[1]) << 16), T::narrow(x[2]) | (T::narrow(x[3]) << 16)};
+  return u32x2{T::narrow2(x[0], x[1]), T::narrow2(x[2], x[3])};
 }
 
 }  // namespace kv4

@@ -49,14 +49,14 @@ __device__ inline V over_row(V v, F f) {
 }
 
 struct Params {
-  uint32_t bits;     // scale and offset, f16 each
-  uint32_t code[8];
+  uint32_t bits;         // scale and offset, f16 each
+  uint32_t low, high;    // codes of a lane's first and last four values
 };
 
-// Codes of a row, 8 values a lane. An estimate in f32 is off by less than 2^-18 of a code; a value
-// that lies within 2^-16 of a border between two codes (one wave in a hundred has one, if values
-// are not on a lattice) is decided by comparing x - offset with (code +- 1/2) scale in 64 bits,
-// which is exact, ties to the even code.
+// Codes of a row, 8 values a lane. An estimate in f32 is off by less than 2^-17 of a code; where a
+// value lies within 2^-15 of a border between two codes (one wave in fifty has one, if values
+// are not on a lattice), all are decided by comparing x - offset with (code +- 1/2) scale in 64
+// bits, which is exact, ties to the even code.
 template <int L>
 __device__ inline Params quantise(const float* x) {
   float lo = x[0], hi = x[0], size = 0.f;
@@ -64,38 +64,44 @@ __device__ inline Params quantise(const float* x) {
   for (int i = 0; i < 8; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
-    size += x[i] * 0.f;            // 0, or NaN where a value is not finite
+    size = fmaf(x[i], 0.f, size);            // 0, or NaN where a value is not finite
   }
   lo = over_row<L>(lo, [](float a, float b) { return fminf(a, b); });
   hi = over_row<L>(hi, [](float a, float b) { return fmaxf(a, b); });
   const float bad = over_row<L>(size == 0.f ? 0.f : 1.f, [](float a, float b) { return fmaxf(a, b); });
   const _Float16 offset = (_Float16)fminf(fmaxf(lo, -65504.f), 65504.f);
-  const double range = (double)hi - (double)lo;
-  const _Float16 step = (_Float16)fminf((float)(range / 15.0), 65504.f);
+  // (the quotient by 15, correctly rounded: a product with the reciprocal and one correction)
+  const double range = (double)hi - (double)lo, q = range * (1.0 / 15.0);
+  const _Float16 step = (_Float16)fminf((float)fma(fma(-15.0, q, range), 1.0 / 15.0, q), 65504.f);
   Params p;
-  const float s = (float)step, m = (float)offset, inv = s > 0.f ? 1.f / s : 0.f;
-  float c[8];
-  bool near = false;
+  const float s = (float)step, m = (float)offset, inv = s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;
+  float c[8], gap = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float t = (x[i] - m) * inv;
     c[i] = rintf(t);
-    near = near || fabsf(fabsf(t - c[i]) - 0.5f) < 0x1p-16f;
-    c[i] = fminf(fmaxf(c[i], 0.f), 15.f);
+    gap = fmaxf(gap, fabsf(t - c[i]));
+    c[i] = __builtin_amdgcn_fmed3f(c[i], 0.f, 15.f);
   }
-  if (near) {
+  if (gap > 0.5f - 0x1p-15f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const double rest = fma(-(double)c[i], (double)s, (double)x[i] - (double)m), half = 0.5 * (double)s;
       const bool odd = ((int)c[i] & 1) != 0;
       const float up = rest > half || (rest == half && odd) ? 1.f : 0.f;
       const float down = rest < -half || (rest == -half && odd) ? 1.f : 0.f;
-      c[i] = fminf(fmaxf(c[i] + up - down, 0.f), 15.f);
+      c[i] = __builtin_amdgcn_fmed3f(c[i] + up - down, 0.f, 15.f);
     }
   }
   const bool stored = s > 0.f && bad == 0.f;
+  p.low = p.high = 0;
+  if (stored) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) p.code[i] = stored ? (uint32_t)c[i] : 0u;
+    for (int i = 0; i < 4; ++i) {
+      p.low |= (uint32_t)c[i] << (4 * i);
+      p.high |= (uint32_t)c[4 + i] << (4 * i);
+    }
+  }
   p.bits = bad == 0.f ? (uint32_t)__builtin_bit_cast(uint16_t, step) |
                             ((uint32_t)__builtin_bit_cast(uint16_t, offset) << 16)
                       : 0x00007E00u;   // scale NaN, offset 0
@@ -211,18 +217,12 @@ __device__ inline void rows_body(const QkNormRopeArgs& a, int64_t block) {
       const Params p = quantise<L>(x);
       if (!exists) continue;
       char* to = a.pool.base + (slot >> a.pool.page_shift) * a.pool.page_stride + head * Block<D>::bytes(page);
-      uint32_t low = 0, high = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        low |= p.code[i] << (4 * i);
-        high |= p.code[4 + i] << (4 * i);
-      }
       if (kKind == kCachedKey) {
-        *(uint16_t*)(to + Block<D>::k_row(at) + d0 / 2) = (uint16_t)low;
-        *(uint16_t*)(to + Block<D>::k_row(at) + d1 / 2) = (uint16_t)high;
+        *(uint16_t*)(to + Block<D>::k_row(at) + d0 / 2) = (uint16_t)p.low;
+        *(uint16_t*)(to + Block<D>::k_row(at) + d1 / 2) = (uint16_t)p.high;
         if (lane == 0) *(uint32_t*)(to + Block<D>::k_params(page, at)) = p.bits;
       } else {
-        *(uint32_t*)(to + Block<D>::v_dword(page, at, lane)) = low | (high << 16);
+        *(uint32_t*)(to + Block<D>::v_dword(page, at, lane)) = p.low | (p.high << 16);
         if (lane == 0) *(uint32_t*)(to + Block<D>::v_params(page, at)) = p.bits;
       }
     }
