@@ -111,6 +111,14 @@ __device__ inline Params quantise(const float* x) {
 __device__ inline float inverse_root(float v) { return rsqrtf(v); }
 __device__ inline double inverse_root(double v) { return 1.0 / sqrt(v); }
 
+// Rows of many tokens leave past the caches, which they would fill (67 MB of queries 26 us,
+// through them 34); those of a few stay for the attention that reads them next.
+template <bool kPast>
+__device__ inline void store(u32x2* to, u32x2 v) {
+  if constexpr (kPast) __builtin_nontemporal_store(v, to);
+  else *to = v;
+}
+
 enum RowKind { kQuery, kKey, kCachedKey, kValue };
 
 // A group of L lanes takes kRows consecutive head rows of one token, so that it reads the token's
@@ -207,8 +215,8 @@ __device__ inline void rows_body(const QkNormRopeArgs& a, int64_t block) {
                       : a.k_out       ? (uint16_t*)a.k_out + token * a.k_out_stride
                                       : nullptr;
       if (dst) {
-        *(u32x2*)(dst + (int64_t)head * D + d0) = r0;
-        *(u32x2*)(dst + (int64_t)head * D + d1) = r1;
+        store<(kRows > 1)>((u32x2*)(dst + (int64_t)head * D + d0), r0);
+        store<(kRows > 1)>((u32x2*)(dst + (int64_t)head * D + d1), r1);
       }
       widen4<T>(r0, x);
       widen4<T>(r1, x + 4);
