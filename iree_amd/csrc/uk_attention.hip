@@ -179,13 +179,15 @@ __device__ inline void request_half(char* lds, const char* block, int page, int 
                                                v_codes + 256 * i, 0, 0);
   }
   if (lane < 8)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + 2 * TileLds<D>::kCodes), 16, p_at, page * D + row * 4, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + 2 * TileLds<D>::kCodes), 16, p_at, row * 4, 0, 0);
 }
 
 template <int N>
 __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+
+__device__ inline void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 union Frag {
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
     k_at[0] = n * (D / 2) + g * (D / 8);
     k_at[1] = g * (D / 8) * 16 + n * 16;
   }
-  p_at = (lane & 3) * 16 + (lane >> 2) * page_size * 4;      // lanes 0..3 the K parameters, 4..7 those of V
+  p_at = page_size * D + (lane & 3) * 16 + (lane >> 2) * page_size * 4;      // lanes 0..3 the K parameters, 4..7 those of V
   // What has been requested: its first key, and whether the pages of its halves exist.
   struct Tile {
     int key, exist;
@@ -379,6 +381,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
     const int ahead = tile + kWaves;
     if (ahead < end) {
       if (ahead >= pages_from + 32 * kWaves) fetch_pages(ahead);
+      wait_reads();                     // (its place was read from a tile ago)
       next = request(slot ^ 1, ahead);
       wait_loads<TileLds<D>::kLoads>();
     } else {
@@ -621,12 +624,6 @@ __global__ __launch_bounds__(kJoinThreads) void attention_kv4_join_kernel(SplitA
 
 // ---------------------------------------------------------------------------
 // Many rows: prompts
-#ifndef PRI
-#define PRI 0
-#endif
-#ifndef OCC
-#define OCC 2
-#endif
 // ---------------------------------------------------------------------------
 
 constexpr int kPromptRows = 128;      // of a workgroup, 32 of each of its four waves
@@ -653,7 +650,7 @@ constexpr int prompt_lds_bytes() { return 2 * PromptLds<D>::kBytes + 64; }
 // score (three for scale and offset, one each for the largest, the sum, the offsets of V and
 // the operand, an exponential at a quarter of the rate).
 template <int D, typename T>
-__global__ __launch_bounds__(256, D == 256 ? 1 : OCC) void attention_kv4_prompt_kernel(SplitArgs args) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
   constexpr int N = prompt_keys<D>(), KB = N / 32, KK = N / 16;     // keys; blocks of 32; steps of 16
   constexpr int S = D / 16, DB = D / 32;                            // steps of a score; blocks of d
@@ -866,73 +863,80 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : OCC) void attention_kv4_prompt_
 #pragma unroll
       for (int i = 0; i < KK; ++i) stop = fmaxf(stop, scales[4 * buffer + i]);
       const int stop_e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(stop));
+      // Scores minus the row's reference. Element j of a lane: key 32 kb + 8 (j / 4) + 4 h + j % 4.
+      floatx16 x[KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        // Scores minus the row's reference. Element j of a lane: key 32 kb + 8 (j / 4) + 4 h + j % 4.
-        floatx16 x = {};
-        if (PRI) __builtin_amdgcn_s_setprio(1);
+      for (int kb = 0; kb < KB; ++kb) x[kb] = floatx16{};
 #pragma unroll
-        for (int i = 0; i < S; ++i)
-          x = F16Cfg::mfma(*(const half8*)(from + ((kb * S + i) * 64 + lane) * 16), qf[i].f, x);
-        if (PRI) __builtin_amdgcn_s_setprio(0);
+      for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+          x[kb] = F16Cfg::mfma(*(const half8*)(from + ((kb * S + i) * 64 + lane) * 16), qf[i].f, x[kb]);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
           const u32x4 kp = *(const u32x4*)(from + PromptLds<D>::kParams + (32 * kb + 2 * j + 4 * h) * 4);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const half2v sm = as_half2(kp[i]);
-            x[j + i] = fmaf((float)sm[0], x[j + i] * f, fmaf((float)sm[1], qsum, -ref));
+            x[kb][j + i] = fmaf((float)sm[0], x[kb][j + i] * f, fmaf((float)sm[1], qsum, -ref));
           }
         }
-        if (!whole) {
+      if (!whole) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
           const int from_lane = key + 32 * kb + 4 * h;
           const int up_to = pos - from_lane, past = below - from_lane, sink = sinks - from_lane;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const int k = 8 * (j >> 2) + (j & 3);
             const bool yes = (k <= up_to) & ((k > past) | (k < sink)) & ((exist >> (2 * kb + j / 8) & 1) != 0);
-            x[j] = yes ? x[j] : -INFINITY;
+            x[kb][j] = yes ? x[kb][j] : -INFINITY;
           }
         }
-        float top = x[0];
+      }
+      float top = -INFINITY;
 #pragma unroll
-        for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
-        if (__ballot(top > limit - (float)stop_e)) {
-          const float most = fmaxf(top, __shfl_xor(top, 32));
-          const float over = most + (float)(stop_e - 1 - kTarget);
-          // (a row's first scores set its reference, wherever they lie; later ones only raise it)
-          const float by = fresh ? (over > -INFINITY ? over : 0.f) : fmaxf(over, 0.f);
-          const float factor = fresh ? 1.f : __builtin_amdgcn_exp2f(-by);
-          if (over > -INFINITY) fresh = false, limit = (float)(kMost + 1);
-          l *= factor;
-          bias *= factor;
-          ref += by;
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) x[j] -= by;
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, x[kb][j]);
+      if (__ballot(top > limit - (float)stop_e)) {
+        const float most = fmaxf(top, __shfl_xor(top, 32));
+        const float over = most + (float)(stop_e - 1 - kTarget);
+        // (a row's first scores set its reference, wherever they lie; later ones only raise it)
+        const float by = fresh ? (over > -INFINITY ? over : 0.f) : fmaxf(over, 0.f);
+        const float factor = fresh ? 1.f : __builtin_amdgcn_exp2f(-by);
+        if (over > -INFINITY) fresh = false, limit = (float)(kMost + 1);
+        l *= factor;
+        bias *= factor;
+        ref += by;
 #pragma unroll
-          for (int i = 0; i < DB; ++i) o[i] *= factor;
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[kb][j] -= by;
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[i] *= factor;
+      }
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        Frag p;
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          const u32x4 vp = *(const u32x4*)(from + PromptLds<D>::kParams + (N + 16 * kk + 2 * j + 4 * h) * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const half2v sm = as_half2(vp[i]);
+            const float w = __builtin_amdgcn_exp2f(x[kk / 2][kk % 2 * 8 + j + i]);
+            l += w;
+            bias = fmaf(w, (float)sm[1], bias);
+            p.f[j + i] = (_Float16)fmaf(w, (float)sm[0], 0.f);
+          }
         }
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int kk = 2 * kb + half;
-          Frag p;
-#pragma unroll
-          for (int j = 0; j < 8; j += 4) {
-            const u32x4 vp = *(const u32x4*)(from + PromptLds<D>::kParams + (N + 16 * kk + 2 * j + 4 * h) * 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const half2v sm = as_half2(vp[i]);
-              const float w = __builtin_amdgcn_exp2f(x[8 * half + j + i]);
-              l += w;
-              bias = fmaf(w, (float)sm[1], bias);
-              p.f[j + i] = (_Float16)fmaf(w, (float)sm[0], 0.f);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < DB; ++i) {
-            const int at = (kk * DB + i) * 64 + h * 32 + (n & 24) + ((n & 7) ^ ((n >> 3) + 4 * h));
-            o[i] = F16Cfg::mfma(*(const half8*)(from + PromptLds<D>::kV + at * 16), p.f, o[i]);
-          }
+        for (int i = 0; i < DB; ++i) {
+          const int at = (kk * DB + i) * 64 + h * 32 + (n & 24) + ((n & 7) ^ ((n >> 3) + 4 * h));
+          o[i] = F16Cfg::mfma(*(const half8*)(from + PromptLds<D>::kV + at * 16), p.f, o[i]);
         }
       }
     }
