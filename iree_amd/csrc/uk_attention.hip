@@ -129,9 +129,14 @@ constexpr int kMaxSplits = 1024;
 
 // A row's weights p = 2^(score - ref) are carried against a reference that is only moved
 // when p s leaves the range of f16: it is set so that the largest score and the largest scale
-// of V together give 2^kTarget, and moved when they would give 2^kMost. What is dropped at the
-// other end lies 2^-31 below the largest p s. A scale counts as at least 2^-24 (it may be 0).
+// of V together give 2^kTarget, and moved when a p s comes to 2^kMost (few rows), or when they
+// would together (prompts). What is dropped at the other end lies 2^-31 below the largest p s. A
+// scale counts as at least 2^-24; where it is 0, the sum of the p shows that they grow.
+// p s is rounded to f16, 2^-12 of each weight, as the result is to its own type: 2.9e-4 of
+// the result of f16 rows in all, 2.1e-4 with a second f16 for the rest, which costs 4 us of 60 at
+// two caches of 131072 keys. The sums of p and of p (m + 8 s) stay in f32.
 constexpr int kTarget = 7, kMost = 13;
+constexpr float kMostWeight = 1 << kMost, kMostSum = 0x1p60f;
 
 // Partial results of a split: per (tile, kv head, split) O [R][D], reference [R], sum [R].
 template <int D, int R>
@@ -159,27 +164,29 @@ struct TileLds {
   static constexpr int kLoads = 2 * (D == 64 ? 2 : 2 * (D / 128) + 1);
 };
 
-// One half straight into LDS: per instruction 64 (params: 8) lanes of 16 bytes.
-template <int D>
+// One half straight into LDS: per instruction 64 (params: 8) lanes of 16 bytes, past the
+// caches (kPast) where nobody else will ask for them.
+template <int D, bool kPast>
 __device__ inline void request_half(char* lds, const char* block, int page, int row, const uint32_t (&k_at)[2],
                                     uint32_t p_at, int lane) {
   typedef __attribute__((address_space(3))) void lds_t;
+  constexpr int kPolicy = kPast ? 2 : 0;            // bit 1: not kept
   const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)block, 0, 0x7FFFFFFF, 0x00020000);
   const int codes = row * (D / 2), v_codes = codes + page * (D / 2);
   if constexpr (D == 64) {
     // (a wave's worth holds K in its first half, V in the second)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)lds, 16, k_at[0], codes, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)lds, 16, k_at[0], codes, 0, kPolicy);
   } else {
 #pragma unroll
     for (int i = 0; i < D / 128; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + 1024 * i), 16, k_at[0], codes + 16 * i, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + 1024 * i), 16, k_at[0], codes + 16 * i, 0, kPolicy);
 #pragma unroll
     for (int i = 0; i < D / 128; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + TileLds<D>::kCodes + 1024 * i), 16, k_at[1],
-                                               v_codes + 256 * i, 0, 0);
+                                               v_codes + 256 * i, 0, kPolicy);
   }
   if (lane < 8)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + 2 * TileLds<D>::kCodes), 16, p_at, row * 4, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t*)(lds + 2 * TileLds<D>::kCodes), 16, p_at, row * 4, 0, kPolicy);
 }
 
 template <int N>
@@ -216,8 +223,8 @@ __device__ inline uint32_t pair_bytes(uint32_t first, uint32_t second) {
   return __builtin_amdgcn_perm(second, first, 0x0C040C00u | b | (b << 16));
 }
 // Tiles of a wave in LDS: the one in use and the one on its way. (Three, which leave room for
-// three workgroups on a compute unit instead of four: two caches of 131072 keys 58.6 us, with
-// two 56.0.)
+// three workgroups on a compute unit instead of four: two caches of 131072 keys 51.2 us, with
+// two 50.4.)
 constexpr int kRing = 2;
 
 // LDS of a workgroup: the waves' rings, later their results; behind them the waves'
@@ -245,13 +252,12 @@ __device__ inline half2v high_codes(uint32_t x, uint32_t bias) {
 // result) is one value of the lane. The waves of a workgroup take key tiles in turn, each
 // with a running softmax of its own; they join through LDS at the end. The next tile is
 // requested before the current one is used.
-template <int D, typename T>
+template <int D, typename T, bool kPast>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
   constexpr int S = D / 32;                        // matrix-core steps of a score
   constexpr int C = D >= 128 ? D / 128 : 1;        // dwords of a V row in a lane
   constexpr int NI = D / 16;                       // accumulators of O
-  constexpr bool kExact = __is_same(T, F16);
   extern __shared__ __attribute__((aligned(1024))) char memory[];
   float (*ref_s)[kRows] = (float (*)[kRows])(memory + split_lds_bytes<D>()) - 2 * kWaves;
   float (*sum_s)[kRows] = ref_s + kWaves;
@@ -359,7 +365,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
       const int p = page_at(t, half);
       const bool ok = (unsigned)p < (unsigned)pages;
       w.exist |= ok ? 1 << half : 0;
-      request_half<D>(to + half * TileLds<D>::kHalf, base + (ok ? p : 0) * a.pool.page_stride, page_size,
+      request_half<D, kPast>(to + half * TileLds<D>::kHalf, base + (ok ? p : 0) * a.pool.page_stride, page_size,
                       (w.key + 16 * half) & (page_size - 1), k_at, p_at, lane);
     }
     return w;
@@ -439,21 +445,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
         vp[j] = yes ? vp[j] : 0u;
       }
     }
-    const float top = fmaxf(max4(x[0], x[1], x[2], x[3]), max4(x[4], x[5], x[6], x[7]));
-    half2v smost = as_half2(vp[0]);                 // (scales are not negative, and the low halves)
+    // The weights, and in the rare tile in which one is too large for f16 all again, against a
+    // reference that holds for its largest score and scale.
+    Frag w;
+    float l_next, bias_next;
+    auto weigh = [&]() {
+      l_next = l, bias_next = bias;
 #pragma unroll
-    for (int j = 1; j < 8; ++j) smost = __builtin_elementwise_max(smost, as_half2(vp[j]));
-    const float stop = fmaxf((float)smost[0], 0x1p-24f);
-    if (__ballot(top > (float)(kMost + 1 - __builtin_amdgcn_frexp_expf(stop)))) {
+      for (int j = 0; j < 8; ++j) {
+        const half2v sm = as_half2(vp[j]);
+        const float p = __builtin_amdgcn_exp2f(x[j]);
+        l_next += p;
+        bias_next = fmaf(p, fmaf((float)sm[0], 8.f, (float)sm[1]), bias_next);
+        w.f[j] = (_Float16)fmaf(p, (float)sm[0], 0.f);
+      }
+    };
+    weigh();
+    half2v most_w = __builtin_elementwise_max(__builtin_elementwise_max(w.h[0], w.h[1]),
+                                              __builtin_elementwise_max(w.h[2], w.h[3]));
+    most_w = __builtin_elementwise_max(most_w, __builtin_shufflevector(most_w, most_w, 1, 0));
+    if (__ballot(most_w[0] > (_Float16)kMostWeight || l_next > kMostSum)) {
       float most = -INFINITY;
+      half2v smost = as_half2(vp[0]);                 // (scales are not negative, and the low halves)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const half2v sm = as_half2(kp[j]);
         x[j] = fmaf((float)sm[0], (j < 4 ? s0 : s1)[j & 3], (float)sm[1] * qsum);
         x[j] = seen >> j & 1 ? x[j] : -INFINITY;
         most = fmaxf(most, x[j]);
+        smost = __builtin_elementwise_max(smost, as_half2(vp[j]));
       }
-      const float raised = fmaxf(ref, across_max(most) + (float)(__builtin_amdgcn_frexp_expf(across_max(stop)) - 1 - kTarget));
+      const float stop = fmaxf(across_max((float)smost[0]), 0x1p-24f);
+      const float raised = fmaxf(ref, across_max(most) + (float)(__builtin_amdgcn_frexp_expf(stop) - 1 - kTarget));
       const float factor = __builtin_amdgcn_exp2f(ref - raised);
       l *= factor;
       bias *= factor;
@@ -462,17 +485,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
       for (int j = 0; j < 8; ++j) x[j] -= ref;
 #pragma unroll
       for (int i = 0; i < NI; ++i) o[i] *= factor;
+      weigh();
     }
-    Frag hi, lo;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const half2v sm = as_half2(vp[j]);
-      const float p = __builtin_amdgcn_exp2f(x[j]);
-      l += p;
-      bias = fmaf(p, fmaf((float)sm[0], 8.f, (float)sm[1]), bias);
-      hi.f[j] = (_Float16)(p * (float)sm[0]);
-      if constexpr (kExact) lo.f[j] = (_Float16)fmaf(p, (float)sm[0], -(float)hi.f[j]);
-    }
+    l = l_next, bias = bias_next;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -485,8 +500,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
         for (int j = 0; j < 4; ++j) d[4 * half + j] = v[j];
       }
       auto add = [&](int i, const Frag& v) {
-        o[i] = F16Cfg16::mfma(v.f, hi.f, o[i]);
-        if constexpr (kExact) o[i] = F16Cfg16::mfma(v.f, lo.f, o[i]);
+        o[i] = F16Cfg16::mfma(v.f, w.f, o[i]);
       };
       auto byte = [&](auto which) {
         constexpr int b = decltype(which)::value;
@@ -982,6 +996,7 @@ struct Split {
   bool prompt;
   int64_t tiles;       // of rows, with the gaps of their numbering
   int splits, chunk;
+  bool past;           // few rows: keys past the caches
 };
 
 Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int64_t window, int64_t sinks,
@@ -997,6 +1012,10 @@ Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int6
   const int64_t key_tiles = keys < 1 ? 1 : ceil_div(keys, tile);
   const int64_t units = (rows / R < batch ? batch : rows / R) * kv_heads;
   const int64_t cus = device_cu_count();
+  // Keys that one tile of rows reads once, and that are too many for the caches to hold until the
+  // next step, go past them: two sequences of 131072 keys 54.8 us through them, 50.4 past them; 72 MB
+  // of windows that a repeated call still finds there 20.8 and 21.4.
+  p.past = !p.prompt && tokens <= batch && G <= kRows && (double)batch * keys * kv_heads * (dim + 8) > 128e6;
   int64_t splits;
   if (p.prompt) {
     // Two workgroups to a compute unit; the tiles of a prompt see half of its keys on average.
@@ -1005,9 +1024,10 @@ Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int6
     splits = units >= cus ? 1 : splits < most ? splits : most;
   } else {
     // Six workgroups to a compute unit, so that lengths that differ even out (32 sequences of
-    // 1000 to 8192 keys: 49 us, two to a unit 59), but no more than 32 splits where fewer fill the
-    // device: the join reads them all (two of 131072 keys: 59 us, with 96 splits 65). A split has
-    // enough tiles to be worth its start and the join, fewer where most of the device is idle.
+    // 1000 to 8192 keys: 40.9 us, with four 44.5, with eight 42.6), but no more than 32 splits where
+    // fewer fill the device: the join reads them all (two of 131072 keys: 49.4 us, with 48 splits
+    // 53.0, with 64 52.0). A split has enough tiles to be worth its start and the join, fewer where
+    // most of the device is idle.
     splits = ceil_div(6 * cus, units);
     if (splits > 32) splits = ceil_div(2 * cus, units) > 32 ? ceil_div(2 * cus, units) : 32;
     const int64_t most = 2 * units <= cus ? ceil_div(key_tiles, 16) : key_tiles / 32;
@@ -1041,14 +1061,15 @@ int launch_split(const AttentionKv4Args& a, hipStream_t s) {
   const uint64_t one = (uint64_t)blocks * (p.prompt ? part_floats<D, kPromptRows>() : part_floats<D, kRows>()) * 4;
   if (p.splits > 1 && a.workspace_bytes < one * p.splits) p.splits = 1;
   SplitArgs args{a, a.heads / a.kv_heads, p.splits, p.chunk};
-  static PerDeviceOnce once[2];
+  static PerDeviceOnce once[3];
   const dim3 grid((unsigned)blocks, (unsigned)p.splits);
   if (p.prompt) {
     UK_RETURN_IF_ERROR(allow_lds(attention_kv4_prompt_kernel<D, T>, prompt_lds_bytes<D>(), once[0]));
     hipLaunchKernelGGL((attention_kv4_prompt_kernel<D, T>), grid, dim3(256), prompt_lds_bytes<D>(), s, args);
   } else {
-    UK_RETURN_IF_ERROR(allow_lds(attention_kv4_split_kernel<D, T>, split_lds_bytes<D>(), once[1]));
-    hipLaunchKernelGGL((attention_kv4_split_kernel<D, T>), grid, dim3(64 * kWaves), split_lds_bytes<D>(), s, args);
+    const auto kernel = p.past ? attention_kv4_split_kernel<D, T, true> : attention_kv4_split_kernel<D, T, false>;
+    UK_RETURN_IF_ERROR(allow_lds(kernel, split_lds_bytes<D>(), once[p.past ? 1 : 2]));
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), split_lds_bytes<D>(), s, args);
   }
   UK_RETURN_IF_HIP(hipGetLastError());
   if (p.splits == 1) return 0;
