@@ -13,7 +13,7 @@ import torch
 
 from . import flags as F
 from ._lib import load_library
-from .ukernel import _check, _stream
+from .ukernel import _check, _raw_stream, _stream
 
 _ROW_TYPES = {F.ATTENTION_TYPE_F16: torch.float16, F.ATTENTION_TYPE_BF16: torch.bfloat16}
 
@@ -39,6 +39,12 @@ def _tensor(t, dtype, name, device):
     if dtype is not None and t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
     return t.data_ptr()
+
+
+def _stream_on(stream, device):
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(device)
+    return _stream(stream)
 
 
 def _row_type(flags):
@@ -73,7 +79,7 @@ def qk_norm_rope(q, k, q_out, k_out, tokens, heads, kv_heads, head_dim, flags, *
         _tensor(cos_sin, torch.float32, "cos_sin", device), table_rows, rotary_dim,
         _tensor(positions, torch.int32, "positions", device), _tensor(cache, None, "cache", device), pages,
         page_stride, page_size, _tensor(slots, torch.int64, "slots", device), tokens, heads, kv_heads, head_dim, flags,
-        _stream(stream)))
+        _stream_on(stream, device)))
 
 
 def kv4_read(cache, pages, page_size, slots, k_out, v_out, rows, kv_heads, head_dim, flags, *, page_stride=None,
@@ -87,7 +93,7 @@ def kv4_read(cache, pages, page_size, slots, k_out, v_out, rows, kv_heads, head_
         _tensor(slots, torch.int64, "slots", device),
         _tensor(k_out, kind, "k_out", device), row if k_out_stride0 is None else k_out_stride0,
         _tensor(v_out, kind, "v_out", device), row if v_out_stride0 is None else v_out_stride0, rows, kv_heads, head_dim,
-        flags, _stream(stream)))
+        flags, _stream_on(stream, device)))
 
 
 def attention_kv4_workspace(tokens, batch, heads, kv_heads, head_dim, *, max_kv_len, window=0, sinks=0):
@@ -131,7 +137,7 @@ def attention_kv4(q, out, cache, pages, page_size, page_table, q_starts, kv_lens
         _tensor(q_starts, torch.int32, "q_starts", device), _tensor(kv_lens, torch.int32, "kv_lens", device), tokens,
         batch, heads, kv_heads, head_dim, scale, window, sinks, max_kv_len,
         _tensor(workspace, None, "workspace", device), 0 if workspace is None else workspace.nbytes, flags,
-        _stream(stream)))
+        _stream_on(stream, device)))
 
 
 def _workspace(nbytes, stream):
@@ -152,7 +158,7 @@ def copy_pages(pool, pages, page_bytes, src, dst, *, page_stride=None, stream=No
         raise ValueError("src and dst must have as many pages")
     _check(load_library().iree_amd_uk_copy_pages(
         _tensor(pool, None, "pool", device), pages, page_bytes, page_bytes if page_stride is None else page_stride,
-        src.data_ptr(), dst.data_ptr(), src.numel(), _stream(stream)))
+        src.data_ptr(), dst.data_ptr(), src.numel(), _stream_on(stream, device)))
 
 
 def _host_pages(v):
