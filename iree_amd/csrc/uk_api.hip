@@ -1037,6 +1037,9 @@ extern "C" int iree_amd_uk_attention_kv4(
   UK_RETURN_IF_ERROR(make_pool(what, cache, pages, page_stride, page_size, kv_heads, head_dim, &a.pool));
   if (max_pages < 0 || max_pages > 0x7FFFFFFF || page_table_stride < 0 || (batch > 1 && page_table_stride < max_pages))
     return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: page table stride below max_pages, or a negative one", what);
+  // (positions and what is added to them stay within 31 bits)
+  if (max_pages << a.pool.page_shift > 0x7FFFF000)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: max_pages of that size hold 2^31 - 4096 tokens or more", what);
   if ((!page_table && max_pages) || !q_starts || !kv_lens)
     return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null page_table, q_starts or kv_lens", what);
   if (!(scale - scale == 0.f)) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: scale is not finite", what);

@@ -132,7 +132,7 @@ constexpr int kMaxSplits = 1024;
 // of V together give 2^kTarget, and moved when a p s comes to 2^kMost (few rows), or when they
 // would together (prompts). What is dropped at the other end lies 2^-31 below the largest p s. A
 // scale counts as at least 2^-24; where it is 0, the sum of the p shows that they grow.
-// p s is rounded to f16, 2^-12 of each weight, as the result is to its own type: 2.9e-4 of
+// p s is rounded to f16, at most 2^-11 of each weight, as the result is to its own type: 2.9e-4 of
 // the result of f16 rows in all, 2.1e-4 with a second f16 for the rest, which costs 4 us of 60 at
 // two caches of 131072 keys. The sums of p and of p (m + 8 s) stay in f32.
 constexpr int kTarget = 7, kMost = 13;
@@ -1057,7 +1057,8 @@ template <int D, typename T>
 int launch_split(const AttentionKv4Args& a, hipStream_t s) {
   Split p = plan(a.tokens, a.batch, a.heads, a.kv_heads, D, a.window, a.sinks, a.max_kv_len);
   const int64_t blocks = p.tiles * a.kv_heads;
-  if (blocks > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "attention_kv4: too many rows for one call");
+  // (a grid's threads are counted in 32 bits)
+  if (blocks > 0xFFFFFFFFll / 256) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "attention_kv4: too many rows for one call");
   const uint64_t one = (uint64_t)blocks * (p.prompt ? part_floats<D, kPromptRows>() : part_floats<D, kRows>()) * 4;
   if (p.splits > 1 && a.workspace_bytes < one * p.splits) p.splits = 1;
   SplitArgs args{a, a.heads / a.kv_heads, p.splits, p.chunk};

@@ -12,6 +12,7 @@ namespace {
 using namespace kv4;
 
 constexpr int kBlock = 256;
+constexpr int64_t kMostBlocks = 0xFFFFFFFFll / kBlock;      // a grid's threads are counted in 32 bits
 
 // ---------------------------------------------------------------------------
 // qk_norm_rope
@@ -253,7 +254,7 @@ int launch_rows(const QkNormRopeArgs& a, hipStream_t s) {
   const int64_t q_blocks = a.q ? ceil_div(a.tokens * ceil_div(a.heads, kRows), kGroups) : 0;
   const int64_t kv_blocks = ceil_div(a.tokens * ceil_div(a.kv_heads, kRows), kGroups);
   const int64_t blocks = q_blocks + (a.k ? kv_blocks : 0) + (a.pool.base ? kv_blocks : 0);
-  if (blocks > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "qk_norm_rope: too many rows for one call");
+  if (blocks > kMostBlocks) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "qk_norm_rope: too many rows for one call");
   hipLaunchKernelGGL((qk_norm_rope_kernel<D, T, kRows>), dim3((unsigned)blocks), dim3(kBlock), 0, s, a, q_blocks,
                      a.k ? kv_blocks : 0);
   return check_hip(hipGetLastError(), "qk_norm_rope");
@@ -303,7 +304,7 @@ __global__ __launch_bounds__(kBlock) void kv4_read_kernel(Kv4ReadArgs a) {
 template <int D, typename T>
 int launch_read(const Kv4ReadArgs& a, hipStream_t s) {
   const int64_t blocks = ceil_div(a.rows * a.kv_heads, kBlock / (D / 8));
-  if (blocks > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "kv4_read: too many rows for one call");
+  if (blocks > kMostBlocks) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "kv4_read: too many rows for one call");
   hipLaunchKernelGGL((kv4_read_kernel<D, T>), dim3((unsigned)blocks), dim3(kBlock), 0, s, a);
   return check_hip(hipGetLastError(), "kv4_read");
 }
@@ -357,7 +358,7 @@ int launch_copy_pages(void* pool, int64_t page_bytes, int64_t page_stride, const
                       int64_t count, hipStream_t s) {
   const int64_t chunks = page_bytes / 16;
   const int64_t blocks = ceil_div(chunks, kBlock * kCopies);
-  if (blocks > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "copy_pages: a page too large for one launch");
+  if (blocks > kMostBlocks) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "copy_pages: a page too large for one launch");
   for (int64_t at = 0; at < count; at += kPairs) {
     PagePairs pairs;
     const int n = (int)(count - at < kPairs ? count - at : kPairs);

@@ -88,6 +88,14 @@ def test_attention_refuses(status, changes):
     assert _call("attention_kv4", ATTENTION, **changes) == status
 
 
+def test_attention_refuses_positions_past_31_bits():
+    most = (2**31 - 4096) // 256
+    at = dict(page_size=256, page_stride=2 * 256 * 136)
+    assert _call("attention_kv4", ATTENTION, max_pages=most + 1, table_stride=most + 1, **at) == 3
+    assert _call("attention_kv4", ATTENTION, max_pages=most, table_stride=most, q=None, **at) == 3      # (that q is null)
+    assert b"null q" in iree_amd.load_library().iree_amd_uk_last_error()
+
+
 def test_attention_of_nothing():
     for empty in (dict(tokens=0), dict(batch=0), dict(heads=0)):
         assert _call("attention_kv4", ATTENTION, **empty) == 0

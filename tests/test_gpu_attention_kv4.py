@@ -333,6 +333,7 @@ def test_long_caches_are_split(uk, cuda, heads, kv_heads, dim, kv_lens):
     the first the same bits twice; what max_kv_len says changes no result beyond its rounding."""
     case = Case(7, F16, heads, kv_heads, dim, 64, [1] * len(kv_lens), kv_lens)
     nbytes = uk.attention_kv4_workspace(case.tokens, len(kv_lens), heads, kv_heads, dim, max_kv_len=max(kv_lens))
+    assert nbytes > 0
     workspace = torch.full((nbytes,), 0xFF, dtype=torch.uint8, device="cuda")
     first = case.run(uk, max_kv_len=max(kv_lens), workspace=workspace)
     case.check(first)
@@ -343,6 +344,56 @@ def test_long_caches_are_split(uk, cuda, heads, kv_heads, dim, kv_lens):
     case.check(case.run(uk, max_kv_len=1))
     case.check(case.run(uk, max_kv_len=1 << 40))
     case.check(case.run(uk, max_kv_len=max(kv_lens), window=3000, sinks=17), window=3000, sinks=17)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,q_lens,kv_lens", [
+    (4, 1, 128, [130, 40], [20000, 333]), (8, 2, 64, [33, 0, 300], [9000, 5000, 30011]), (2, 1, 256, [90], [7001])])
+def test_prompts_over_long_caches_are_split(uk, cuda, heads, kv_heads, dim, q_lens, kv_lens):
+    """The next part of a prompt whose first parts are cached, as above."""
+    case = Case(12, BF16, heads, kv_heads, dim, 32, q_lens, kv_lens)
+    nbytes = uk.attention_kv4_workspace(case.tokens, len(kv_lens), heads, kv_heads, dim, max_kv_len=max(kv_lens))
+    assert nbytes > 0
+    workspace = torch.full((nbytes,), 0xFF, dtype=torch.uint8, device="cuda")
+    first = case.run(uk, max_kv_len=max(kv_lens), workspace=workspace)
+    case.check(first)
+    workspace.fill_(0x7F)
+    assert torch.equal(first, case.run(uk, max_kv_len=max(kv_lens), workspace=workspace))
+    case.check(case.run(uk, max_kv_len=max(kv_lens), workspace=workspace[:64]))
+    case.check(case.run(uk, max_kv_len=1))
+    case.check(case.run(uk, max_kv_len=max(kv_lens), window=2500, sinks=40), window=2500, sinks=40)
+
+
+@pytest.mark.parametrize("q_len,every,batch,heads", [(1, 1, 65, 2), (1, 41, 4200, 3), (120, 9, 130, 16)])
+def test_many_sequences(uk, cuda, q_len, every, batch, heads):
+    """More sequences than a wave looks at in one step, most without queries between those with."""
+    q_lens = [q_len if b % every == every // 2 else 0 for b in range(batch)]
+    case = Case(batch, F16, heads, 1, 64, 16, q_lens, [b % 50 + q_len for b in range(batch)])
+    case.check(case.run(uk))
+
+
+def test_no_pages(uk, cuda):
+    """A page table without columns, or a pool without pages: nothing is visible."""
+    case = Case(4, F16, 4, 2, 64, 16, [1, 100], [5, 100])
+    case.wide = 0
+    out = case.run(uk)
+    case.wide, case.pages = case.table.shape[1] - 2, 0
+    for out in (out, case.run(uk)):
+        assert bool((out[case.rows][:, :4 * 64] == 0).all()) and bool((out[~case.rows] == 3).all())
+
+
+def test_two_calls_at_once(uk, cuda):
+    """Calls on two streams, each with the workspace that it takes for itself, do not disturb each other."""
+    cases = [Case(50 + i, F16, 8, 2, 128, 64, [1, 1], [20000 - 999 * i, 7000]) for i in range(2)]
+    want = [case.run(uk) for case in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = [[torch.full_like(w, 3.0) for _ in range(10)] for w in want]
+    torch.cuda.synchronize()
+    for turn in range(10):
+        for case, stream, mine in zip(cases, streams, outs):
+            case.run(uk, out=mine[turn], stream=stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, w) for w, mine in zip(want, outs) for out in mine)
 
 
 def test_a_pool_past_32_bits(uk, cuda):
@@ -474,6 +525,117 @@ def test_block_of_a_decode_step_captured(uk, cuda):
         assert torch.equal(out, eager) and torch.equal(after, pool.buffer)
 
 
+def test_layer_of_a_decode_step(uk, cuda):
+    """One layer of 32 sequences, as a program runs it: int4 projections of q, k and v, norms, rotation
+    and append, attention, the int4 output projection, the fp8 gate/up/down block. Each stage of
+    the block against 64 bits on the inputs that it got, and all of it in one graph, replayed over
+    steps, against the eager bits; a sequence that has ended is padding (position and slot -1)."""
+    gen = _gen(123)
+    batch, heads, kv_heads, dim, page, ffn, gs = 32, 4, 2, 64, 16, 512, 128
+    hidden, row = heads * dim, (heads + 2 * kv_heads) * dim
+    pool = uk.Kv4Cache(200, page, 1, kv_heads, dim)
+    seqs = [pool.new() for _ in range(batch)]
+    table = kv4ref.angles(256, dim, "cuda")
+    weights = [(1 + 0.1 * _normal(gen, dim)).half() for _ in range(2)]
+
+    def int4(n, k):
+        w = torch.randint(0, 256, (n, k // 2), generator=gen, device="cuda", dtype=torch.uint8)
+        tiled = torch.empty_like(w)
+        uk.pack_i4_weights(w, tiled, n, k)
+        scale = (torch.rand(n, k // gs, generator=gen, device="cuda") * 0.01 + 0.005).half()
+        zp = torch.full((n, k // gs), 7.5, dtype=F16, device="cuda")
+        return w, tiled, scale, zp
+
+    def project(x, weight, out, n, k):
+        uk.dequant_matmul_i4(x, weight[1], weight[2], weight[3], out, batch, n, k, gs, F.DEQUANT_MATMUL_W_TILED)
+
+    def dense(weight, n, k):
+        codes = torch.stack((weight[0] & 15, weight[0] >> 4), -1).view(n, k // gs, gs).double()
+        return ((codes - 7.5) * weight[2].double()[..., None]).view(n, k)
+
+    w_qkv, w_o = int4(row, hidden), int4(hidden, hidden)
+    codes = [torch.randint(0, 120, (n,), generator=gen, device="cuda", dtype=torch.uint8)
+             for n in (ffn * hidden, ffn * hidden, hidden * ffn)]
+    mlp = uk.Fp8Mlp(hidden, ffn, *codes, 2e-3, 2e-3, 2e-3, 0.05, 0.05, max_tokens=batch)
+    ones = torch.arange(batch + 1, dtype=torch.int32, device="cuda")
+
+    class Step:
+        def __init__(self):
+            self.qkv = torch.empty(batch, row, dtype=F16, device="cuda")
+            self.turned, self.seen, self.added = (torch.empty(batch, hidden, dtype=F16, device="cuda") for _ in range(3))
+            self.y = torch.empty(batch, hidden, dtype=torch.float32, device="cuda")
+
+        def run(self, x, positions, slots, tables):
+            project(x, w_qkv, self.qkv, row, hidden)
+            q, k, v = self.qkv[:, :hidden], self.qkv[:, hidden:-kv_heads * dim], self.qkv[:, -kv_heads * dim:]
+            uk.qk_norm_rope(q, k, self.turned, None, batch, heads, kv_heads, dim, F.ATTENTION_TYPE_F16,
+                            q_weight=weights[0], k_weight=weights[1], eps=2.0**-17, cos_sin=table, table_rows=256,
+                            rotary_dim=dim, positions=positions, q_stride0=row, k_stride0=row, v=v, v_stride0=row,
+                            cache=pool.layer(0), pages=pool.pages, page_size=page, slots=slots)
+            uk.attention_kv4(self.turned, self.seen, pool.layer(0), pool.pages, page, tables[0], ones, tables[1], batch,
+                             batch, heads, kv_heads, dim, tables[2], F.ATTENTION_TYPE_F16, scale=dim**-0.5)
+            project(self.seen, w_o, self.added, hidden, hidden)
+            mlp(self.added, self.y, batch)
+
+    # what is cached before the first step: rows of their own, nothing for the first sequence
+    lens = [7 * i % 61 for i in range(batch)]
+    slots = pool.extend(seqs, lens)
+    k, v = (_normal(gen, sum(lens), kv_heads, dim).half() for _ in range(2))
+    uk.qk_norm_rope(None, k, None, None, sum(lens), 0, kv_heads, dim, F.ATTENTION_TYPE_F16, v=v, cache=pool.layer(0),
+                    pages=pool.pages, page_size=page, slots=slots)
+    eager, replayed = Step(), Step()
+    # (tables for all steps at once, as wide as they come to be; lengths and slots are a step's own)
+    steps = 3
+    new_slots = pool.extend(seqs, [steps] * batch).view(batch, steps)
+    wide_table, _, wide = pool.tables(seqs)
+    x, positions = torch.empty(batch, hidden, dtype=F16, device="cuda"), torch.empty_like(ones[:batch])
+    slots, kv_lens = torch.empty(batch, dtype=torch.int64, device="cuda"), torch.empty_like(positions)
+    tables = (wide_table, kv_lens, wide)
+    ended = 9
+    graph = None
+    for step in range(steps):
+        x.copy_(_normal(gen, batch, hidden))
+        positions.copy_(torch.tensor(lens).int() + step)
+        slots.copy_(new_slots[:, step])
+        kv_lens.copy_(positions + 1)
+        if step:
+            positions[ended] = slots[ended] = -1
+            kv_lens[ended] = 0
+        before = pool.buffer.clone()
+        eager.turned.zero_()
+        eager.run(x, positions, slots, tables)
+        after = pool.buffer.clone()
+        if graph is None:
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                replayed.run(x, positions, slots, tables)
+        pool.buffer.copy_(before)
+        replayed.turned.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(pool.buffer, after)
+        for name in ("qkv", "turned", "seen", "added", "y"):
+            assert torch.equal(getattr(eager, name), getattr(replayed, name)), name
+        assert bool(torch.isfinite(eager.y).all())
+        # projections: f32 sums of exact products, or of products with a weight rounded to f16, one
+        # rounding at the end
+        for got, weight, source in ((eager.qkv, w_qkv, x), (eager.added, w_o, eager.seen)):
+            w = dense(weight, got.shape[1], hidden)
+            size = source.double().abs() @ w.abs().T.contiguous()
+            kv4ref.assert_near(got, source.double() @ w.T.contiguous(), size * (2.0**-11 + hidden * 2.0**-24))
+        live = positions >= 0
+        q = eager.qkv[:, :hidden].view(batch, heads, dim)
+        want = kv4ref.norm_rope(q, weights[0], 2.0**-17, table, positions.clamp(min=0), False)
+        # (f32: 64 products and a few steps more)
+        kv4ref.assert_near(eager.turned.view(batch, heads, dim), want, 80 * 2.0**-24 * want.abs().amax(-1, keepdim=True), live)
+        want, bound = kv4ref.attention(eager.turned.view(batch, heads, dim), pool.buffer, page, wide_table,
+                                       list(range(batch + 1)), kv_lens.tolist(), kv_heads, dim**-0.5)
+        kv4ref.assert_near(eager.seen.view(batch, heads, dim), want, bound)
+        if step:
+            assert bool((eager.seen[ended] == 0).all()) and bool((eager.turned[ended] == 0).all())
+
+
 # ---------------------------------------------------------------------------
 # copy_pages, Kv4Cache
 # ---------------------------------------------------------------------------
@@ -493,6 +655,29 @@ def test_copy_pages(uk, cuda, pages, page_bytes, gap, count):
     assert torch.equal(pool, want)
     uk.copy_pages(pool, pages, page_bytes, [], [])
     assert torch.equal(pool, want)
+
+
+def test_copy_pages_captured(uk, cuda):
+    """A captured call copies its pages as they are at each replay; what the program does with its
+    lists of page numbers afterwards changes nothing. 800 pairs: more than one launch."""
+    gen = _gen(6)
+    pool = torch.empty(2000, 144, dtype=torch.uint8, device="cuda")
+    perm = torch.randperm(2000, generator=gen, device="cuda").int().cpu()
+    src, dst = perm[:800].clone(), perm[800:1600].clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        uk.copy_pages(pool, 2000, 144, src, dst)
+    at = src.long().cuda(), dst.long().cuda()
+    src.fill_(0)
+    dst.fill_(1999)
+    for _ in range(3):
+        pool.copy_(torch.randint(0, 256, (2000, 144), generator=gen, device="cuda", dtype=torch.uint8))
+        want = pool.clone()
+        want[at[1]] = want[at[0]]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(pool, want)
 
 
 def test_sequences_fork_drop_and_compact(uk, cuda):
