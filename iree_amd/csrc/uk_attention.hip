@@ -23,9 +23,9 @@ using namespace kv4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Where a workgroup's rows stand. Rows r of a sequence are its query tokens times the G
-// heads of one kv head, token by token; tiles of R rows are numbered over the batch with
-// gaps: sequence b has the tiles from floor(q_starts[b] G / R) + b on, which leaves room
-// for its own and needs no sums over the batch.
+// heads of one kv head, token by token. Tiles of R rows are numbered over the batch: number b
+// < batch is the first tile of sequence b (a decode step has no others), the numbers from
+// batch on are the sequences' further tiles.
 struct Rows {
   int b;             // sequence, -1: none
   int first;         // first row of the tile
@@ -36,36 +36,57 @@ struct Rows {
   int64_t slot;
 };
 
-// The sequence of tile `slot`: the last b whose first tile is at most it. 64 lanes look at
-// 64 sequences at a time, with all that is asked of them, so a batch of up to 64 costs one
-// memory latency.
+// Of up to 64 sequences the further tiles stand one after the other, as a sum over 64 lanes
+// finds them. Of more, sequence b's begin at floor(q_starts[b] G / R), which leaves room for
+// all before it, and the last sequence that begins at or before a number is the one to have it:
+// 64 lanes look for it at 64 sequences at a time. (Numbers without rows cost more than their own
+// start: workgroups go to the parts of the device in turn, and with every second number empty half of it
+// stays idle: 16 sequences of 128 rows, 414 us instead of 241.)
 __device__ inline Rows find_rows(const AttentionKv4Args& a, int64_t slot, int G, int R) {
   const int lane = threadIdx.x & 63;
-  int64_t lo = 0, n = a.batch;                      // candidates [lo, lo + n)
-  while (n > 64) {
-    const int64_t step = (n + 63) / 64;
-    const int64_t b = lo + lane * step;
-    const uint64_t yes = __ballot(b < lo + n && (int64_t)a.q_starts[b < lo + n ? b : lo] * G / R + b <= slot);
-    const int64_t from = lo + (yes ? 63 - __builtin_clzll(yes) : 0) * step;
-    n = from + step < lo + n ? step : lo + n - from;
-    lo = from;
+  const int64_t further = slot - a.batch;
+  int64_t b = slot, tile = 0;
+  if (further >= 0) {
+    int64_t lo = 0, n = a.batch;                    // candidates [lo, lo + n)
+    while (n > 64) {
+      const int64_t step = (n + 63) / 64;
+      const int64_t at = lo + lane * step;
+      const uint64_t yes = __ballot(at < lo + n && (int64_t)a.q_starts[at < lo + n ? at : lo] * G / R <= further);
+      const int64_t from = lo + (yes ? 63 - __builtin_clzll(yes) : 0) * step;
+      n = from + step < lo + n ? step : lo + n - from;
+      lo = from;
+    }
+    const int64_t at = lo + (lane < n ? lane : n - 1);
+    const int64_t start = a.q_starts[at];
+    int64_t before = start * G / R;
+    if (a.batch <= 64) {
+      const int64_t rows = (a.q_starts[at + 1] - start) * G;
+      const int mine = lane < n && rows > 0 ? (int)((rows - 1) / R) : 0;
+      int sum = mine;
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        const int other = __shfl_up(sum, m);
+        sum += lane >= m ? other : 0;
+      }
+      before = sum - mine;
+    }
+    const uint64_t yes = __ballot(lane < n && before <= further);
+    const int last = yes ? 63 - __builtin_clzll(yes) : 0;
+    b = lo + last;
+    tile = further - __builtin_amdgcn_readlane((int)before, last) + 1;
   }
-  const int64_t b = lo + (lane < n ? lane : n - 1);
-  const int start = a.q_starts[b], next = a.q_starts[b + 1], len = a.kv_lens[b];
-  const uint64_t yes = __ballot(lane < n && (int64_t)start * G / R + b <= slot);
-  const int last = yes ? 63 - __builtin_clzll(yes) : 0;
-  const int from = __builtin_amdgcn_readlane(start, last), to = __builtin_amdgcn_readlane(next, last);
-  const int64_t first = (slot - ((int64_t)from * G / R + lo + last)) * R;
-  const int64_t rows = ((int64_t)to - from) * G;
+  b = __builtin_amdgcn_readfirstlane((int)b);
+  const int from = a.q_starts[b], to = a.q_starts[b + 1];
+  const int64_t first = tile * R, rows = ((int64_t)to - from) * G;
   const bool mine = from >= 0 && to <= a.tokens && first >= 0 && first < rows;
   // (the same in all lanes, which the compiler is told: all addresses follow from them)
   Rows r;
-  r.b = __builtin_amdgcn_readfirstlane(mine ? (int)(lo + last) : -1);
+  r.b = __builtin_amdgcn_readfirstlane(mine ? (int)b : -1);
   r.first = __builtin_amdgcn_readfirstlane((int)first);
   r.count = __builtin_amdgcn_readfirstlane((int)rows);
   r.tokens = __builtin_amdgcn_readfirstlane(to - from);
   r.token0 = __builtin_amdgcn_readfirstlane(from);
-  r.kv_len = __builtin_amdgcn_readlane(len, last);
+  r.kv_len = __builtin_amdgcn_readfirstlane(a.kv_lens[b]);
   r.slot = slot;
   return r;
 }
@@ -641,15 +662,14 @@ __global__ __launch_bounds__(kJoinThreads) void attention_kv4_join_kernel(SplitA
 // ---------------------------------------------------------------------------
 
 constexpr int kPromptRows = 128;      // of a workgroup, 32 of each of its four waves
-template <int D>
-constexpr int prompt_keys() { return D == 256 ? 32 : 64; }
+constexpr int kPromptKeys = 64;
 
 // One of the two buffers of key tiles in LDS: K and V codes as f16 in the order in which the
 // lanes read them, then the keys' parameters, scale and offset (of V: scale and offset + 8
 // scales, rounded to f16, next to which the rounding of the weights is several times as large).
 template <int D>
 struct PromptLds {
-  static constexpr int N = prompt_keys<D>();
+  static constexpr int N = kPromptKeys;
   static constexpr int kV = N * D * 2;                  // K before it: [N / 32][D / 16][64 lanes] of 16 bytes
   static constexpr int kParams = 2 * kV;                // V: [N / 16][D / 32][64 lanes]
   static constexpr int kBytes = kParams + N * 8;
@@ -664,9 +684,9 @@ constexpr int prompt_lds_bytes() { return 2 * PromptLds<D>::kBytes + 64; }
 // score (three for scale and offset, one each for the largest, the sum, the offsets of V and
 // the operand, an exponential at a quarter of the rate).
 template <int D, typename T>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_kernel(SplitArgs args) {
+__global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
-  constexpr int N = prompt_keys<D>(), KB = N / 32, KK = N / 16;     // keys; blocks of 32; steps of 16
+  constexpr int N = kPromptKeys, KB = N / 32, KK = N / 16;     // keys; blocks of 32; steps of 16
   constexpr int S = D / 16, DB = D / 32;                            // steps of a score; blocks of d
   extern __shared__ __attribute__((aligned(1024))) char memory[];
   const int G = args.group;
@@ -728,15 +748,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
     qsum = sum * (fabsf(a.scale) * kLog2e);
   }
 
-  // Staging. A wave takes a group of 16 keys (D = 256: half of one's bytes), so that their page
-  // is the same for all its lanes: 16 (D = 64: 8) bytes of K codes a lane, and of V the 8 keys
+  // Staging. A wave takes a group of 16 keys, so that their page is the same for all its lanes: 16 (D = 64: 8) bytes of K codes a lane, and of V the 8 keys
   // x 8 d of two 16-byte pieces to two (four) lanes, which turn a part of the d each.
   const int shift = a.pool.page_shift, page_size = 1 << shift, pages = (int)a.pool.pages, wide = (int)a.max_pages;
   const char* base = a.pool.base + head * Block<D>::bytes(page_size);
   const int32_t* table = a.page_table + rows.b * a.page_table_stride;
   constexpr int KL = D == 64 ? 2 : 4;                    // dwords of K to a lane
   constexpr int VL = D == 64 ? 4 : 2;                    // lanes to a unit of V
-  const int group = D == 256 ? wave >> 1 : wave, part_of = D == 256 ? wave & 1 : 0;
+  const int group = wave;
   // (a lane's places are worked out anew for each tile: kept over the loop, they would take the
   // registers of the results)
   struct Place {
@@ -746,9 +765,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
     Place w;
     w.lane = lane;
     asm volatile("" : "+v"(w.lane));
-    const int unit = w.lane / VL + (D == 256 ? 32 * part_of : 0), piece = w.lane + 64 * part_of;
+    const int unit = w.lane / VL;
     w.v_h = unit / (D / 8), w.v_w = unit % (D / 8);
-    w.k_row = piece / (D / 8 / KL), w.k_c = piece % (D / 8 / KL) * KL;
+    w.k_row = w.lane / (D / 8 / KL), w.k_c = w.lane % (D / 8 / KL) * KL;
     return w;
   };
   int pages_from = begin, page_ids = -1;
@@ -824,26 +843,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
       *(half8*)(v_to + ((2 * b) ^ turn) * 16) = even.f;
       *(half8*)(v_to + ((2 * b + 1) ^ turn) * 16) = odd.f;
     }
-    if (part_of == 0) {
-      // A key whose V row is not finite (in scale or offset) gets a K row that is not, and zeros
-      // for V: rows that see it have a NaN for their weight, for all others its weight is 0.
-      const bool broken = (raw_p & 0x7C00u) == 0x7C00u || (raw_p & 0x7C000000u) == 0x7C000000u;
-      const uint32_t all_broken = (uint32_t)__ballot(broken);
-      const half2v sm = as_half2(broken ? 0u : raw_p);
-      float most = (float)sm[0];
-      most = row16_max(most);
-      uint32_t bits;
-      if (lane >= 16) {
-        half2v v = sm;
-        v[1] = (_Float16)fmaf((float)sm[0], 8.f, (float)sm[1]);
-        bits = __builtin_bit_cast(uint32_t, v);
-      } else {
-        bits = (all_broken | all_broken >> 16) >> lane & 1 ? 0x7E007E00u : raw_p;
-      }
-      if (lane < 32)
-        *(uint32_t*)(to + PromptLds<D>::kParams + (lane >= 16 ? N * 4 : 0) + (16 * group + (lane & 15)) * 4) = bits;
-      if (lane == 16) scales[4 * buffer + group] = most;
+    // A key whose V row is not finite (in scale or offset) gets a K row that is not, and zeros
+    // for V: rows that see it have a NaN for their weight, for all others its weight is 0.
+    const bool broken = (raw_p & 0x7C00u) == 0x7C00u || (raw_p & 0x7C000000u) == 0x7C000000u;
+    const uint32_t all_broken = (uint32_t)__ballot(broken);
+    const half2v sm = as_half2(broken ? 0u : raw_p);
+    float most = (float)sm[0];
+    most = row16_max(most);
+    uint32_t bits;
+    if (lane >= 16) {
+      half2v v = sm;
+      v[1] = (_Float16)fmaf((float)sm[0], 8.f, (float)sm[1]);
+      bits = __builtin_bit_cast(uint32_t, v);
+    } else {
+      bits = (all_broken | all_broken >> 16) >> lane & 1 ? 0x7E007E00u : raw_p;
     }
+    if (lane < 32)
+      *(uint32_t*)(to + PromptLds<D>::kParams + (lane >= 16 ? N * 4 : 0) + (16 * group + (lane & 15)) * 4) = bits;
+    if (lane == 16) scales[4 * buffer + group] = most;
   };
 
   floatx16 o[DB];
@@ -994,41 +1011,63 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_kv4_prompt_ke
 // grid can hold, and of the keys the longest sequence shows them.
 struct Split {
   bool prompt;
-  int64_t tiles;       // of rows, with the gaps of their numbering
+  int64_t tiles;       // numbers of tiles of rows
   int splits, chunk;
   bool past;           // few rows: keys past the caches
 };
 
+// Splits of the prompt kernel: `units` workgroups with `tiles` key tiles each at most. In half
+// microseconds, a key tile costs 7.2 for each two workgroups that share a compute unit and 6 for a
+// last one alone, a workgroup's start about four tiles, the join a little and more with each
+// partial result. (8 sequences of 8192 keys with 128 rows each, 64 units: 8 splits 85 us, 4 splits 121;
+// with 512 rows, 256 units: 2 splits 236 us, none 290.)
+int64_t prompt_splits(int64_t units, int64_t tiles, int64_t cus) {
+  int64_t best = 1;
+  double least = INFINITY;
+  for (int64_t s = 1; s == 1 || (s <= tiles / 8 && s <= 64); ++s) {
+    const int64_t load = ceil_div(units * s, cus);         // workgroups of the busiest compute unit
+    const double tile = 7.2 * (load / 2) + 6 * (load % 2);
+    const double cost = (ceil_div(tiles, s) + 4) * tile + (s > 1 ? 8 + 0.02 * units * s : 0);
+    if (cost < 0.95 * least) best = s, least = cost;      // (more of them only where it shows)
+  }
+  return best;
+}
+
 Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int64_t window, int64_t sinks,
            int64_t max_kv_len) {
-  const int64_t G = heads / kv_heads, rows = tokens * G;
+  const int64_t G = heads / kv_heads, rows = tokens * G, cus = device_cu_count();
+  auto seen = [&](int64_t R, int64_t tile) {           // keys that a tile of R rows sees
+    int64_t keys = max_kv_len;
+    const int64_t reach = window + sinks + R / G + 2 * tile;
+    if (window && reach < keys) keys = reach;
+    return keys < 1 ? 1 : keys > 0x7FFFFFFF ? 0x7FFFFFFF : keys;
+  };
+  auto units_of = [&](int64_t R) { return batch * ceil_div(ceil_div(rows, batch), R) * kv_heads; };
+  // Prompts where sequences have a tile's rows on average and there is work for the whole device
+  // (8 sequences of 8192 keys with 128 rows each 85 us, as few rows 91; 4 of 1024 keys with 384 rows
+  // 37, as few rows 24, with 2048 rows 64 and 88). Never with heads of 256, whose tiles leave room for one
+  // wave on a vector unit (2048 rows on 4096 keys 349 us, as few rows 235).
   Split p;
-  p.prompt = rows >= 64 * batch;
-  const int64_t R = p.prompt ? kPromptRows : kRows, tile = !p.prompt ? kTile : dim == 256 ? 32 : 64;
-  p.tiles = rows / R + batch;
-  int64_t keys = max_kv_len;
-  if (window && window + sinks + (p.prompt ? R / G : 0) < keys) keys = window + sinks + (p.prompt ? R / G : 0) + 2 * tile;
-  if (keys > 0x7FFFFFFF) keys = 0x7FFFFFFF;
-  const int64_t key_tiles = keys < 1 ? 1 : ceil_div(keys, tile);
-  const int64_t units = (rows / R < batch ? batch : rows / R) * kv_heads;
-  const int64_t cus = device_cu_count();
+  int64_t units = units_of(kPromptRows), keys = seen(kPromptRows, kPromptKeys);
+  p.prompt = dim <= 128 && rows >= kPromptRows * batch &&
+             (units >= cus || units * ceil_div(keys, kPromptKeys) >= 32 * cus);
+  if (!p.prompt) units = units_of(kRows), keys = seen(kRows, kTile);
+  p.tiles = rows / (p.prompt ? kPromptRows : kRows) + batch;
   // Keys that one tile of rows reads once, and that are too many for the caches to hold until the
   // next step, go past them: two sequences of 131072 keys 54.8 us through them, 50.4 past them; 72 MB
   // of windows that a repeated call still finds there 20.8 and 21.4.
   p.past = !p.prompt && tokens <= batch && G <= kRows && (double)batch * keys * kv_heads * (dim + 8) > 128e6;
+  const int64_t key_tiles = ceil_div(keys, p.prompt ? kPromptKeys : kTile);
   int64_t splits;
   if (p.prompt) {
-    // Two workgroups to a compute unit; the tiles of a prompt see half of its keys on average.
-    splits = ceil_div(2 * cus, units);
-    const int64_t most = key_tiles / 8;
-    splits = units >= cus ? 1 : splits < most ? splits : most;
+    splits = prompt_splits(units, key_tiles, cus);
   } else {
-    // Six workgroups to a compute unit, so that lengths that differ even out (32 sequences of
-    // 1000 to 8192 keys: 40.9 us, with four 44.5, with eight 42.6), but no more than 32 splits where
+    // Five workgroups to a compute unit, so that lengths that differ even out (32 sequences of
+    // 1000 to 8192 keys: 40.5 us, with four 45.2, with eight 42.9), but no more than 32 splits where
     // fewer fill the device: the join reads them all (two of 131072 keys: 49.4 us, with 48 splits
     // 53.0, with 64 52.0). A split has enough tiles to be worth its start and the join, fewer where
     // most of the device is idle.
-    splits = ceil_div(6 * cus, units);
+    splits = ceil_div(5 * cus, units);
     if (splits > 32) splits = ceil_div(2 * cus, units) > 32 ? ceil_div(2 * cus, units) : 32;
     const int64_t most = 2 * units <= cus ? ceil_div(key_tiles, 16) : key_tiles / 32;
     splits = splits < most ? splits : most;
@@ -1064,13 +1103,17 @@ int launch_split(const AttentionKv4Args& a, hipStream_t s) {
   SplitArgs args{a, a.heads / a.kv_heads, p.splits, p.chunk};
   static PerDeviceOnce once[3];
   const dim3 grid((unsigned)blocks, (unsigned)p.splits);
-  if (p.prompt) {
-    UK_RETURN_IF_ERROR(allow_lds(attention_kv4_prompt_kernel<D, T>, prompt_lds_bytes<D>(), once[0]));
-    hipLaunchKernelGGL((attention_kv4_prompt_kernel<D, T>), grid, dim3(256), prompt_lds_bytes<D>(), s, args);
-  } else {
-    const auto kernel = p.past ? attention_kv4_split_kernel<D, T, true> : attention_kv4_split_kernel<D, T, false>;
-    UK_RETURN_IF_ERROR(allow_lds(kernel, split_lds_bytes<D>(), once[p.past ? 1 : 2]));
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), split_lds_bytes<D>(), s, args);
+  auto run = [&](auto kernel, int bytes, PerDeviceOnce& set) {
+    UK_RETURN_IF_ERROR(allow_lds(kernel, bytes, set));
+    hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, s, args);
+    return 0;
+  };
+  if (!p.prompt && p.past) {
+    UK_RETURN_IF_ERROR(run(attention_kv4_split_kernel<D, T, true>, split_lds_bytes<D>(), once[0]));
+  } else if (!p.prompt) {
+    UK_RETURN_IF_ERROR(run(attention_kv4_split_kernel<D, T, false>, split_lds_bytes<D>(), once[1]));
+  } else if constexpr (D <= 128) {
+    UK_RETURN_IF_ERROR(run(attention_kv4_prompt_kernel<D, T>, prompt_lds_bytes<D>(), once[2]));
   }
   UK_RETURN_IF_HIP(hipGetLastError());
   if (p.splits == 1) return 0;
@@ -1081,10 +1124,10 @@ int launch_split(const AttentionKv4Args& a, hipStream_t s) {
   shares = shares < 1 ? 1 : shares > R ? R : shares;
   if (p.prompt && shares < 8) shares = 8;
   const dim3 join((unsigned)blocks, (unsigned)shares);
-  if (p.prompt)
-    hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kPromptRows, prompt_keys<D>()>), join, dim3(kJoinThreads), 0, s, args);
-  else
+  if (!p.prompt)
     hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kRows, kTile>), join, dim3(kJoinThreads), 0, s, args);
+  else if constexpr (D <= 128)
+    hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kPromptRows, kPromptKeys>), join, dim3(kJoinThreads), 0, s, args);
   return check_hip(hipGetLastError(), "attention_kv4");
 }
 
