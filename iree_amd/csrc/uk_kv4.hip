@@ -1,7 +1,10 @@
 // Head norms with position rotation, rows into and out of the 4-bit cache, and copies of
 // its pages (include/iree_amd_uk.h has the formulas and the layout).
 //
-// All four are bound by memory, or for a few tokens by the launch.
+// All four are bound by memory, or for a few tokens by the launch: norms and rotation of 4099 tokens
+// with 32 + 8 heads of 128, 85 MB, in 17.5 us (4.8 TB/s), of one token in 2.5; with values and the
+// cache 8191 tokens, 181 MB, in 46 us (3.9 TB/s: a 4-bit row is written in pieces of 16 and 64
+// bytes), and these rows back out of the cache, 42 MB, in 10.
 #include "uk_common.h"
 #include "uk_kv4.h"
 
