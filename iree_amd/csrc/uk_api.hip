@@ -1011,14 +1011,17 @@ extern "C" int iree_amd_uk_kv4_read(const void* cache, iree_amd_uk_index_t pages
   return launch_kv4_read(a, (hipStream_t)stream);
 }
 
-// Sizes that the call and its workspace query check alike.
+// Sizes that the call and its workspace query check, and bring into range, alike.
 static int validate_attention_sizes(const char* what, int64_t tokens, int64_t batch, int32_t heads, int32_t kv_heads,
-                                    int64_t window, int64_t sinks, int64_t max_kv_len) {
+                                    int64_t& window, int64_t& sinks, int64_t max_kv_len) {
   if (tokens < 0 || tokens > 0x7FFFFFFF || batch < 0 || batch > 0x7FFFFFFF || heads < 0 || heads > 0xFFFF ||
       window < 0 || sinks < 0 || max_kv_len < 0)
     return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: a size is negative or too large", what);
   if (heads && (kv_heads < 1 || heads % kv_heads))
     return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: heads must be a multiple of kv_heads", what);
+  // (positions lie below 2^31)
+  if (window >= 0x7FFFFFFF) window = 0;
+  if (sinks > 0x7FFFFFFF) sinks = 0x7FFFFFFF;
   return 0;
 }
 
@@ -1051,9 +1054,7 @@ extern "C" int iree_amd_uk_attention_kv4(
   a.page_table = page_table, a.page_table_stride = page_table_stride, a.max_pages = max_pages;
   a.q_starts = q_starts, a.kv_lens = kv_lens, a.tokens = tokens, a.batch = batch;
   a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
-  // (positions lie below 2^31)
-  a.window = window < 0x7FFFFFFF ? window : 0;
-  a.sinks = sinks < 0x7FFFFFFF ? sinks : 0x7FFFFFFF;
+  a.window = window, a.sinks = sinks;
   const int64_t capacity = max_pages << a.pool.page_shift;
   a.max_kv_len = max_kv_len && max_kv_len < capacity ? max_kv_len : capacity;
   a.workspace = workspace, a.workspace_bytes = workspace ? workspace_bytes : 0;

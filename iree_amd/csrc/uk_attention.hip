@@ -685,7 +685,7 @@ constexpr int prompt_lds_bytes() { return 2 * PromptLds<D>::kBytes + 64; }
 // few rows, 32 rows a wave. Two waves fit a vector unit, and one's softmax (ten instructions to a
 // score: three for scale and offset, one each for the largest, the sum, the offsets of V and the operand, an
 // exponential at a quarter of the rate) has only the other's products beside it: a prompt of
-// 4096 tokens, 32 heads of 128, 137 GFLOP, in 220 us (0.62 PFLOP/s), one of 8192 in 770 (0.72).
+// 4096 tokens, 32 heads of 128, 137 GFLOP, in 213 us (0.65 PFLOP/s), one of 8192 in 760 to 790 (0.70 to 0.72).
 template <int D, typename T>
 __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
@@ -820,16 +820,19 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs 
   asm volatile("v_mov_b32 %0, 0x54005400" : "=v"(bias_high));
   float* scales = (float*)(memory + 2 * PromptLds<D>::kBytes);      // per buffer and wave the largest scale of V
   // In LDS the d of a unit of V lie next to each other, turned by the unit, or the lanes that
-  // write them would meet in an eighth of the banks.
+  // write them would meet in an eighth of the banks; the lanes' places of a step of K likewise.
+  auto k_turn = [](int step) { return D == 128 ? step & 6 : 0; };
   auto stage = [&](int buffer) {
     const Place w = place();
     char* to = memory + buffer * PromptLds<D>::kBytes;
-    char* k_to = to + ((group >> 1) * S * 64 + w.k_c / 2 * 64 + w.k_c % 2 * 32 + (group & 1) * 16 + w.k_row) * 16;
+    char* k_to = to + ((group >> 1) * S * 64 + w.k_c / 2 * 64) * 16;
     char* v_to = to + PromptLds<D>::kV + ((group * DB + w.v_w / 4) * 64 + w.v_h * 32 + w.v_w % 4 * 8) * 16;
     const int turn = (w.v_w & 3) + 4 * w.v_h;
 #pragma unroll
-    for (int i = 0; i < KL; ++i)
-      *(half8*)(k_to + (i / 2 * 64 + i % 2 * 32) * 16) = k_frag(raw_k[i]);      // (k_c is even)
+    for (int i = 0; i < KL; ++i) {      // (k_c is even)
+      const int at = ((w.k_c + i) % 2 * 32 + (group & 1) * 16 + w.k_row) ^ k_turn(w.k_c / 2 + i / 2);
+      *(half8*)(k_to + (i / 2 * 64 + at) * 16) = k_frag(raw_k[i]);
+    }
 #pragma unroll
     for (int i = 0; i < 4 / VL; ++i) {
       // Byte b of every token's dword: d = 2 b and 2 b + 1.
@@ -905,7 +908,7 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs 
       for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
-          x[kb] = F16Cfg::mfma(*(const half8*)(from + ((kb * S + i) * 64 + lane) * 16), qf[i].f, x[kb]);
+          x[kb] = F16Cfg::mfma(*(const half8*)(from + ((kb * S + i) * 64 + (lane ^ k_turn(i))) * 16), qf[i].f, x[kb]);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll

@@ -396,6 +396,24 @@ def test_two_calls_at_once(uk, cuda):
     assert all(torch.equal(out, w) for w, mine in zip(want, outs) for out in mine)
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(F16, 8, 2, 128), (BF16, 4, 4, 64), (F16, 2, 1, 256)])
+def test_caches_too_large_to_stay_in_the_device_s_caches(uk, cuda, dtype, heads, kv_heads, dim):
+    """Steps whose keys may come to more than the device's caches hold, by the longest length, which read
+    them past these; each result is that of the step that is told of short ones, or nearly."""
+    kv_lens = [30001] + [3 * i for i in range(40)]
+    case = Case(8, dtype, heads, kv_heads, dim, 16, [1] * 41, kv_lens)
+    case.check(case.run(uk, max_kv_len=30001))
+    case.check(case.run(uk, max_kv_len=100))
+
+
+def test_windows_past_every_position_are_none(uk, cuda):
+    sizes = (2, 2, 8, 2, 128)
+    for window in (2**31, 2**63 - 1):
+        for sinks in (0, 2**63 - 1):
+            assert uk.attention_kv4_workspace(*sizes, max_kv_len=1 << 17, window=window, sinks=sinks) == \
+                uk.attention_kv4_workspace(*sizes, max_kv_len=1 << 17)
+
+
 def test_a_pool_past_32_bits(uk, cuda):
     """Pages whose bytes begin beyond 4 GiB, stored, read back, attended and copied."""
     dim, page, heads, pages, stride = 128, 16, 1, 4200, 1 << 20
