@@ -685,7 +685,7 @@ constexpr int prompt_lds_bytes() { return 2 * PromptLds<D>::kBytes + 64; }
 // few rows, 32 rows a wave. Two waves fit a vector unit, and one's softmax (ten instructions to a
 // score: three for scale and offset, one each for the largest, the sum, the offsets of V and the operand, an
 // exponential at a quarter of the rate) has only the other's products beside it: a prompt of
-// 4096 tokens, 32 heads of 128, 137 GFLOP, in 213 us (0.65 PFLOP/s), one of 8192 in 760 to 790 (0.70 to 0.72).
+// 4096 tokens, 32 heads of 128, 137 GFLOP, in 195 us (0.71 PFLOP/s), one of 8192 in 750 (0.73).
 template <int D, typename T>
 __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
@@ -759,20 +759,15 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs 
   constexpr int KL = D == 64 ? 2 : 4;                    // dwords of K to a lane
   constexpr int VL = D == 64 ? 4 : 2;                    // lanes to a unit of V
   const int group = wave;
-  // (a lane's places are worked out anew for each tile: kept over the loop, they would take the
-  // registers of the results)
-  struct Place {
-    int lane, v_h, v_w, k_row, k_c;
-  };
-  auto place = [&]() {
-    Place w;
-    w.lane = lane;
-    asm volatile("" : "+v"(w.lane));
-    const int unit = w.lane / VL;
-    w.v_h = unit / (D / 8), w.v_w = unit % (D / 8);
-    w.k_row = w.lane / (D / 8 / KL), w.k_c = w.lane % (D / 8 / KL) * KL;
-    return w;
-  };
+  auto k_turn = [](int step) { return D == 128 ? step & 6 : step * 2 & 6; };
+  // Where a lane's pieces lie in a block (behind a group's first key) and where they go in LDS.
+  const int v_h = lane / VL / (D / 8), v_w = lane / VL % (D / 8);
+  const int k_row = lane / (D / 8 / KL), k_c = lane % (D / 8 / KL) * KL;
+  const int k_from = k_row * (D / 2) + k_c * 4, v_from = v_h * (D / 8) * 16 + v_w * 16;
+  const int p_from = ((lane & 15) + (lane >> 4) * page_size) * 4;
+  const int k_to = ((group >> 1) * S * 64 + k_c / 2 * 64) * 16 + (((group & 1) * 16 + k_row) ^ k_turn(k_c / 2)) * 16;
+  const int v_to = PromptLds<D>::kV + ((group * DB + v_w / 4) * 64 + v_h * 32 + v_w % 4 * 8) * 16;
+  const int turn = (v_w & 3) + 4 * v_h;
   int pages_from = begin, page_ids = -1;
   auto fetch_pages = [&](int from) {
     const int t = from + lane / KK;
@@ -794,11 +789,10 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs 
     for (int i = 0; i < KL; ++i) raw_k[i] = 0;
     raw_p = 0;
     if (exist_next >> group & 1) {
-      const Place w = place();
       const int p = __builtin_amdgcn_readlane(page_ids, (t - pages_from) * KK + group);
       const char* block = base + p * a.pool.page_stride;
       const int r = key & (page_size - 1);
-      const char* k_at = block + Block<D>::k_row(r) + (w.k_row * (D / 2) + w.k_c * 4);
+      const char* k_at = block + Block<D>::k_row(r) + k_from;
       if constexpr (D == 64) {
         const u32x2 v = *(const u32x2*)k_at;
         raw_k[0] = v[0], raw_k[1] = v[1];
@@ -807,12 +801,12 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs 
 #pragma unroll
         for (int i = 0; i < 4; ++i) raw_k[i] = v[i];
       }
-      const char* v_at = block + Block<D>::v_dword(page_size, r, 0) + (w.v_h * (D / 8) * 16 + w.v_w * 16);
+      const char* v_at = block + Block<D>::v_dword(page_size, r, 0) + v_from;
       raw_v[0] = *(const u32x4*)v_at;
       raw_v[1] = *(const u32x4*)(v_at + D / 8 * 32);
       // (lanes 0..15: of K, 16..31: of V)
-      if (w.lane < 32 && key + (w.lane & 15) <= wg_hi)
-        raw_p = *(const uint32_t*)(block + Block<D>::k_params(page_size, r) + ((w.lane & 15) + (w.lane >> 4) * page_size) * 4);
+      if (lane < 32 && key + (lane & 15) <= wg_hi)
+        raw_p = *(const uint32_t*)(block + Block<D>::k_params(page_size, r) + p_from);
     }
   };
   uint32_t bias_low, bias_high;
@@ -821,22 +815,15 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs 
   float* scales = (float*)(memory + 2 * PromptLds<D>::kBytes);      // per buffer and wave the largest scale of V
   // In LDS the d of a unit of V lie next to each other, turned by the unit, or the lanes that
   // write them would meet in an eighth of the banks; the lanes' places of a step of K likewise.
-  auto k_turn = [](int step) { return D == 128 ? step & 6 : 0; };
   auto stage = [&](int buffer) {
-    const Place w = place();
     char* to = memory + buffer * PromptLds<D>::kBytes;
-    char* k_to = to + ((group >> 1) * S * 64 + w.k_c / 2 * 64) * 16;
-    char* v_to = to + PromptLds<D>::kV + ((group * DB + w.v_w / 4) * 64 + w.v_h * 32 + w.v_w % 4 * 8) * 16;
-    const int turn = (w.v_w & 3) + 4 * w.v_h;
+    // (the two halves of a step have the same turn, with D = 128 the next step's too)
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {      // (k_c is even)
-      const int at = ((w.k_c + i) % 2 * 32 + (group & 1) * 16 + w.k_row) ^ k_turn(w.k_c / 2 + i / 2);
-      *(half8*)(k_to + (i / 2 * 64 + at) * 16) = k_frag(raw_k[i]);
-    }
+    for (int i = 0; i < KL; ++i) *(half8*)(to + k_to + (i / 2 * 64 + i % 2 * 32) * 16) = k_frag(raw_k[i]);
 #pragma unroll
     for (int i = 0; i < 4 / VL; ++i) {
       // Byte b of every token's dword: d = 2 b and 2 b + 1.
-      const int b = w.lane % VL * (4 / VL) + i;
+      const int b = lane % VL * (4 / VL) + i;
       const uint32_t select = 0x0C040C00u | b | (b << 16);
       Frag even, odd;
 #pragma unroll
@@ -846,8 +833,8 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs 
         even.h[p] = low_codes(both, bias_low);
         odd.h[p] = high_codes(both, bias_high);
       }
-      *(half8*)(v_to + ((2 * b) ^ turn) * 16) = even.f;
-      *(half8*)(v_to + ((2 * b + 1) ^ turn) * 16) = odd.f;
+      *(half8*)(to + v_to + ((2 * b) ^ turn) * 16) = even.f;
+      *(half8*)(to + v_to + ((2 * b + 1) ^ turn) * 16) = odd.f;
     }
     // A key whose V row is not finite (in scale or offset) gets a K row that is not, and zeros
     // for V: rows that see it have a NaN for their weight, for all others its weight is 0.
