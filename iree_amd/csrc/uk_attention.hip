@@ -41,7 +41,7 @@ struct Rows {
 // all before it, and the last sequence that begins at or before a number is the one to have it:
 // 64 lanes look for it at 64 sequences at a time. (Numbers without rows cost more than their own
 // start: workgroups go to the parts of the device in turn, and with every second number empty half of it
-// stays idle: 16 sequences of 128 rows, 414 us instead of 241.)
+// stays idle: 16 sequences of 128 rows on 16384 keys in four splits, 414 us, so 241.)
 __device__ inline Rows find_rows(const AttentionKv4Args& a, int64_t slot, int G, int R) {
   const int lane = threadIdx.x & 63;
   const int64_t further = slot - a.batch;
@@ -1012,8 +1012,8 @@ struct Split {
 // Splits of the prompt kernel: `units` workgroups with `tiles` key tiles each at most. In half
 // microseconds, a key tile costs 7.2 for each two workgroups that share a compute unit and 6 for a
 // last one alone, a workgroup's start about four tiles, the join a little and more with each
-// partial result. (8 sequences of 8192 keys with 128 rows each, 64 units: 8 splits 85 us, 4 splits 121;
-// with 512 rows, 256 units: 2 splits 236 us, none 290.)
+// partial result. (8 sequences of 8192 keys with 128 rows each, 64 units: 8 splits 79 us, 4 splits 110;
+// with 512 rows, 256 units: 2 splits 215 us, none 258.)
 int64_t prompt_splits(int64_t units, int64_t tiles, int64_t cus) {
   int64_t best = 1;
   double least = INFINITY;
@@ -1037,8 +1037,8 @@ Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int6
   };
   auto units_of = [&](int64_t R) { return batch * ceil_div(ceil_div(rows, batch), R) * kv_heads; };
   // Prompts where sequences have a tile's rows on average and there is work for the whole device
-  // (8 sequences of 8192 keys with 128 rows each 85 us, as few rows 91; 4 of 1024 keys with 384 rows
-  // 37, as few rows 24, with 2048 rows 64 and 88). Never with heads of 256, whose tiles leave room for one
+  // (8 sequences of 8192 keys with 128 rows each 80 us, as few rows 94; 4 of 1024 keys with 384 rows
+  // 33, as few rows 23, with 2048 rows 58 and 87). Never with heads of 256, whose tiles leave room for one
   // wave on a vector unit (2048 rows on 4096 keys 349 us, as few rows 235).
   Split p;
   int64_t units = units_of(kPromptRows), keys = seen(kPromptRows, kPromptKeys);
