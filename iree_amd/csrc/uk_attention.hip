@@ -667,8 +667,9 @@ constexpr int kPromptRows = 128;      // of a workgroup, 32 of each of its four 
 constexpr int kPromptKeys = 64;
 
 // One of the two buffers of key tiles in LDS: K and V codes as f16 in the order in which the
-// lanes read them, then the keys' parameters, scale and offset (of V: scale and offset + 8
-// scales, rounded to f16, next to which the rounding of the weights is several times as large).
+// lanes read them, then the keys' parameters, scale and offset. (Offset + 8 scales of V is formed where
+// it is used, in f32: f16 ends at 65504, which either of the two may come to. From LDS as f32
+// it costs more than the multiply-add: a prompt of 8192 tokens 720 us, so 678.)
 template <int D>
 struct PromptLds {
   static constexpr int N = kPromptKeys;
@@ -682,12 +683,12 @@ constexpr int prompt_lds_bytes() { return 2 * PromptLds<D>::kBytes + 64; }
 // 128 rows of one kv head against its key tiles. The workgroup turns each tile's codes into f16
 // once, in LDS (centred for V, see above; subnormals for K), while its waves multiply the tile
 // before it: v_mfma_f32_32x32x16_f16 with the keys as rows of the scores, as in the kernel for
-// few rows, 32 rows a wave. Two waves fit a vector unit, and one's softmax (ten instructions to a
-// score: three for scale and offset, one each for the largest, the sum, the offsets of V and the operand, an
-// exponential at a quarter of the rate) has only the other's products beside it: a prompt of
-// 4096 tokens, 32 heads of 128, 137 GFLOP, in 195 us (0.71 PFLOP/s), one of 8192 in 750 (0.73).
+// few rows, 32 rows a wave. Two waves fit a vector unit (three with D = 64), and one's softmax (eleven
+// instructions to a score: three for scale and offset, one each for the largest, the sum and the operand, two
+// for the offsets of V, an exponential at a quarter of the rate) has only the other's products beside it: a prompt of
+// 4096 tokens, 32 heads of 128, 137 GFLOP, in 202 us (0.68 PFLOP/s), one of 8192 in 678 (0.81).
 template <int D, typename T>
-__global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs args) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_kv4_prompt_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
   constexpr int N = kPromptKeys, KB = N / 32, KK = N / 16;     // keys; blocks of 32; steps of 16
   constexpr int S = D / 16, DB = D / 32;                            // steps of a score; blocks of d
@@ -843,14 +844,8 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs 
     const half2v sm = as_half2(broken ? 0u : raw_p);
     float most = (float)sm[0];
     most = row16_max(most);
-    uint32_t bits;
-    if (lane >= 16) {
-      half2v v = sm;
-      v[1] = (_Float16)fmaf((float)sm[0], 8.f, (float)sm[1]);
-      bits = __builtin_bit_cast(uint32_t, v);
-    } else {
-      bits = (all_broken | all_broken >> 16) >> lane & 1 ? 0x7E007E00u : raw_p;
-    }
+    uint32_t bits = __builtin_bit_cast(uint32_t, sm);
+    if (lane < 16) bits = (all_broken | all_broken >> 16) >> lane & 1 ? 0x7E007E00u : raw_p;
     if (lane < 32)
       *(uint32_t*)(to + PromptLds<D>::kParams + (lane >= 16 ? N * 4 : 0) + (16 * group + (lane & 15)) * 4) = bits;
     if (lane == 16) scales[4 * buffer + group] = most;
@@ -953,7 +948,7 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_prompt_kernel(SplitArgs 
             const half2v sm = as_half2(vp[i]);
             const float w = __builtin_amdgcn_exp2f(x[kk / 2][kk % 2 * 8 + j + i]);
             l += w;
-            bias = fmaf(w, (float)sm[1], bias);
+            bias = fmaf(w, fmaf((float)sm[0], 8.f, (float)sm[1]), bias);
             p.f[j + i] = (_Float16)fmaf(w, (float)sm[0], 0.f);
           }
         }
