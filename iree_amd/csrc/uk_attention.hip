@@ -1104,7 +1104,10 @@ int launch_split(const AttentionKv4Args& a, hipStream_t s) {
     UK_RETURN_IF_ERROR(run(attention_kv4_prompt_kernel<D, T>, prompt_lds_bytes<D>(), once[2]));
   }
   UK_RETURN_IF_HIP(hipGetLastError());
-  if (p.splits == 1) return 0;
+  if (p.splits == 1) {
+    note_kernel_path(p.prompt ? "attention_kv4:prompt" : "attention_kv4:few-rows");
+    return 0;
+  }
   // A row a workgroup where the tiles are few, one workgroup a tile where they fill the device
   // (most rows of a tile are not there in a decode step, and each workgroup has to find that out).
   const int64_t R = p.prompt ? kPromptRows : kRows;
@@ -1116,7 +1119,9 @@ int launch_split(const AttentionKv4Args& a, hipStream_t s) {
     hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kRows, kTile>), join, dim3(kJoinThreads), 0, s, args);
   else if constexpr (D <= 128)
     hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kPromptRows, kPromptKeys>), join, dim3(kJoinThreads), 0, s, args);
-  return check_hip(hipGetLastError(), "attention_kv4");
+  UK_RETURN_IF_HIP(hipGetLastError());
+  note_kernel_path(p.prompt ? "attention_kv4:prompt-split" : "attention_kv4:few-rows-split");
+  return 0;
 }
 
 }  // namespace

@@ -29,8 +29,8 @@ def _check(status):
 
 
 def last_kernel_path():
-    """Name of the kernel family that served this thread's last mmt4d or
-    dequant_matmul_i4 call (see include/iree_amd_uk.h)."""
+    """Name of the kernel family that served this thread's last mmt4d,
+    dequant_matmul_i4 or attention_kv4 call (see include/iree_amd_uk.h)."""
     return load_library().iree_amd_uk_last_kernel_path().decode()
 
 
