@@ -22,6 +22,9 @@ using namespace kv4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+__device__ inline half2v as_half2(uint32_t u) { return __builtin_bit_cast(half2v, u); }
+
 // Where a workgroup's rows stand. Rows r of a sequence are its query tokens times the G
 // heads of one kv head, token by token. Tiles of R rows are numbered over the batch: number b
 // < batch is the first tile of sequence b (a decode step has no others), the numbers from
@@ -149,15 +152,19 @@ constexpr int kRows = 16;
 constexpr int kMaxSplits = 1024;
 
 // A row's weights p = 2^(score - ref) are carried against a reference that is only moved
-// when p s leaves the range of f16: it is set so that the largest score and the largest scale
-// of V together give 2^kTarget, and moved when a p s comes to 2^kMost (few rows), or when they
-// would together (prompts). What is dropped at the other end lies 2^-31 below the largest p s. A
-// scale counts as at least 2^-24; where it is 0, the sum of the p shows that they grow.
+// when p s leaves the range of f16: it is set so that the largest p s of the keys that the row sees
+// is 2^kTarget, and looked at again when a p s comes to 2^kMost (few rows), or when the tile's largest
+// score and its largest scale of V would together (prompts). What is dropped at the other end lies
+// 2^-31 below the largest p s. A scale counts as at least 2^-24; where it is 0, the sum of the p shows
+// that they grow.
 // p s is rounded to f16, at most 2^-11 of each weight, as the result is to its own type: 2.9e-4 of
 // the result of f16 rows in all, 2.1e-4 with a second f16 for the rest, which costs 4 us of 60 at
 // two caches of 131072 keys. The sums of p and of p (m + 8 s) stay in f32.
 constexpr int kTarget = 7, kMost = 13;
 constexpr float kMostWeight = 1 << kMost, kMostSum = 0x1p60f;
+
+// Of a key's scale and offset.
+__device__ inline float log2_scale(half2v sm) { return __builtin_amdgcn_logf(fmaxf((float)sm[0], 0x1p-24f)); }
 
 // Partial results of a split: per (tile, kv head, split) O [R][D], reference [R], sum [R].
 template <int D, int R>
@@ -217,14 +224,11 @@ __device__ inline void wait_loads() {
 
 __device__ inline void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 union Frag {
   uint32_t u[4];
   half2v h[4];
   half8 f;
 };
-
-__device__ inline half2v as_half2(uint32_t u) { return __builtin_bit_cast(half2v, u); }
 
 // A dword of K codes as 8 f16 subnormals, 2^-24 of their values (products and sums are exact
 // all the same): nibbles 0, 4, 1, 5, 2, 6, 3, 7, the odd ones 16 times too large, which the
@@ -489,17 +493,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
     most_w = __builtin_elementwise_max(most_w, __builtin_shufflevector(most_w, most_w, 1, 0));
     if (__ballot(most_w[0] > (_Float16)kMostWeight || l_next > kMostSum)) {
       float most = -INFINITY;
-      half2v smost = as_half2(vp[0]);                 // (scales are not negative, and the low halves)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const half2v sm = as_half2(kp[j]);
         x[j] = fmaf((float)sm[0], (j < 4 ? s0 : s1)[j & 3], (float)sm[1] * qsum);
         x[j] = seen >> j & 1 ? x[j] : -INFINITY;
-        most = fmaxf(most, x[j]);
-        smost = __builtin_elementwise_max(smost, as_half2(vp[j]));
+        most = fmaxf(most, x[j] + log2_scale(as_half2(vp[j])));
       }
-      const float stop = fmaxf(across_max((float)smost[0]), 0x1p-24f);
-      const float raised = fmaxf(ref, across_max(most) + (float)(__builtin_amdgcn_frexp_expf(stop) - 1 - kTarget));
+      const float raised = fmaxf(ref, across_max(most) - kTarget);
       const float factor = __builtin_amdgcn_exp2f(ref - raised);
       l *= factor;
       bias *= factor;
@@ -921,8 +922,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_kv4_prompt_ker
 #pragma unroll
         for (int j = 0; j < 16; ++j) top = fmaxf(top, x[kb][j]);
       if (__ballot(top > limit - (float)stop_e)) {
-        const float most = fmaxf(top, __shfl_xor(top, 32));
-        const float over = most + (float)(stop_e - 1 - kTarget);
+        float most = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const u32x4 vp = *(const u32x4*)(from + PromptLds<D>::kParams + (N + 32 * kb + 2 * j + 4 * h) * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, x[kb][j + i] + log2_scale(as_half2(vp[i])));
+          }
+        const float over = fmaxf(most, __shfl_xor(most, 32)) - kTarget;
         // (a row's first scores set its reference, wherever they lie; later ones only raise it)
         const float by = fresh ? (over > -INFINITY ? over : 0.f) : fmaxf(over, 0.f);
         const float factor = fresh ? 1.f : __builtin_amdgcn_exp2f(-by);

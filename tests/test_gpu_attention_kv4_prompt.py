@@ -236,3 +236,24 @@ def test_two_calls_at_once(uk, cuda):
             case.run(uk, out=mine[turn], stream=stream)
     torch.cuda.synchronize()
     assert all(torch.equal(out, w) for w, mine in zip(want, outs) for out in mine)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads,q_lens", [(8, 2, [1, 5]), WIDE])
+def test_a_key_of_all_the_weight_with_small_values(uk, cuda, dtype, dim, heads, kv_heads, q_lens):
+    """One key whose score is far above the others' and whose V row is 2^-28 of theirs: the weights keep
+    their bits next to what they are multiplied with."""
+    case = Case(33, dtype, heads, kv_heads, dim, 16, q_lens, [n + 150 for n in q_lens])
+    case.q.abs_()
+    gen = _gen(34)
+    shape = (case.pages, kv_heads, 16, dim)
+    k, v = _normal(gen, *shape), _normal(gen, *shape).clamp(-3, 3) * 2.0**14
+    for b in range(len(q_lens)):
+        page = int(case.table[b, 2])
+        k[page, :, 9] = 300 / dim
+        v[page, :, 9] *= 2.0**-28
+    _replace(case, k.half(), v.half())
+    case.check(case.run(uk, scale=0.13), scale=0.13)
+    if dim < 256:
+        assert uk.last_kernel_path() == "attention_kv4:" + ("prompt" if q_lens is WIDE[2] else "few-rows")
