@@ -768,9 +768,10 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_kv4_read(
  * sequences) lies in [0, pages) (a program that has freed the pages behind its window
  * writes -1), and j < max_pages * page_size, which is at most 2^31 - 4096.
  *   out = sum_j softmax_j(scale * q . k_j) v_j over the visible tokens
- * Scores, the softmax and sums in f32, a key's weight times its scale rounded to f16, the
- * result rounded once to the rows' type; zeros where nothing is visible. Rows of q outside [q_starts[0], q_starts[batch]) are neither read nor
- * written. What masked tokens and pages hold, NaN among it, changes nothing.
+ * Scores, the softmax and sums in f32, a key's weight times its scale to 22 bits for rows of f16,
+ * rounded to f16 for rows of bf16 (an eighth of the result's own rounding), the result rounded
+ * once to the rows' type; zeros where nothing is visible. Rows of q outside
+ * [q_starts[0], q_starts[batch]) are neither read nor written. What masked tokens and pages hold, NaN among it, changes nothing.
  *   max_kv_len: the longest of kv_lens as far as the caller knows (it sets how the work is
  * split, not what is computed; 0: max_pages * page_size).
  *   workspace: partial results of a long cache that is read by several workgroups, at

@@ -157,10 +157,14 @@ constexpr int kMaxSplits = 1024;
 // score and its largest scale of V would together (prompts). What is dropped at the other end lies
 // 2^-31 below the largest p s. A scale counts as at least 2^-24; where it is 0, the sum of the p shows
 // that they grow.
-// p s is rounded to f16, at most 2^-11 of each weight, as the result is to its own type: 2.9e-4 of
-// the result of f16 rows in all, 2.1e-4 with a second f16 for the rest, which costs 4 us of 60 at
-// two caches of 131072 keys. The sums of p and of p (m + 8 s) stay in f32.
+// p s goes to the matrix cores as f16, for rows of f16 with a second f16 for the rest. One f16, at most
+// 2^-11 of each weight off, next to a result of f16 would show: 2.9e-4 of it in all, 2.1e-4 with two, which is
+// the result's own rounding (two caches of 131072 keys 53 us, with two 58; a prompt of 4096 tokens 207 and
+// 248). Next to one of bf16 it does not: 1.67e-3, with two 1.66e-3. The sums of p and of p (m + 8 s)
+// stay in f32.
 constexpr int kTarget = 7, kMost = 13;
+template <typename T>
+constexpr bool kTwo = std::is_same<T, F16>::value;
 constexpr float kMostWeight = 1 << kMost, kMostSum = 0x1p60f;
 
 // Of a key's scale and offset.
@@ -474,7 +478,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
     }
     // The weights, and in the rare tile in which one is too large for f16 all again, against a
     // reference that holds for its largest score and scale.
-    Frag w;
+    Frag w, rest;
     float l_next, bias_next;
     auto weigh = [&]() {
       l_next = l, bias_next = bias;
@@ -485,6 +489,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
         l_next += p;
         bias_next = fmaf(p, fmaf((float)sm[0], 8.f, (float)sm[1]), bias_next);
         w.f[j] = (_Float16)fmaf(p, (float)sm[0], 0.f);
+        if constexpr (kTwo<T>) rest.f[j] = (_Float16)fmaf(p, (float)sm[0], -(float)w.f[j]);
       }
     };
     weigh();
@@ -525,6 +530,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
       }
       auto add = [&](int i, const Frag& v) {
         o[i] = F16Cfg16::mfma(v.f, w.f, o[i]);
+        if constexpr (kTwo<T>) o[i] = F16Cfg16::mfma(v.f, rest.f, o[i]);
       };
       auto byte = [&](auto which) {
         constexpr int b = decltype(which)::value;
@@ -948,7 +954,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_kv4_prompt_ker
       }
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        Frag p;
+        Frag p, rest;
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {
           const u32x4 vp = *(const u32x4*)(from + PromptLds<D>::kParams + (N + 16 * kk + 2 * j + 4 * h) * 4);
@@ -959,12 +965,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_kv4_prompt_ker
             l += w;
             bias = fmaf(w, fmaf((float)sm[0], 8.f, (float)sm[1]), bias);
             p.f[j + i] = (_Float16)fmaf(w, (float)sm[0], 0.f);
+            if constexpr (kTwo<T>) rest.f[j + i] = (_Float16)fmaf(w, (float)sm[0], -(float)p.f[j + i]);
           }
         }
+        half8 v[DB];
 #pragma unroll
         for (int i = 0; i < DB; ++i) {
           const int at = (kk * DB + i) * 64 + h * 32 + (n & 24) + ((n & 7) ^ ((n >> 3) + 4 * h));
-          o[i] = F16Cfg::mfma(*(const half8*)(from + PromptLds<D>::kV + at * 16), p.f, o[i]);
+          v[i] = *(const half8*)(from + PromptLds<D>::kV + at * 16);
+          o[i] = F16Cfg::mfma(v[i], p.f, o[i]);
+        }
+        // (after all of the first products, or each would wait for the one before it)
+        if constexpr (kTwo<T>) {
+#pragma unroll
+          for (int i = 0; i < DB; ++i) o[i] = F16Cfg::mfma(v[i], rest.f, o[i]);
         }
       }
     }

@@ -257,3 +257,23 @@ def test_a_key_of_all_the_weight_with_small_values(uk, cuda, dtype, dim, heads, 
     case.check(case.run(uk, scale=0.13), scale=0.13)
     if dim < 256:
         assert uk.last_kernel_path() == "attention_kv4:" + ("prompt" if q_lens is WIDE[2] else "few-rows")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads,q_lens,kv_lens", [(64, 8, [1] * 8, [300, 1000, 20000, 77, 4000, 513, 900, 65]),
+                                                           (*WIDE, [130, 500, 2000, 150])])
+def test_results_are_off_by_their_own_rounding(uk, cuda, dtype, dim, heads, kv_heads, q_lens, kv_lens):
+    """A rounding to a type is off evenly within half a step: by step^2 / 12 in the mean square. Over 32768 results
+    and more that mean is within 3 % (5 / sqrt(32768)) of it, and f32 scores and sums, at 2^-24 times a few hundred
+    (bf16: an f16 weight, whose 2^-11 is squared 1/64 of the result's 2^-8), leave the rest of a tenth. One f16 weight
+    a key would come to twice as much with results of f16."""
+    case = Case(71, dtype, heads, kv_heads, dim, 64, q_lens, kv_lens)
+    out = case.run(uk)
+    q = case.q[:, :heads * dim].reshape(case.tokens, heads, dim)
+    want, _ = kv4ref.attention(q, case.cache, 64, case.table[:, :case.wide], case.starts, kv_lens, kv_heads,
+                               case.scale(None))
+    got = out[case.rows][:, :heads * dim].double()
+    want = want[case.rows].reshape(got.shape)
+    step = torch.exp2(torch.frexp(want)[1].double()) * torch.finfo(dtype).eps / 2
+    assert float((got - want).square().mean()) < 1.1 * float(step.square().mean()) / 12
