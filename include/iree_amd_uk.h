@@ -776,7 +776,9 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_kv4_read(
  * split, not what is computed; 0: max_pages * page_size).
  *   workspace: partial results of a long cache that is read by several workgroups, at
  * least what iree_amd_uk_attention_kv4_workspace says, 16-byte aligned; with less, or
- * null, the call runs unsplit (slower). The caller's: calls that may overlap, and graphs
+ * null, the call runs unsplit: slower, and less exact where more than 65536 keys are visible (their
+ * f32 sums are rounded that often: 2.3e-4 of results of f16 on 131072 keys, 4.3e-4 on 524288, where
+ * their own rounding is 2.1e-4). The caller's: calls that may overlap, and graphs
  * whose replays may, need one each.
  * The library's memory is not used and nothing is allocated. Alignment as above. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4(
@@ -788,7 +790,9 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4(
     int32_t head_dim, float scale, iree_amd_uk_index_t window, iree_amd_uk_index_t sinks,
     iree_amd_uk_index_t max_kv_len, void* workspace, uint64_t workspace_bytes, uint32_t flags,
     void* stream);
-/* Bytes of workspace such a call of these sizes uses on the current device (0: none). */
+/* Bytes of workspace such a call of these sizes uses on the current device (0: none); at most 256 MiB, or
+ * where that is more what one tile of rows takes (128 rows of every kv head): long prompts
+ * run in several launches that share it. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4_workspace(
     iree_amd_uk_index_t tokens, iree_amd_uk_index_t batch, int32_t heads, int32_t kv_heads,
     int32_t head_dim, iree_amd_uk_index_t window, iree_amd_uk_index_t sinks,

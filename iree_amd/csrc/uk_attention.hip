@@ -170,7 +170,7 @@ constexpr float kMostWeight = 1 << kMost, kMostSum = 0x1p60f;
 // Of a key's scale and offset.
 __device__ inline float log2_scale(half2v sm) { return __builtin_amdgcn_logf(fmaxf((float)sm[0], 0x1p-24f)); }
 
-// Partial results of a split: per (tile, kv head, split) O [R][D], reference [R], sum [R].
+// Partial results of a split: per (tile of the launch, kv head, split) O [R][D], reference [R], sum [R].
 template <int D, int R>
 __host__ __device__ constexpr int64_t part_floats() { return R * (D + 2); }
 
@@ -178,6 +178,7 @@ struct SplitArgs {
   AttentionKv4Args a;
   int group;           // G
   int splits, chunk;   // key tiles of a split
+  int64_t slot0;       // number of the launch's first tile of rows
 };
 
 __device__ inline int active_splits(const SplitArgs& s, int total) {
@@ -295,7 +296,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(Spl
   float (*o_s)[kRows][D + 4] = (float (*)[kRows][D + 4])memory;      // (once all tiles are used)
   const int G = args.group;
   const int head = blockIdx.x % a.kv_heads;
-  const Rows rows = find_rows(a, blockIdx.x / a.kv_heads, G, kRows);
+  const Rows rows = find_rows(a, args.slot0 + blockIdx.x / a.kv_heads, G, kRows);
   if (rows.b < 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int last_row = rows.count - 1 < rows.first + kRows - 1 ? rows.count - 1 : rows.first + kRows - 1;
@@ -616,7 +617,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_kv4_join_kernel(SplitA
   constexpr int L = D / 4, kGroups = kJoinThreads / L;
   __shared__ float sum_s[kGroups][D], total_s[kGroups];
   const int head = blockIdx.x % a.kv_heads, G = args.group;
-  const Rows rows = find_rows(a, blockIdx.x / a.kv_heads, G, R);
+  const Rows rows = find_rows(a, args.slot0 + blockIdx.x / a.kv_heads, G, R);
   if (rows.b < 0) return;
   const int last_row = rows.count - 1 < rows.first + R - 1 ? rows.count - 1 : rows.first + R - 1;
   const Keys<kKeys> keys(a, position(rows, rows.first / G), position(rows, last_row / G));
@@ -703,7 +704,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_kv4_prompt_ker
   const int G = args.group;
   const int head = blockIdx.x % a.kv_heads;
   // (the last tiles of a prompt see most keys: they start first)
-  const Rows rows = find_rows(a, gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads, G, kPromptRows);
+  const Rows rows = find_rows(a, args.slot0 + gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads, G, kPromptRows);
   if (rows.b < 0) return;
   const int last_row = rows.count - 1 < rows.first + kPromptRows - 1 ? rows.count - 1 : rows.first + kPromptRows - 1;
   const int wg_lo = position(rows, rows.first / G), wg_hi = position(rows, last_row / G);
@@ -991,7 +992,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_kv4_prompt_ker
   bias += __shfl_xor(bias, 32);
   if (wave_first + n > wave_last) return;
   if (parts > 1) {
-    float* part = (float*)a.workspace + ((int64_t)(rows.slot * a.kv_heads + head) * args.splits + split) * part_floats<D, kPromptRows>();
+    const int64_t unit = (rows.slot - args.slot0) * a.kv_heads + head;
+    float* part = (float*)a.workspace + (unit * args.splits + split) * part_floats<D, kPromptRows>();
     const int r = wave * 32 + n;
 #pragma unroll
     for (int i = 0; i < DB; ++i)
@@ -1025,7 +1027,13 @@ struct Split {
   int64_t tiles;       // numbers of tiles of rows
   int splits, chunk;
   bool past;           // few rows: keys past the caches
+  int64_t slice;       // tiles of rows to a launch
+  uint64_t bytes;      // of partial results of a launch
 };
+// Partial results that a long prompt may ask for: more of them come from more work than fills the
+// device many times over (4096 workgroups of the prompt kernel), in launches one after the other that
+// use the same memory. (All at once, a prompt of 131072 tokens of 32 + 8 heads of 128 takes 17.5 GB.)
+constexpr uint64_t kMostPartBytes = 256ull << 20;
 
 // Splits of the prompt kernel: `units` workgroups with `tiles` key tiles each at most. In half
 // microseconds, a key tile costs 7.2 for each two workgroups that share a compute unit and 6 for a
@@ -1083,12 +1091,22 @@ Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int6
     const int64_t most = 2 * units <= cus ? ceil_div(key_tiles, 16) : key_tiles / 32;
     splits = splits < most ? splits : most;
   }
-  // (past 16384 keys the f32 sums of a wave would begin to show in the result)
+  // Past 16384 keys the f32 sums of a wave, which the matrix cores cut off, would begin to show in the
+  // result: f16 of a prompt on 65536 keys in one split 2.14e-4 off, on 131072 2.3e-4, on 524288 4.3e-4, next to
+  // 2.08e-4; of few rows on 524288 2.2e-4.
   if (splits < ceil_div(keys, 16384)) splits = ceil_div(keys, 16384);
   splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
   p.chunk = (int)ceil_div(key_tiles, splits);
   if (!p.prompt) p.chunk = (int)(ceil_div(p.chunk, kWaves) * kWaves);
   p.splits = (int)ceil_div(key_tiles, p.chunk);
+  p.slice = p.tiles;
+  p.bytes = 0;
+  if (p.splits > 1) {
+    const uint64_t one = (uint64_t)kv_heads * p.splits * (p.prompt ? kPromptRows : kRows) * (dim + 2) * 4;
+    const int64_t most = kMostPartBytes > one ? (int64_t)(kMostPartBytes / one) : 1;
+    p.slice = ceil_div(p.tiles, ceil_div(p.tiles, most));
+    p.bytes = p.slice * one;
+  }
   return p;
 }
 
@@ -1106,44 +1124,45 @@ int allow_lds(Kernel kernel, int bytes, PerDeviceOnce& once) {
 template <int D, typename T>
 int launch_split(const AttentionKv4Args& a, hipStream_t s) {
   Split p = plan(a.tokens, a.batch, a.heads, a.kv_heads, D, a.window, a.sinks, a.max_kv_len);
-  const int64_t blocks = p.tiles * a.kv_heads;
   // (a grid's threads are counted in 32 bits)
-  if (blocks > 0xFFFFFFFFll / 256) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "attention_kv4: too many rows for one call");
-  const uint64_t one = (uint64_t)blocks * (p.prompt ? part_floats<D, kPromptRows>() : part_floats<D, kRows>()) * 4;
-  if (p.splits > 1 && a.workspace_bytes < one * p.splits) p.splits = 1;
-  SplitArgs args{a, a.heads / a.kv_heads, p.splits, p.chunk};
+  if (p.tiles * a.kv_heads > 0xFFFFFFFFll / 256)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "attention_kv4: too many rows for one call");
+  if (p.splits > 1 && a.workspace_bytes < p.bytes) p.splits = 1, p.slice = p.tiles;
   static PerDeviceOnce once[3];
-  const dim3 grid((unsigned)blocks, (unsigned)p.splits);
-  auto run = [&](auto kernel, int bytes, PerDeviceOnce& set) {
-    UK_RETURN_IF_ERROR(allow_lds(kernel, bytes, set));
-    hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, s, args);
-    return 0;
-  };
-  if (!p.prompt && p.past) {
-    UK_RETURN_IF_ERROR(run(attention_kv4_split_kernel<D, T, true>, split_lds_bytes<D>(), once[0]));
-  } else if (!p.prompt) {
-    UK_RETURN_IF_ERROR(run(attention_kv4_split_kernel<D, T, false>, split_lds_bytes<D>(), once[1]));
-  } else if constexpr (D <= 128) {
-    UK_RETURN_IF_ERROR(run(attention_kv4_prompt_kernel<D, T>, prompt_lds_bytes<D>(), once[2]));
+  // (a prompt's last tiles see most keys: they start first)
+  for (int64_t to = p.tiles; to > 0; to -= p.slice) {
+    const int64_t from = to > p.slice ? to - p.slice : 0, blocks = (to - from) * a.kv_heads;
+    SplitArgs args{a, a.heads / a.kv_heads, p.splits, p.chunk, from};
+    const dim3 grid((unsigned)blocks, (unsigned)p.splits);
+    auto run = [&](auto kernel, int bytes, PerDeviceOnce& set) {
+      UK_RETURN_IF_ERROR(allow_lds(kernel, bytes, set));
+      hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, s, args);
+      return 0;
+    };
+    if (!p.prompt && p.past) {
+      UK_RETURN_IF_ERROR(run(attention_kv4_split_kernel<D, T, true>, split_lds_bytes<D>(), once[0]));
+    } else if (!p.prompt) {
+      UK_RETURN_IF_ERROR(run(attention_kv4_split_kernel<D, T, false>, split_lds_bytes<D>(), once[1]));
+    } else if constexpr (D <= 128) {
+      UK_RETURN_IF_ERROR(run(attention_kv4_prompt_kernel<D, T>, prompt_lds_bytes<D>(), once[2]));
+    }
+    UK_RETURN_IF_HIP(hipGetLastError());
+    if (p.splits == 1) continue;
+    // A row a workgroup where the tiles are few, one workgroup a tile where they fill the device
+    // (most rows of a tile are not there in a decode step, and each workgroup has to find that out).
+    const int64_t R = p.prompt ? kPromptRows : kRows;
+    int64_t shares = 2ll * device_cu_count() / blocks;
+    shares = shares < 1 ? 1 : shares > R ? R : shares;
+    if (p.prompt && shares < 8) shares = 8;
+    const dim3 join((unsigned)blocks, (unsigned)shares);
+    if (!p.prompt)
+      hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kRows, kTile>), join, dim3(kJoinThreads), 0, s, args);
+    else if constexpr (D <= 128)
+      hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kPromptRows, kPromptKeys>), join, dim3(kJoinThreads), 0, s, args);
+    UK_RETURN_IF_HIP(hipGetLastError());
   }
-  UK_RETURN_IF_HIP(hipGetLastError());
-  if (p.splits == 1) {
-    note_kernel_path(p.prompt ? "attention_kv4:prompt" : "attention_kv4:few-rows");
-    return 0;
-  }
-  // A row a workgroup where the tiles are few, one workgroup a tile where they fill the device
-  // (most rows of a tile are not there in a decode step, and each workgroup has to find that out).
-  const int64_t R = p.prompt ? kPromptRows : kRows;
-  int64_t shares = 2ll * device_cu_count() / blocks;
-  shares = shares < 1 ? 1 : shares > R ? R : shares;
-  if (p.prompt && shares < 8) shares = 8;
-  const dim3 join((unsigned)blocks, (unsigned)shares);
-  if (!p.prompt)
-    hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kRows, kTile>), join, dim3(kJoinThreads), 0, s, args);
-  else if constexpr (D <= 128)
-    hipLaunchKernelGGL((attention_kv4_join_kernel<D, T, kPromptRows, kPromptKeys>), join, dim3(kJoinThreads), 0, s, args);
-  UK_RETURN_IF_HIP(hipGetLastError());
-  note_kernel_path(p.prompt ? "attention_kv4:prompt-split" : "attention_kv4:few-rows-split");
+  note_kernel_path(p.prompt ? (p.splits > 1 ? "attention_kv4:prompt-split" : "attention_kv4:prompt")
+                            : (p.splits > 1 ? "attention_kv4:few-rows-split" : "attention_kv4:few-rows"));
   return 0;
 }
 
@@ -1151,9 +1170,7 @@ int launch_split(const AttentionKv4Args& a, hipStream_t s) {
 
 uint64_t attention_kv4_workspace(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int64_t window,
                                  int64_t sinks, int64_t max_kv_len) {
-  const Split p = plan(tokens, batch, heads, kv_heads, dim, window, sinks, max_kv_len);
-  if (p.splits == 1) return 0;
-  return (uint64_t)p.tiles * kv_heads * p.splits * (p.prompt ? kPromptRows : kRows) * (dim + 2) * 4;
+  return plan(tokens, batch, heads, kv_heads, dim, window, sinks, max_kv_len).bytes;
 }
 
 int launch_attention_kv4(const AttentionKv4Args& a, hipStream_t s) {

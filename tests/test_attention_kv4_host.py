@@ -263,3 +263,13 @@ def test_cache_compacts(monkeypatch):
     assert len(copies) == 2 and pool.free_pages() == 5
     assert pool.compact() == 3 and len(copies) == 2
     assert sorted(pool.extend([seqs[1]], [80]).tolist()) == list(range(48, 128))
+
+
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim", [(32768, 32, 8, 128), (131072, 32, 8, 128), (524288, 32, 8, 64),
+                                                       (131072, 16, 4, 256), (1 << 20, 8, 8, 256)])
+def test_long_prompts_ask_for_a_bounded_workspace(tokens, heads, kv_heads, dim):
+    assert 0 < iree_amd.attention_kv4_workspace(tokens, 1, heads, kv_heads, dim, max_kv_len=tokens) <= 256 << 20
+    assert iree_amd.attention_kv4_workspace(tokens, 1, heads, kv_heads, dim, max_kv_len=tokens, window=50000) <= 256 << 20
+    # (one tile of 128 rows of every head, in 64 parts, is more)
+    most = max(256 << 20, kv_heads * 64 * 128 * (dim + 2) * 4)
+    assert iree_amd.attention_kv4_workspace(tokens, 1, heads, kv_heads, dim, max_kv_len=1 << 20) <= most

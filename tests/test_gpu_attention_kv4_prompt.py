@@ -277,3 +277,31 @@ def test_results_are_off_by_their_own_rounding(uk, cuda, dtype, dim, heads, kv_h
     want = want[case.rows].reshape(got.shape)
     step = torch.exp2(torch.frexp(want)[1].double()) * torch.finfo(dtype).eps / 2
     assert float((got - want).square().mean()) < 1.1 * float(step.square().mean()) / 12
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,q_lens", [(64, 16, 128, [2500, 1700]), (64, 16, 256, [1100, 1000])])
+def test_prompts_whose_partial_results_are_many(uk, cuda, heads, kv_heads, dim, q_lens):
+    """More partial results than a call asks memory for: several launches use the same. Rows from all over both
+    sequences, the last row of each among them, against the formula; all rows against the call without memory."""
+    kv_lens = [33000, 20000]
+    case = Case(81, F16, heads, kv_heads, dim, 64, q_lens, kv_lens)
+    nbytes = uk.attention_kv4_workspace(case.tokens, 2, heads, kv_heads, dim, max_kv_len=max(kv_lens))
+    tile = 128 if dim <= 128 else 16      # rows; 33000 keys are split in 3 at least
+    assert (case.tokens * 4 // tile + 2) * kv_heads * 3 * tile * (dim + 2) * 4 > 256 << 20 >= nbytes
+    workspace = torch.full((nbytes,), 0xFF, dtype=torch.uint8, device="cuda")
+    out = case.run(uk, max_kv_len=max(kv_lens), workspace=workspace)
+    assert uk.last_kernel_path() == "attention_kv4:" + ("prompt" if dim <= 128 else "few-rows") + "-split"
+    assert bool((out[~case.rows] == 3).all()) and bool((out[:, heads * dim:] == 3).all())
+    plain = case.run(uk, max_kv_len=max(kv_lens), workspace=workspace[:64])
+    assert "split" not in uk.last_kernel_path()
+    a, b = out[case.rows][:, :heads * dim].double(), plain[case.rows][:, :heads * dim].double()
+    # (each within half a step and what f32 sums of 33000 keys come to)
+    assert bool(((a - b).abs() <= 2.0**-10 * b.abs() + 2.0**-10 * 0.05).all())
+    for s, (q_len, kv_len) in enumerate(zip(q_lens, kv_lens)):
+        token = torch.tensor(sorted({0, 1, 31, 32, q_len // 3, q_len // 2 + 5, q_len - 33, q_len - 1}), device="cuda")
+        rows = case.starts[s] + token
+        q = case.q[rows][:, :heads * dim].reshape(len(token), heads, dim)
+        table = case.table[s:s + 1, :case.wide].expand(len(token), -1)
+        want, bound = kv4ref.attention(q, case.cache, 64, table, list(range(len(token) + 1)),
+                                       [kv_len - q_len + int(t) + 1 for t in token], kv_heads, case.scale(None))
+        kv4ref.assert_near(out[rows][:, :heads * dim].reshape(want.shape), want, bound)
