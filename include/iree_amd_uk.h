@@ -792,7 +792,8 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4(
     void* stream);
 /* Bytes of workspace such a call of these sizes uses on the current device (0: none); at most 256 MiB, or
  * where that is more what one tile of rows takes (128 rows of every kv head): long prompts
- * run in several launches that share it. */
+ * run in several launches that share it. max_kv_len as the call has it, at least 1 and at most the
+ * call's max_pages * page_size, which is what to ask with for a call that passes 0. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4_workspace(
     iree_amd_uk_index_t tokens, iree_amd_uk_index_t batch, int32_t heads, int32_t kv_heads,
     int32_t head_dim, iree_amd_uk_index_t window, iree_amd_uk_index_t sinks,

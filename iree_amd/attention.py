@@ -97,7 +97,8 @@ def kv4_read(cache, pages, page_size, slots, k_out, v_out, rows, kv_heads, head_
 
 
 def attention_kv4_workspace(tokens, batch, heads, kv_heads, head_dim, *, max_kv_len, window=0, sinks=0):
-    """Bytes of workspace that ``attention_kv4`` of these sizes uses (0: none)."""
+    """Bytes of workspace that ``attention_kv4`` of these sizes uses (0: none). ``max_kv_len``: the
+    call's own, or ``max_pages * page_size`` for a call without one."""
     out = C.c_uint64(0)
     _check(load_library().iree_amd_uk_attention_kv4_workspace(
         tokens, batch, heads, kv_heads, head_dim, window, sinks, max_kv_len, C.byref(out)))
@@ -116,15 +117,16 @@ def attention_kv4(q, out, cache, pages, page_size, page_table, q_starts, kv_lens
                   page_table_stride=None, q_stride0=None, out_stride0=None, workspace=None, stream=None):
     """Attention of the query tokens of ``batch`` sequences over the paged 4-bit cache,
     causal, optionally with a sliding window and ``sinks`` first tokens that stay visible.
-    ``max_kv_len``: the longest of ``kv_lens`` as far as the caller knows. Without a
-    ``workspace`` the call takes one from torch's allocator for its own duration."""
+    ``max_kv_len``: the longest of ``kv_lens`` as far as the caller knows (None or 0: as many as the
+    page table holds). Without a ``workspace`` the call takes one from torch's allocator for its own
+    duration."""
     kind, row, device = _row_type(flags), heads * head_dim, _device()
     if page_stride is None:
         page_stride = kv_heads * page_size * (head_dim + 8)
     capacity = max_pages * page_size
-    max_kv_len = capacity if max_kv_len is None else min(max_kv_len, capacity)
+    max_kv_len = min(max_kv_len or capacity, capacity)
     where = _tensor(q, kind, "q", device)
-    if workspace is None:
+    if workspace is None and max_kv_len:
         nbytes = _workspace_bytes(device, tokens, batch, heads, kv_heads, head_dim, window, sinks, max_kv_len)
         if nbytes:
             workspace = _workspace(nbytes, stream)

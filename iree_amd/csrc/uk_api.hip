@@ -1070,9 +1070,12 @@ extern "C" int iree_amd_uk_attention_kv4_workspace(iree_amd_uk_index_t tokens, i
   UK_RETURN_IF_ERROR(validate_rows(what, IREE_AMD_UK_FLAG_ATTENTION_TYPE_F16, 0, kv_heads, head_dim));
   UK_RETURN_IF_ERROR(validate_attention_sizes(what, tokens, batch, heads, kv_heads, window, sinks, max_kv_len));
   if (!out_bytes) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null result", what);
-  *out_bytes = tokens && batch && heads
-                   ? attention_kv4_workspace(tokens, batch, heads, kv_heads, head_dim, window, sinks, max_kv_len)
-                   : 0;
+  *out_bytes = 0;
+  if (tokens == 0 || batch == 0 || heads == 0) return 0;
+  // (the call takes 0 for its page table's capacity, which is not known here)
+  if (max_kv_len == 0)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: max_kv_len 0 (max_pages * page_size for a call that passes 0)", what);
+  *out_bytes = attention_kv4_workspace(tokens, batch, heads, kv_heads, head_dim, window, sinks, max_kv_len);
   return 0;
 }
 

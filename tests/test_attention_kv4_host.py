@@ -273,3 +273,12 @@ def test_long_prompts_ask_for_a_bounded_workspace(tokens, heads, kv_heads, dim):
     # (one tile of 128 rows of every head, in 64 parts, is more)
     most = max(256 << 20, kv_heads * 64 * 128 * (dim + 2) * 4)
     assert iree_amd.attention_kv4_workspace(tokens, 1, heads, kv_heads, dim, max_kv_len=1 << 20) <= most
+
+
+def test_the_workspace_query_refuses_a_length_it_cannot_know():
+    """0 is the page table's capacity for the call; the query, which has no page table, took it for one key."""
+    with pytest.raises(iree_amd.UkError):
+        iree_amd.attention_kv4_workspace(2, 2, 8, 2, 128, max_kv_len=0)
+    assert b"max_kv_len" in iree_amd.load_library().iree_amd_uk_last_error()
+    assert iree_amd.attention_kv4_workspace(2, 2, 8, 2, 128, max_kv_len=1) == 0
+    assert iree_amd.attention_kv4_workspace(0, 2, 8, 2, 128, max_kv_len=0) == 0

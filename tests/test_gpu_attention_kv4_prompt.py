@@ -305,3 +305,12 @@ def test_prompts_whose_partial_results_are_many(uk, cuda, heads, kv_heads, dim, 
         want, bound = kv4ref.attention(q, case.cache, 64, table, list(range(len(token) + 1)),
                                        [kv_len - q_len + int(t) + 1 for t in token], kv_heads, case.scale(None))
         kv4ref.assert_near(out[rows][:, :heads * dim].reshape(want.shape), want, bound)
+
+
+def test_no_idea_of_the_lengths_is_the_capacity(uk, cuda):
+    """0 and None split a long cache alike, with the memory that the call takes for itself."""
+    case = Case(91, F16, 8, 2, 128, 64, [1, 1], [40000, 33])
+    want = case.run(uk)
+    assert uk.last_kernel_path() == "attention_kv4:few-rows-split"
+    assert torch.equal(want, case.run(uk, max_kv_len=0))
+    assert uk.last_kernel_path() == "attention_kv4:few-rows-split"
