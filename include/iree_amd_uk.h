@@ -700,9 +700,9 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_batch_matmul_packed_rhs(
  *   K params  [page_size] pairs of f16, scale and offset of the token's K row
  *   V params  [page_size] pairs of f16 of its V row
  * A code c stands for c * scale + offset. A row x of head_dim values is stored as
- *   offset = f16(min x), scale = f16((max x - min x) / 15)   (saturating at 65504)
+ *   offset = f16(min x), scale = f16(f32((max x - min x) / 15))   (saturating at 65504)
  *   c = clamp(rne((x - offset) / scale), 0, 15), 0 where scale = 0
- * computed without a rounding before the code; a row with a value that is not finite
+ * computed without another rounding before the code; a row with a value that is not finite
  * gets the scale NaN, so that all of it reads as NaN.
  * head_dim is 64, 128 or 256. Page p begins at byte p * page_stride of the cache
  * (a multiple of 16, at least iree_amd_uk_kv4_page_bytes: a pool that holds all
@@ -750,7 +750,7 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_qk_norm_rope(
     void* stream);
 
 /* Rows back out of the cache: k_out[i] and v_out[i] ([rows][kv_heads][head_dim], either
- * may be null) receive what slots[i] holds, rounded once to the rows' type. A row whose
+ * may be null) receive what slots[i] holds, a fused multiply-add in f32 rounded to the rows' type. A row whose
  * slot lies outside the cache is left as it was. Alignment as above. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_kv4_read(
     const void* cache, iree_amd_uk_index_t pages, iree_amd_uk_index_t page_stride,
@@ -768,18 +768,20 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_kv4_read(
  * sequences) lies in [0, pages) (a program that has freed the pages behind its window
  * writes -1), and j < max_pages * page_size, which is at most 2^31 - 4096.
  *   out = sum_j softmax_j(scale * q . k_j) v_j over the visible tokens
- * Scores, the softmax and sums in f32, a key's weight times its scale to 22 bits for rows of f16,
- * rounded to f16 for rows of bf16 (an eighth of the result's own rounding), the result rounded
- * once to the rows' type; zeros where nothing is visible. Rows of q outside
- * [q_starts[0], q_starts[batch]) are neither read nor written. What masked tokens and pages hold, NaN among it, changes nothing.
+ * Scores, the softmax and sums in f32 (finite as long as |scale| times the largest of a row
+ * of q lies below 2^110), a key's weight times its scale to 22 bits for rows of f16, rounded to
+ * f16 for rows of bf16 (an eighth of the result's own rounding), the result rounded once to
+ * the rows' type; zeros where nothing is visible. Rows of q outside
+ * [q_starts[0], q_starts[batch]) are neither read nor written. What masked tokens and pages hold,
+ * NaN among it, changes nothing.
  *   max_kv_len: the longest of kv_lens as far as the caller knows (it sets how the work is
  * split, not what is computed; 0: max_pages * page_size).
  *   workspace: partial results of a long cache that is read by several workgroups, at
  * least what iree_amd_uk_attention_kv4_workspace says, 16-byte aligned; with less, or
- * null, the call runs unsplit: slower, and less exact where more than 65536 keys are visible (their
- * f32 sums are rounded that often: 2.3e-4 of results of f16 on 131072 keys, 4.3e-4 on 524288, where
- * their own rounding is 2.1e-4). The caller's: calls that may overlap, and graphs
- * whose replays may, need one each.
+ * null, the call runs unsplit: slower, and less exact where more than 65536 keys are
+ * visible (their f32 sums are rounded that often: 2.3e-4 of results of f16 on 131072 keys, 4.3e-4
+ * on 524288, where their own rounding is 2.1e-4). The caller's: calls that may overlap, and
+ * graphs whose replays may, need one each.
  * The library's memory is not used and nothing is allocated. Alignment as above. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4(
     const void* q, iree_amd_uk_index_t q_stride0, void* out, iree_amd_uk_index_t out_stride0,
@@ -790,9 +792,9 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4(
     int32_t head_dim, float scale, iree_amd_uk_index_t window, iree_amd_uk_index_t sinks,
     iree_amd_uk_index_t max_kv_len, void* workspace, uint64_t workspace_bytes, uint32_t flags,
     void* stream);
-/* Bytes of workspace such a call of these sizes uses on the current device (0: none); at most 256 MiB, or
- * where that is more what one tile of rows takes (128 rows of every kv head): long prompts
- * run in several launches that share it. max_kv_len as the call has it, at least 1 and at most the
+/* Bytes of workspace such a call of these sizes uses on the current device (0: none); at
+ * most 256 MiB, or where that is more what one tile of rows takes (128 rows of every kv head): long
+ * prompts run in several launches that share it. max_kv_len as the call has it, at least 1 and at most the
  * call's max_pages * page_size, which is what to ask with for a call that passes 0. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_attention_kv4_workspace(
     iree_amd_uk_index_t tokens, iree_amd_uk_index_t batch, int32_t heads, int32_t kv_heads,

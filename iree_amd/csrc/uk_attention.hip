@@ -44,7 +44,7 @@ struct Rows {
 // all before it, and the last sequence that begins at or before a number is the one to have it:
 // 64 lanes look for it at 64 sequences at a time. (Numbers without rows cost more than their own
 // start: workgroups go to the parts of the device in turn, and with every second number empty half of it
-// stays idle: 16 sequences of 128 rows on 16384 keys in four splits, 414 us, so 241.)
+// stays idle: 16 sequences of 128 rows on 16384 keys in four splits, with one f16 a weight, 414 us, so 241.)
 __device__ inline Rows find_rows(const AttentionKv4Args& a, int64_t slot, int G, int R) {
   const int lane = threadIdx.x & 63;
   const int64_t further = slot - a.batch;
@@ -253,8 +253,8 @@ __device__ inline uint32_t pair_bytes(uint32_t first, uint32_t second) {
   return __builtin_amdgcn_perm(second, first, 0x0C040C00u | b | (b << 16));
 }
 // Tiles of a wave in LDS: the one in use and the one on its way. (Three, which leave room for
-// three workgroups on a compute unit instead of four: two caches of 131072 keys 51.2 us, with
-// two 50.4.)
+// three workgroups on a compute unit instead of four: two caches of 131072 keys, with one f16 a
+// weight, 51.2 us, with two tiles 50.4.)
 constexpr int kRing = 2;
 
 // LDS of a workgroup: the waves' rings, later their results; behind them the waves'
@@ -281,9 +281,9 @@ __device__ inline half2v high_codes(uint32_t x, uint32_t bias) {
 // keys), and everything that belongs to a row (its reference, its sums, the factor of its
 // result) is one value of the lane. The waves of a workgroup take key tiles in turn, each
 // with a running softmax of its own; they join through LDS at the end. The next tile is
-// requested before the current one is used. Bound by HBM, with the vector instructions (about 190 a
-// tile of 32 keys and D = 128) not far behind: two caches of 131072 keys, 251 MB, in 45 us (5.6
-// TB/s), 32 of 1000 to 8192 keys, 160 MB, in 36 us (4.5 TB/s), without the join.
+// requested before the current one is used. Bound by HBM, with the vector instructions (about 200 a
+// tile of 32 keys and D = 128) not far behind: two caches of 131072 keys, 251 MB, in 50 us (5.0
+// TB/s), 32 of 1000 to 8192 keys, 160 MB, in 38 us (4.2 TB/s), without the join (rows of bf16 45 and 36).
 template <int D, typename T, bool kPast>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_kv4_split_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
@@ -693,8 +693,9 @@ constexpr int prompt_lds_bytes() { return 2 * PromptLds<D>::kBytes + 64; }
 // before it: v_mfma_f32_32x32x16_f16 with the keys as rows of the scores, as in the kernel for
 // few rows, 32 rows a wave. Two waves fit a vector unit (three with D = 64), and one's softmax (eleven
 // instructions to a score: three for scale and offset, one each for the largest, the sum and the operand, two
-// for the offsets of V, an exponential at a quarter of the rate) has only the other's products beside it: a prompt of
-// 4096 tokens, 32 heads of 128, 137 GFLOP, in 202 us (0.68 PFLOP/s), one of 8192 in 678 (0.81).
+// for the offsets of V, an exponential at a quarter of the rate; one more for the rest of a weight) has only the
+// other's products beside it: a prompt of 4096 tokens, 32 heads of 128, 137 GFLOP, in 240 us (0.57 PFLOP/s; vector
+// unit 59 % of the time, matrix cores 35 %), one of 8192 in 867 (0.63), rows of bf16 in 202 and 678.
 template <int D, typename T>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_kv4_prompt_kernel(SplitArgs args) {
   const AttentionKv4Args& a = args.a;
@@ -1038,8 +1039,8 @@ constexpr uint64_t kMostPartBytes = 256ull << 20;
 // Splits of the prompt kernel: `units` workgroups with `tiles` key tiles each at most. In half
 // microseconds, a key tile costs 7.2 for each two workgroups that share a compute unit and 6 for a
 // last one alone, a workgroup's start about four tiles, the join a little and more with each
-// partial result. (8 sequences of 8192 keys with 128 rows each, 64 units: 8 splits 79 us, 4 splits 110;
-// with 512 rows, 256 units: 2 splits 215 us, none 258.)
+// partial result. (8 sequences of 8192 keys with 128 rows each, 64 units: 8 splits 86 us, 4 splits 125, 16
+// splits 98; with 512 rows, 256 units: 2 splits 245 us, 4 splits 247, none 274.)
 int64_t prompt_splits(int64_t units, int64_t tiles, int64_t cus) {
   int64_t best = 1;
   double least = INFINITY;
@@ -1063,9 +1064,12 @@ Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int6
   };
   auto units_of = [&](int64_t R) { return batch * ceil_div(ceil_div(rows, batch), R) * kv_heads; };
   // Prompts where sequences have a tile's rows on average and there is work for the whole device
-  // (8 sequences of 8192 keys with 128 rows each 80 us, as few rows 94; 4 of 1024 keys with 384 rows
-  // 33, as few rows 23, with 2048 rows 58 and 87). Never with heads of 256, whose tiles leave room for one
-  // wave on a vector unit (2048 rows on 4096 keys 349 us, as few rows 235).
+  // (8 sequences of 8192 keys with 128 rows each 87 us, as few rows 97; 4 of 1024 keys with 384 rows
+  // 34, as few rows 24, with 2048 rows 64 and 87; 4 of 512 with 1024 rows 26 and 33). The device is full
+  // by tiles of the longest, and of one whole prompt half as many work: one of 1024 tokens, which is at the
+  // line, 50 us, as few rows 37, of 1024 on 2048 keys 79 and 70, of 1536 on 2048 keys 82 and 90. Never with heads
+  // of 256, whose tiles leave room for one wave on a vector unit (2048 tokens with 16 + 4 heads on
+  // 4096 keys, with one f16 a weight, 349 us, as few rows 235).
   Split p;
   int64_t units = units_of(kPromptRows), keys = seen(kPromptRows, kPromptKeys);
   p.prompt = dim <= 128 && rows >= kPromptRows * batch &&
@@ -1073,8 +1077,8 @@ Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int6
   if (!p.prompt) units = units_of(kRows), keys = seen(kRows, kTile);
   p.tiles = rows / (p.prompt ? kPromptRows : kRows) + batch;
   // Keys that one tile of rows reads once, and that are too many for the caches to hold until the
-  // next step, go past them: two sequences of 131072 keys 54.8 us through them, 50.4 past them; 72 MB
-  // of windows that a repeated call still finds there 20.8 and 21.4.
+  // next step, go past them: two sequences of 131072 keys 58.8 us through them, 54.4 past them, 32 of 1000 to
+  // 8192 keys 48.6 and 44.5; 72 MB of windows 20.5 and 20.2, which a repeated call still finds there.
   p.past = !p.prompt && tokens <= batch && G <= kRows && (double)batch * keys * kv_heads * (dim + 8) > 128e6;
   const int64_t key_tiles = ceil_div(keys, p.prompt ? kPromptKeys : kTile);
   int64_t splits;
@@ -1082,9 +1086,9 @@ Split plan(int64_t tokens, int64_t batch, int heads, int kv_heads, int dim, int6
     splits = prompt_splits(units, key_tiles, cus);
   } else {
     // Five workgroups to a compute unit, so that lengths that differ even out (32 sequences of
-    // 1000 to 8192 keys: 40.5 us, with four 45.2, with eight 42.9), but no more than 32 splits where
-    // fewer fill the device: the join reads them all (two of 131072 keys: 49.4 us, with 48 splits
-    // 53.0, with 64 52.0). A split has enough tiles to be worth its start and the join, fewer where
+    // 1000 to 8192 keys: 44.5 us, with four 48.6, with eight 47.8), but no more than 32 splits where
+    // fewer fill the device: the join reads them all (two of 131072 keys, rows of bf16: 52.1 us, with 48 splits
+    // 54.9, with 64 54.3; of f16 all 57). A split has enough tiles to be worth its start and the join, fewer where
     // most of the device is idle.
     splits = ceil_div(5 * cus, units);
     if (splits > 32) splits = ceil_div(2 * cus, units) > 32 ? ceil_div(2 * cus, units) : 32;

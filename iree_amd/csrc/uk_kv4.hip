@@ -1,10 +1,12 @@
 // Head norms with position rotation, rows into and out of the 4-bit cache, and copies of
 // its pages (include/iree_amd_uk.h has the formulas and the layout).
 //
-// All four are bound by memory, or for a few tokens by the launch: norms and rotation of 4099 tokens
-// with 32 + 8 heads of 128, 85 MB, in 17.5 us (4.8 TB/s), of one token in 2.5; with values and the
-// cache 8191 tokens, 181 MB, in 46 us (3.9 TB/s: a 4-bit row is written in pieces of 16 and 64
-// bytes), and these rows back out of the cache, 42 MB, in 10.
+// Norms and rotation, rows back out and copies are bound by memory, or for a few tokens by the launch:
+// 4099 tokens with 32 + 8 heads of 128, 85 MB, in 17.5 us (4.8 TB/s), one token in 2.5; 8191 tokens back
+// out of the cache, 42 MB, in 10, of which 6.5 are HBM at a copy's rate and 2.4 what a launch of a few rows
+// takes. Norms with values and the cache are bound by memory and by the vector unit: 8191 tokens, 181 MB
+// (written to the byte what is kept: 76 MB), in 46 us, of HBM 28 and of 16300 vector instructions a
+// vector unit 27, 56 % of which are the stored third of the rows: keys in 64 bits, codes.
 #include "uk_common.h"
 #include "uk_kv4.h"
 

@@ -314,3 +314,14 @@ def test_no_idea_of_the_lengths_is_the_capacity(uk, cuda):
     assert uk.last_kernel_path() == "attention_kv4:few-rows-split"
     assert torch.equal(want, case.run(uk, max_kv_len=0))
     assert uk.last_kernel_path() == "attention_kv4:few-rows-split"
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,q_lens,wide", [(8, 2, [1, 5], 3), (*WIDE, 9)])
+def test_tokens_past_the_page_table_are_not_seen(uk, cuda, heads, kv_heads, q_lens, wide, dim):
+    """Lengths that pass max_pages pages, in the middle of a tile."""
+    case = Case(95, F16, heads, kv_heads, dim, 16, q_lens, [n + 60 for n in q_lens])
+    case.wide = wide
+    for window, sinks in ((0, 0), (33, 5)):
+        case.check(case.run(uk, window=window, sinks=sinks), window=window, sinks=sinks)
+        assert uk.last_kernel_path() == "attention_kv4:" + ("prompt" if wide == 9 else "few-rows")
