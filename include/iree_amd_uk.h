@@ -769,7 +769,7 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_kv4_read(
  * writes -1), and j < max_pages * page_size, which is at most 2^31 - 4096.
  *   out = sum_j softmax_j(scale * q . k_j) v_j over the visible tokens
  * Scores, the softmax and sums in f32 (finite as long as |scale| times the largest of a row
- * of q lies below 2^110), a key's weight times its scale to 22 bits for rows of f16, rounded to
+ * of q lies below 2^96), a key's weight times its scale to 22 bits for rows of f16, rounded to
  * f16 for rows of bf16 (an eighth of the result's own rounding), the result rounded once to
  * the rows' type; zeros where nothing is visible. Rows of q outside
  * [q_starts[0], q_starts[batch]) are neither read nor written. What masked tokens and pages hold,

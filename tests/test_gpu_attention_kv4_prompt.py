@@ -325,3 +325,22 @@ def test_tokens_past_the_page_table_are_not_seen(uk, cuda, heads, kv_heads, q_le
     for window, sinks in ((0, 0), (33, 5)):
         case.check(case.run(uk, window=window, sinks=sinks), window=window, sinks=sinks)
         assert uk.last_kernel_path() == "attention_kv4:" + ("prompt" if wide == 9 else "few-rows")
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,q_lens", [(8, 2, [1, 5]), WIDE])
+def test_scores_of_any_size_are_finite(uk, cuda, heads, kv_heads, q_lens, dim):
+    """Queries of 2^90, or 2^-100: of scores that lie so far apart one key has all of the weight; of scores of 0 all
+    keys have the same. (A weight in f16 is within 2^-11 of itself, of V rows whose 15 scales and offset come to less
+    than 8.)"""
+    case = Case(97, BF16, heads, kv_heads, dim, 32, q_lens, [n + 60 for n in q_lens])
+    case.q.mul_(2.0**88)
+    for _ in range(2):
+        out = case.run(uk)
+        q = case.q[:, :heads * dim].reshape(case.tokens, heads, dim)
+        want, _ = kv4ref.attention(q, case.cache, 32, case.table[:, :case.wide], case.starts, case.kv_lens, kv_heads,
+                                   case.scale(None))
+        got = out[:, :heads * dim].reshape(want.shape)
+        assert bool(torch.isfinite(got[case.rows]).all())
+        kv4ref.assert_near(got, want, torch.full_like(want, 2.0**-11 * 8), rows=case.rows)
+        case.q.mul_(2.0**-95).mul_(2.0**-95)
