@@ -814,6 +814,117 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_copy_pages(void* pool, iree_amd_uk_index_t pa
                                               const int32_t* dst, iree_amd_uk_index_t count,
                                               void* stream);
 
+/*===------------------------------------------------------------------------===
+ * A layer in 8-bit integers and its experts (no reference ukernel): rows of 8 bits
+ * with a scale for each token, their products with packed 8-bit weights that have a
+ * scale for each channel, and the same products over the ragged groups of rows that
+ * the tokens of every expert are.
+ *
+ * A row y of 8 bits is q = rne(127 y / max|y|) and scale = max|y| / 127; zeros, with
+ * scale 0, where all of y is 0. A row with a value that is not finite, or whose largest
+ * size f32 does not hold, gets zeros and the scale NaN: all of it, and of what is
+ * multiplied from it, reads as NaN. q has the bits of the formula in 64 bits
+ * (products of two values of 16 bits are in it as far as f32 holds them).
+ * Rows lie `stride0` elements apart at any alignment of their elements; rows of 8 bits
+ * that the products read, 16-byte aligned and whole 16s apart.
+ *===------------------------------------------------------------------------===*/
+#define IREE_AMD_UK_FLAG_ROWS_TYPE_MASK 0xFF
+#define IREE_AMD_UK_FLAG_ROWS_TYPE_F16 0x01
+#define IREE_AMD_UK_FLAG_ROWS_TYPE_BF16 0x02
+#define IREE_AMD_UK_FLAG_ROWS_TYPE_F32 0x03   /* results of the products, and logits */
+/* moe_route: the weights of a token's experts are divided by their sum. */
+#define IREE_AMD_UK_FLAG_ROUTE_RENORMALIZE 0x100
+/* grouped_matmul_w8a8: rows of the left-hand side, rows of the result by the list. */
+#define IREE_AMD_UK_FLAG_GROUPED_GATHER 0x100
+#define IREE_AMD_UK_FLAG_GROUPED_SCATTER 0x200
+
+/* The residual's addition, RMS norm and 8 bits, in one pass:
+ *   h = T(residual + sum_j w_j x_j),  y = h / sqrt(mean(h^2) + eps) * weight
+ * and y's row of 8 bits. x is [tokens][addends][dim], x_stride0 elements between
+ * tokens and x_stride1 between a token's addends (one where addends = 1); w_j is
+ * addend_weights[token][j] (addend_weights_stride0 apart; null: 1), and an addend whose
+ * weight is 0 changes nothing, whatever it holds: a layer's own output, or those of a
+ * token's experts with their weights. One addend without a weight is added in f32,
+ * others in 64 bits, in order; h is rounded to the rows' type T (F16 or BF16) and written
+ * to sum_out unless that is null. residual and weight may be null (0, and 1). sum_out
+ * may be residual's own buffer, or with one addend x's, with the same stride; other
+ * buffers must not overlap. dim up to 65536. */
+IREE_AMD_UK_EXPORT int iree_amd_uk_rms_norm_quantize(
+    const void* x, iree_amd_uk_index_t x_stride0, iree_amd_uk_index_t x_stride1, int32_t addends,
+    const float* addend_weights, iree_amd_uk_index_t addend_weights_stride0, const void* residual,
+    iree_amd_uk_index_t residual_stride0, void* sum_out, iree_amd_uk_index_t sum_out_stride0,
+    const void* weight, float eps, void* q, iree_amd_uk_index_t q_stride0, float* scale,
+    iree_amd_uk_index_t tokens, iree_amd_uk_index_t dim, uint32_t flags, void* stream);
+
+/* Rows of 8 bits of x ([rows][cols], F16 or BF16), or with up of silu(x) up, x being
+ * the gate: silu(g) = g / (1 + exp(-g)). cols up to 65536. Buffers must not overlap
+ * (x and up may). */
+IREE_AMD_UK_EXPORT int iree_amd_uk_quantize_rows(
+    const void* x, iree_amd_uk_index_t x_stride0, const void* up, iree_amd_uk_index_t up_stride0,
+    void* q, iree_amd_uk_index_t q_stride0, float* scale, iree_amd_uk_index_t rows,
+    iree_amd_uk_index_t cols, uint32_t flags, void* stream);
+
+/* out[m][n] = T((sum_k lhs[m][k] rhs[n][k]) lhs_scale[m] rhs_scale[n] + bias[n])
+ * with exact 32-bit integer sums (K up to 131071), scales and bias in f32, T the type in
+ * the flags (F16, BF16 or F32), rounded once; bias may be null. lhs is row-major, of 8
+ * bits, its rows readable up to K rounded up to 16 (what lies past K does not count). rhs
+ * is packed as iree_amd_uk_pack does for the right-hand side of a matmul, in tiles of
+ * 32 x 16 with padding 0: [N / 32][K / 16][32][16], rhs_stride0 bytes between
+ * outer columns; 16-byte aligned. out is row-major with any alignment of its elements.
+ *   workspace: partial sums of a long K over few tiles, at least what
+ * iree_amd_uk_matmul_w8a8_workspace says, 16-byte aligned; with less, or null, the call
+ * runs unsplit: slower, the same bits. The caller's: calls that may overlap, and graphs
+ * whose replays may, need one each. */
+IREE_AMD_UK_EXPORT int iree_amd_uk_matmul_w8a8(
+    const void* lhs, iree_amd_uk_index_t lhs_stride0, const float* lhs_scale, const void* rhs,
+    iree_amd_uk_index_t rhs_stride0, const float* rhs_scale, const float* bias, void* out,
+    iree_amd_uk_index_t out_stride0, iree_amd_uk_index_t M, iree_amd_uk_index_t N,
+    iree_amd_uk_index_t K, void* workspace, uint64_t workspace_bytes, uint32_t flags, void* stream);
+/* Bytes of workspace such a call uses on the current device (0: none). */
+IREE_AMD_UK_EXPORT int iree_amd_uk_matmul_w8a8_workspace(iree_amd_uk_index_t M, iree_amd_uk_index_t N,
+                                                         iree_amd_uk_index_t K, uint64_t* out_bytes);
+
+/* The top_k experts of each token (top_k up to 64 and `experts`, which is up to 512) by
+ * its logits ([tokens][experts], any ROWS_TYPE, logits_stride0 elements apart), the
+ * largest first, of equal ones the lowest: expert_ids[token][slot], and
+ * expert_weights[token][slot] = exp(l - max) / sum exp(l - max), the sum over all experts
+ * or, with ROUTE_RENORMALIZE, over the chosen ones, in f32. An expert whose logit is
+ * -inf or NaN is not chosen, +inf counts as the largest f32; a slot that no expert is left
+ * for has id -1 and weight 0 (all slots of a token whose logits are all -inf: padding).
+ * The slots, numbered token * top_k + slot, in the order of their experts and within an
+ * expert in their own: rows[tokens * top_k], those of expert e at [offsets[e],
+ * offsets[e + 1]), and -1 from offsets[experts] on. The same lists on every call.
+ * tokens * top_k lies below 2^31.
+ *   workspace: at least what iree_amd_uk_moe_route_workspace says, 16-byte aligned, as
+ * above; without it one workgroup does all. */
+IREE_AMD_UK_EXPORT int iree_amd_uk_moe_route(
+    const void* logits, iree_amd_uk_index_t logits_stride0, int32_t* expert_ids,
+    float* expert_weights, int32_t* offsets, int32_t* rows, iree_amd_uk_index_t tokens,
+    int32_t experts, int32_t top_k, void* workspace, uint64_t workspace_bytes, uint32_t flags,
+    void* stream);
+IREE_AMD_UK_EXPORT int iree_amd_uk_moe_route_workspace(iree_amd_uk_index_t tokens, int32_t experts,
+                                                       uint64_t* out_bytes);
+
+/* The product of matmul_w8a8 (without a bias) by expert: positions [offsets[e],
+ * offsets[e + 1]) of a list of `positions` (offsets, on the device, does not fall; what it says
+ * outside the list is not used) are multiplied with the weights of expert e, at
+ * rhs + e * rhs_expert_stride bytes, with rhs_scale[e][N]. Position p has
+ *   the row p of lhs, or with GROUPED_GATHER the row rows[p] / rows_per_token, and
+ *   the row p of out, or with GROUPED_SCATTER the row rows[p]:
+ * the tokens of moe_route's slots for the experts' first product (GATHER), and their
+ * slots for the second one (SCATTER), whose rows rms_norm_quantize adds up with the
+ * slots' weights. A position whose row lies outside [0, lhs_rows) or [0, out_rows) is
+ * left out; of two that scatter to one row, either may leave each part of it. Rows of out
+ * that no position has stay as they were. experts up to 512; with GATHER, lhs_rows *
+ * lhs_stride0 lies below 2^32. */
+IREE_AMD_UK_EXPORT int iree_amd_uk_grouped_matmul_w8a8(
+    const void* lhs, iree_amd_uk_index_t lhs_stride0, iree_amd_uk_index_t lhs_rows,
+    const float* lhs_scale, const void* rhs, iree_amd_uk_index_t rhs_stride0,
+    iree_amd_uk_index_t rhs_expert_stride, const float* rhs_scale, void* out,
+    iree_amd_uk_index_t out_stride0, iree_amd_uk_index_t out_rows, const int32_t* offsets,
+    const int32_t* rows, int32_t rows_per_token, iree_amd_uk_index_t positions, int32_t experts,
+    iree_amd_uk_index_t N, iree_amd_uk_index_t K, uint32_t flags, void* stream);
+
 /* buf[i] *= scale over n f32 elements, in place (applies the product of the
  * per-tensor scales to an fp8 matmul result). */
 IREE_AMD_UK_EXPORT int iree_amd_uk_scale_f32(void* buf_f32, iree_amd_uk_index_t n,
@@ -878,14 +989,15 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_release_scratch(void);
 /* Human-readable text of the calling thread's last non-OK status ("" if none). */
 IREE_AMD_UK_EXPORT const char* iree_amd_uk_last_error(void);
 /* Name of the kernel family that served the calling thread's last mmt4d (its
- * batch and fused forms included, the SiLU one aside), dequant_matmul_i4 or attention_kv4 call:
+ * batch and fused forms included, the SiLU one aside), dequant_matmul_i4, attention_kv4 or
+ * (grouped_)matmul_w8a8 call:
  * "mmt4d:mfma", "mmt4d:mfma-narrow", "mmt4d:mfma-one-launch"
  * (iree_amd_uk_matmul_data_tiled), "mmt4d:mfma-widened-s4",
  * "mmt4d:mfma-s16-planes", "mmt4d:element-wise", "dequant_i4:mfma",
  * "dequant_i4:gemv", "dequant_i4:gemm", "dequant_i4:reassociated",
  * "dequant_i4:reassociated-element-wise", "dequant_i4:element-wise",
  * "attention_kv4:few-rows", "attention_kv4:prompt", each with "-split" behind it when the
- * caches were split over workgroups ("" before the first call). A static string. No counterpart in the reference, whose
+ * caches were split over workgroups, "w8a8:few-rows", "w8a8:mfma", "w8a8:mfma-split" ("" before the first call). A static string. No counterpart in the reference, whose
  * tile-function choice is visible through iree_uk_mmt4d_info only. */
 IREE_AMD_UK_EXPORT const char* iree_amd_uk_last_kernel_path(void);
 /* Rows and columns of the macro tile of the calling thread's last "mmt4d:mfma"

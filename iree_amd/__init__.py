@@ -48,3 +48,12 @@ from .ukernel import (  # noqa: F401
     silu_mul_quantize_tiled,
     unpack,
 )
+from .w8a8 import (  # noqa: F401
+    grouped_matmul_w8a8,
+    matmul_w8a8,
+    matmul_w8a8_workspace,
+    moe_route,
+    moe_route_workspace,
+    quantize_rows,
+    rms_norm_quantize,
+)

@@ -169,6 +169,22 @@ def _declare(lib):
     lib.iree_amd_uk_attention_kv4_workspace.argtypes = [i64, i64, i32, i32, i32, i64, i64, i64, C.POINTER(u64)]
     lib.iree_amd_uk_copy_pages.restype = C.c_int
     lib.iree_amd_uk_copy_pages.argtypes = [vp, i64, i64, i64, vp, vp, i64, vp]
+    lib.iree_amd_uk_rms_norm_quantize.restype = C.c_int
+    lib.iree_amd_uk_rms_norm_quantize.argtypes = [vp, i64, i64, i32, vp, i64, vp, i64, vp, i64, vp, C.c_float, vp, i64, vp,
+                                                  i64, i64, u32, vp]
+    lib.iree_amd_uk_quantize_rows.restype = C.c_int
+    lib.iree_amd_uk_quantize_rows.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i64, u32, vp]
+    lib.iree_amd_uk_matmul_w8a8.restype = C.c_int
+    lib.iree_amd_uk_matmul_w8a8.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, i64, i64, i64, i64, vp, C.c_uint64, u32, vp]
+    lib.iree_amd_uk_matmul_w8a8_workspace.restype = C.c_int
+    lib.iree_amd_uk_matmul_w8a8_workspace.argtypes = [i64, i64, i64, C.POINTER(C.c_uint64)]
+    lib.iree_amd_uk_moe_route.restype = C.c_int
+    lib.iree_amd_uk_moe_route.argtypes = [vp, i64, vp, vp, vp, vp, i64, i32, i32, vp, C.c_uint64, u32, vp]
+    lib.iree_amd_uk_moe_route_workspace.restype = C.c_int
+    lib.iree_amd_uk_moe_route_workspace.argtypes = [i64, i32, C.POINTER(C.c_uint64)]
+    lib.iree_amd_uk_grouped_matmul_w8a8.restype = C.c_int
+    lib.iree_amd_uk_grouped_matmul_w8a8.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, vp, i64, i64, vp, vp, i32, i64, i32,
+                                                    i64, i64, u32, vp]
     lib.iree_amd_uk_scale_f32.restype = C.c_int
     lib.iree_amd_uk_scale_f32.argtypes = [vp, i64, C.c_float, vp]
     lib.iree_amd_uk_mfma_probe.restype = C.c_int

@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include "uk_common.h"
+#include "uk_w8a8.h"
 
 namespace uk {
 
@@ -1110,6 +1111,246 @@ extern "C" int iree_amd_uk_copy_pages(void* pool, iree_amd_uk_index_t pages, ire
   if (page_bytes == 0) return 0;
   if (!pool || !aligned16(pool)) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: the pool is null or not 16-byte aligned", what);
   return launch_copy_pages(pool, page_bytes, page_stride, src, dst, count, (hipStream_t)stream);
+}
+
+// ---------------------------------------------------------------------------
+// A layer in 8-bit integers and its experts
+// ---------------------------------------------------------------------------
+
+// The flag word: a type up to `last_type` and the bits of `known`.
+static int validate_rows8_flags(const char* what, uint32_t flags, uint32_t known, uint32_t last_type) {
+  const uint32_t type = flags & IREE_AMD_UK_FLAG_ROWS_TYPE_MASK;
+  if (flags & ~(known | IREE_AMD_UK_FLAG_ROWS_TYPE_MASK))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: unknown flag bits 0x%x", what,
+                flags & ~(known | IREE_AMD_UK_FLAG_ROWS_TYPE_MASK));
+  if (type < IREE_AMD_UK_FLAG_ROWS_TYPE_F16 || type > last_type)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: unknown type 0x%x", what, type);
+  return 0;
+}
+
+// Rows of `width` elements of `size` bytes each, `stride` elements apart.
+static int validate_matrix(const char* what, const char* name, const void* p, int64_t stride, int64_t rows, int64_t width,
+                           int64_t size) {
+  if (!p || (uintptr_t)p % size) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null or misaligned %s", what, name);
+  if (stride < 0 || (rows > 1 && stride < width))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: %s stride below a row", what, name);
+  if (rows > 1 && stride > (INT64_MAX >> 4) / rows)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: %s stride too large", what, name);
+  return 0;
+}
+
+// f32 or int32 values; `p` may be null where `optional`.
+static int validate_words(const char* what, const char* name, const void* p, bool optional = false) {
+  if ((!p && !optional) || (uintptr_t)p % 4)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null or misaligned %s", what, name);
+  return 0;
+}
+
+static int validate_workspace(const char* what, const void* workspace, uint64_t bytes) {
+  if (bytes && (!workspace || !aligned16(workspace)))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: the workspace is null or not 16-byte aligned", what);
+  return 0;
+}
+
+constexpr int64_t kMostRowElements = 65536;
+
+extern "C" int iree_amd_uk_rms_norm_quantize(
+    const void* x, iree_amd_uk_index_t x_stride0, iree_amd_uk_index_t x_stride1, int32_t addends,
+    const float* addend_weights, iree_amd_uk_index_t addend_weights_stride0, const void* residual,
+    iree_amd_uk_index_t residual_stride0, void* sum_out, iree_amd_uk_index_t sum_out_stride0, const void* weight, float eps,
+    void* q, iree_amd_uk_index_t q_stride0, float* scale, iree_amd_uk_index_t tokens, iree_amd_uk_index_t dim,
+    uint32_t flags, void* stream) {
+  const char* what = "rms_norm_quantize";
+  UK_RETURN_IF_ERROR(validate_rows8_flags(what, flags, 0, IREE_AMD_UK_FLAG_ROWS_TYPE_BF16));
+  if (tokens < 0 || tokens > 0x7FFFFFFF || dim < 0 || addends < 1 || addends > 1024)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: tokens outside [0, 2^31), addends outside [1, 1024] or negative dim",
+                what);
+  if (dim > kMostRowElements)
+    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: dim above %lld", what, (long long)kMostRowElements);
+  if (!(eps >= 0.f)) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: eps is not at least 0", what);
+  if (tokens == 0 || dim == 0) return 0;
+  // (a token's addends, then the tokens)
+  if (addends > 1 && (x_stride1 < dim || x_stride1 > (INT64_MAX >> 16)))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: x_stride1 below a row or too large", what);
+  if (addends == 1) x_stride1 = 0;
+  UK_RETURN_IF_ERROR(validate_matrix(what, "x", x, x_stride0, tokens, (addends - 1) * x_stride1 + dim, 2));
+  if (residual) UK_RETURN_IF_ERROR(validate_matrix(what, "residual", residual, residual_stride0, tokens, dim, 2));
+  if (sum_out) UK_RETURN_IF_ERROR(validate_matrix(what, "sum_out", sum_out, sum_out_stride0, tokens, dim, 2));
+  UK_RETURN_IF_ERROR(validate_matrix(what, "q", q, q_stride0, tokens, dim, 1));
+  UK_RETURN_IF_ERROR(validate_words(what, "scale", scale));
+  if (addend_weights)
+    UK_RETURN_IF_ERROR(validate_matrix(what, "addend_weights", addend_weights, addend_weights_stride0, tokens, addends, 4));
+  if ((uintptr_t)weight % 2) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: misaligned weight", what);
+  if (sum_out && tokens > 1 &&
+      ((sum_out == residual && sum_out_stride0 != residual_stride0) || (sum_out == x && sum_out_stride0 != x_stride0)))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: in place with another stride", what);
+  if (sum_out && sum_out == x && addends > 1)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: in place of several addends", what);
+  RmsNormQuantizeArgs a{};
+  a.x = x, a.x_stride0 = x_stride0, a.x_stride1 = x_stride1, a.addends = addends;
+  a.factors = addend_weights, a.factors_stride = addend_weights_stride0;
+  a.residual = residual, a.residual_stride = residual_stride0, a.sum_out = sum_out, a.sum_out_stride = sum_out_stride0;
+  a.weight = weight, a.eps = eps, a.q = q, a.q_stride = q_stride0, a.scale = scale;
+  a.tokens = tokens, a.dim = (int)dim;
+  a.bf16 = (flags & IREE_AMD_UK_FLAG_ROWS_TYPE_MASK) == IREE_AMD_UK_FLAG_ROWS_TYPE_BF16;
+  return launch_rms_norm_quantize(a, (hipStream_t)stream);
+}
+
+extern "C" int iree_amd_uk_quantize_rows(const void* x, iree_amd_uk_index_t x_stride0, const void* up,
+                                         iree_amd_uk_index_t up_stride0, void* q, iree_amd_uk_index_t q_stride0,
+                                         float* scale, iree_amd_uk_index_t rows, iree_amd_uk_index_t cols, uint32_t flags,
+                                         void* stream) {
+  const char* what = "quantize_rows";
+  UK_RETURN_IF_ERROR(validate_rows8_flags(what, flags, 0, IREE_AMD_UK_FLAG_ROWS_TYPE_BF16));
+  if (rows < 0 || rows > 0x7FFFFFFF || cols < 0)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: rows outside [0, 2^31) or negative cols", what);
+  if (cols > kMostRowElements)
+    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: cols above %lld", what, (long long)kMostRowElements);
+  if (rows == 0 || cols == 0) return 0;
+  UK_RETURN_IF_ERROR(validate_matrix(what, "x", x, x_stride0, rows, cols, 2));
+  if (up) UK_RETURN_IF_ERROR(validate_matrix(what, "up", up, up_stride0, rows, cols, 2));
+  UK_RETURN_IF_ERROR(validate_matrix(what, "q", q, q_stride0, rows, cols, 1));
+  UK_RETURN_IF_ERROR(validate_words(what, "scale", scale));
+  QuantizeRowsArgs a{};
+  a.x = x, a.x_stride = x_stride0, a.up = up, a.up_stride = up_stride0, a.q = q, a.q_stride = q_stride0, a.scale = scale;
+  a.rows = rows, a.cols = (int)cols;
+  a.bf16 = (flags & IREE_AMD_UK_FLAG_ROWS_TYPE_MASK) == IREE_AMD_UK_FLAG_ROWS_TYPE_BF16;
+  return launch_quantize_rows(a, (hipStream_t)stream);
+}
+
+extern "C" int iree_amd_uk_moe_route(const void* logits, iree_amd_uk_index_t logits_stride0, int32_t* expert_ids,
+                                     float* expert_weights, int32_t* offsets, int32_t* rows, iree_amd_uk_index_t tokens,
+                                     int32_t experts, int32_t top_k, void* workspace, uint64_t workspace_bytes,
+                                     uint32_t flags, void* stream) {
+  const char* what = "moe_route";
+  UK_RETURN_IF_ERROR(
+      validate_rows8_flags(what, flags, IREE_AMD_UK_FLAG_ROUTE_RENORMALIZE, IREE_AMD_UK_FLAG_ROWS_TYPE_F32));
+  if (tokens < 0 || experts < 1 || top_k < 1 || top_k > experts || tokens > 0x7FFFFFFF / top_k)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT,
+                "%s: negative tokens, top_k outside [1, experts] or tokens * top_k not below 2^31", what);
+  if (experts > 512 || top_k > 64)
+    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: more than 512 experts or 64 of a token", what);
+  UK_RETURN_IF_ERROR(validate_words(what, "offsets", offsets));
+  UK_RETURN_IF_ERROR(validate_workspace(what, workspace, workspace_bytes));
+  MoeRouteArgs a{};
+  a.type = (int)(flags & IREE_AMD_UK_FLAG_ROWS_TYPE_MASK);
+  if (tokens > 0) {
+    UK_RETURN_IF_ERROR(validate_matrix(what, "logits", logits, logits_stride0, tokens, experts, a.type == 3 ? 4 : 2));
+    UK_RETURN_IF_ERROR(validate_words(what, "expert_ids", expert_ids));
+    UK_RETURN_IF_ERROR(validate_words(what, "expert_weights", expert_weights));
+    UK_RETURN_IF_ERROR(validate_words(what, "rows", rows));
+  }
+  a.logits = logits, a.logits_stride = logits_stride0, a.expert_ids = expert_ids, a.expert_weights = expert_weights;
+  a.offsets = offsets, a.rows = rows, a.tokens = tokens, a.experts = experts, a.top_k = top_k;
+  a.renormalize = (flags & IREE_AMD_UK_FLAG_ROUTE_RENORMALIZE) != 0;
+  a.workspace = workspace, a.workspace_bytes = workspace ? workspace_bytes : 0;
+  return launch_moe_route(a, (hipStream_t)stream);
+}
+
+extern "C" int iree_amd_uk_moe_route_workspace(iree_amd_uk_index_t tokens, int32_t experts, uint64_t* out_bytes) {
+  const char* what = "moe_route_workspace";
+  if (!out_bytes) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null result", what);
+  *out_bytes = 0;
+  if (tokens < 0 || tokens > 0x7FFFFFFF || experts < 1 || experts > 512)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: tokens outside [0, 2^31) or experts outside [1, 512]", what);
+  *out_bytes = moe_route_workspace(tokens, experts);
+  return 0;
+}
+
+// What the two products share: sizes, rows of 8 bits, packed weights of `experts`, the result.
+static int validate_w8a8(const char* what, const W8A8Args& a, int64_t N, int64_t K) {
+  if (N < 0 || N > (1 << 24) || K < 0)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: N outside [0, 2^24] or negative K", what);
+  if (K > 131071) return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: K above 131071", what);
+  return 0;
+}
+static int validate_w8a8_buffers(const char* what, const W8A8Args& a) {
+  const int64_t wide = ceil_div((int64_t)a.K, (int64_t)16) * 16;
+  UK_RETURN_IF_ERROR(validate_matrix(what, "lhs", a.lhs, a.lhs_stride, a.lhs_rows, wide, 16));
+  if (a.lhs_rows > 1 && a.lhs_stride % 16)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: rows of lhs must be whole 16 bytes apart", what);
+  if (a.lhs_rows > 1 && a.lhs_stride > (1 << 22))
+    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: rows of lhs more than 4 MiB apart", what);
+  const int64_t outer = ceil_div((int64_t)a.N, (int64_t)32);
+  if (!a.rhs || !aligned16(a.rhs) || a.rhs_stride % 16 || a.rhs_stride < 0 || (outer > 1 && a.rhs_stride < wide * 32) ||
+      a.rhs_stride > (1 << 24))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT,
+                "%s: rhs must be 16-byte aligned, its outer columns whole 16 bytes and at least their own size apart, at "
+                "most 16 MiB", what);
+  UK_RETURN_IF_ERROR(validate_words(what, "lhs_scale", a.lhs_scale));
+  UK_RETURN_IF_ERROR(validate_words(what, "rhs_scale", a.rhs_scale));
+  UK_RETURN_IF_ERROR(validate_words(what, "bias", a.bias, true));
+  return validate_matrix(what, "out", a.out, a.out_stride, a.out_rows, a.N, a.type == 3 ? 4 : 2);
+}
+
+extern "C" int iree_amd_uk_matmul_w8a8(const void* lhs, iree_amd_uk_index_t lhs_stride0, const float* lhs_scale,
+                                       const void* rhs, iree_amd_uk_index_t rhs_stride0, const float* rhs_scale,
+                                       const float* bias, void* out, iree_amd_uk_index_t out_stride0,
+                                       iree_amd_uk_index_t M, iree_amd_uk_index_t N, iree_amd_uk_index_t K,
+                                       void* workspace, uint64_t workspace_bytes, uint32_t flags, void* stream) {
+  const char* what = "matmul_w8a8";
+  UK_RETURN_IF_ERROR(validate_rows8_flags(what, flags, 0, IREE_AMD_UK_FLAG_ROWS_TYPE_F32));
+  W8A8Args a{};
+  if (M < 0 || M > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: M outside [0, 2^31)", what);
+  UK_RETURN_IF_ERROR(validate_w8a8(what, a, N, K));
+  UK_RETURN_IF_ERROR(validate_workspace(what, workspace, workspace_bytes));
+  if (M == 0 || N == 0) return 0;
+  a.lhs = (const char*)lhs, a.lhs_stride = lhs_stride0, a.lhs_rows = M, a.lhs_scale = lhs_scale;
+  a.rhs = (const char*)rhs, a.rhs_stride = rhs_stride0, a.rhs_scale = rhs_scale, a.bias = bias;
+  a.out = (char*)out, a.out_stride = out_stride0, a.out_rows = M, a.positions = M, a.rows_per_token = 1;
+  a.experts = 1, a.N = (int)N, a.K = (int)K, a.type = (int)(flags & IREE_AMD_UK_FLAG_ROWS_TYPE_MASK);
+  a.workspace = workspace, a.workspace_bytes = workspace ? workspace_bytes : 0;
+  UK_RETURN_IF_ERROR(validate_w8a8_buffers(what, a));
+  return launch_w8a8(a, (hipStream_t)stream);
+}
+
+extern "C" int iree_amd_uk_matmul_w8a8_workspace(iree_amd_uk_index_t M, iree_amd_uk_index_t N, iree_amd_uk_index_t K,
+                                                 uint64_t* out_bytes) {
+  const char* what = "matmul_w8a8_workspace";
+  if (!out_bytes) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null result", what);
+  *out_bytes = 0;
+  if (M < 0 || M > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: M outside [0, 2^31)", what);
+  UK_RETURN_IF_ERROR(validate_w8a8(what, W8A8Args{}, N, K));
+  if (M && N && K) *out_bytes = w8a8_workspace(M, N, K);
+  return 0;
+}
+
+extern "C" int iree_amd_uk_grouped_matmul_w8a8(
+    const void* lhs, iree_amd_uk_index_t lhs_stride0, iree_amd_uk_index_t lhs_rows, const float* lhs_scale, const void* rhs,
+    iree_amd_uk_index_t rhs_stride0, iree_amd_uk_index_t rhs_expert_stride, const float* rhs_scale, void* out,
+    iree_amd_uk_index_t out_stride0, iree_amd_uk_index_t out_rows, const int32_t* offsets, const int32_t* rows,
+    int32_t rows_per_token, iree_amd_uk_index_t positions, int32_t experts, iree_amd_uk_index_t N, iree_amd_uk_index_t K,
+    uint32_t flags, void* stream) {
+  const char* what = "grouped_matmul_w8a8";
+  UK_RETURN_IF_ERROR(validate_rows8_flags(what, flags, IREE_AMD_UK_FLAG_GROUPED_GATHER | IREE_AMD_UK_FLAG_GROUPED_SCATTER,
+                                          IREE_AMD_UK_FLAG_ROWS_TYPE_F32));
+  W8A8Args a{};
+  UK_RETURN_IF_ERROR(validate_w8a8(what, a, N, K));
+  if (lhs_rows < 0 || lhs_rows > 0x7FFFFFFF || out_rows < 0 || out_rows > 0x7FFFFFFF || positions < 0 ||
+      positions > 0x7FFFFFFF || experts < 0)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: rows, positions or experts outside [0, 2^31)", what);
+  if (experts > 512) return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: more than 512 experts", what);
+  a.gather = (flags & IREE_AMD_UK_FLAG_GROUPED_GATHER) != 0;
+  a.scatter = (flags & IREE_AMD_UK_FLAG_GROUPED_SCATTER) != 0;
+  if (a.gather && rows_per_token < 1)
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: rows_per_token below 1", what);
+  if (lhs_rows == 0 || out_rows == 0 || positions == 0 || experts == 0 || N == 0) return 0;
+  a.lhs = (const char*)lhs, a.lhs_stride = lhs_stride0, a.lhs_rows = lhs_rows, a.lhs_scale = lhs_scale;
+  a.rhs = (const char*)rhs, a.rhs_stride = rhs_stride0, a.rhs_expert = rhs_expert_stride, a.rhs_scale = rhs_scale;
+  a.out = (char*)out, a.out_stride = out_stride0, a.out_rows = out_rows;
+  a.offsets = offsets, a.rows = rows, a.rows_per_token = rows_per_token, a.positions = positions;
+  a.experts = experts, a.N = (int)N, a.K = (int)K, a.type = (int)(flags & IREE_AMD_UK_FLAG_ROWS_TYPE_MASK);
+  UK_RETURN_IF_ERROR(validate_w8a8_buffers(what, a));
+  UK_RETURN_IF_ERROR(validate_words(what, "offsets", offsets));
+  UK_RETURN_IF_ERROR(validate_words(what, "rows", rows, !a.gather && !a.scatter));
+  const int64_t wide = ceil_div(K, (int64_t)16) * 16, outer = ceil_div(N, (int64_t)32);
+  if (experts > 1 && (rhs_expert_stride % 16 || rhs_expert_stride < (outer - 1) * rhs_stride0 + wide * 32 ||
+                      rhs_expert_stride > (INT64_MAX >> 1) / experts))
+    return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT,
+                "%s: the experts' weights must lie whole 16 bytes and at least their own size apart", what);
+  if (a.gather && lhs_rows > 1 && lhs_rows * lhs_stride0 >= 0xFFFFFFF0ll)
+    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: rows to gather from 4 GiB or more", what);
+  return launch_w8a8(a, (hipStream_t)stream);
 }
 
 extern "C" int iree_amd_uk_scale_f32(void* buf_f32, iree_amd_uk_index_t n, float scale,

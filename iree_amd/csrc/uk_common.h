@@ -323,6 +323,53 @@ uint64_t attention_kv4_workspace(int64_t tokens, int64_t batch, int heads, int k
                                  int64_t sinks, int64_t max_kv_len);
 int launch_copy_pages(void* pool, int64_t page_bytes, int64_t page_stride, const int32_t* src, const int32_t* dst,
                       int64_t count, hipStream_t s);
+// Rows of 8 bits (uk_rows8.hip) and the experts of tokens (uk_route.hip).
+struct RmsNormQuantizeArgs {
+  const void* x;
+  int64_t x_stride0, x_stride1;      // elements between tokens, between a token's addends
+  int addends;
+  const float* factors;              // of the addends, or null
+  int64_t factors_stride;
+  const void* residual;
+  int64_t residual_stride;
+  void* sum_out;
+  int64_t sum_out_stride;
+  const void* weight;
+  float eps;
+  void* q;
+  int64_t q_stride;
+  float* scale;
+  int64_t tokens;
+  int dim;
+  bool bf16;
+};
+int launch_rms_norm_quantize(const RmsNormQuantizeArgs& a, hipStream_t s);
+struct QuantizeRowsArgs {
+  const void *x, *up;                // up null: rows as they are
+  int64_t x_stride, up_stride;
+  void* q;
+  int64_t q_stride;
+  float* scale;
+  int64_t rows;
+  int cols;
+  bool bf16;
+};
+int launch_quantize_rows(const QuantizeRowsArgs& a, hipStream_t s);
+struct MoeRouteArgs {
+  const void* logits;
+  int64_t logits_stride;             // elements
+  int32_t* expert_ids;
+  float* expert_weights;
+  int32_t *offsets, *rows;
+  int64_t tokens;
+  int experts, top_k;
+  int type;                          // of the logits: 1 f16, 2 bf16, 3 f32
+  bool renormalize;
+  void* workspace;
+  uint64_t workspace_bytes;
+};
+int launch_moe_route(const MoeRouteArgs& a, hipStream_t s);
+uint64_t moe_route_workspace(int64_t tokens, int experts);
 int launch_scale_f32(void* buf, int64_t n, float scale, hipStream_t s);
 int launch_mfma_probe(uint32_t type_flag, const void* operands, int64_t iters, void* sink,
                       int64_t* out_ops_per_launch, hipStream_t s);

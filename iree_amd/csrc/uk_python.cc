@@ -113,6 +113,11 @@ PyMethodDef g_entries[] = {
     UK_ENTRY(iree_amd_uk_kv4_read),
     UK_ENTRY(iree_amd_uk_attention_kv4),
     UK_ENTRY(iree_amd_uk_copy_pages),
+    UK_ENTRY(iree_amd_uk_rms_norm_quantize),
+    UK_ENTRY(iree_amd_uk_quantize_rows),
+    UK_ENTRY(iree_amd_uk_matmul_w8a8),
+    UK_ENTRY(iree_amd_uk_moe_route),
+    UK_ENTRY(iree_amd_uk_grouped_matmul_w8a8),
     {"iree_amd_uk_query_matmul_tile_sizes", (PyCFunction)(void (*)(void))query, METH_FASTCALL, nullptr},
 };
 

@@ -1,0 +1,296 @@
+// Each token's experts and their weights from its logits, and the tokens' slots in the order of
+// their experts (include/iree_amd_uk.h).
+//
+// A wave chooses for a token: its lanes hold the logits, and top_k times the largest of all lanes is
+// taken, as one 64-bit key of the value and, below it, the number of the expert counted down, so that
+// of equal values the lowest expert wins. The slots are then sorted by expert the way one digit of
+// a radix sort is: blocks of consecutive tokens count their slots of every expert, and a slot's place
+// is its expert's first place, plus the counts of the blocks and waves before, plus the lanes before it
+// with the same expert. The order of no addition decides anything: the lists are the same on every call.
+//
+// Up to 128 tokens one workgroup does all; more take two launches, the counts of the blocks in the
+// workspace between them.
+#include "uk_common.h"
+#include "uk_kv4.h"
+
+#include <type_traits>
+
+namespace uk {
+namespace {
+using namespace kv4;
+
+constexpr int kMostExperts = 512;
+constexpr int kMostBlocks = 256;           // blocks of tokens
+constexpr int kBlockTokens = 64;           // of one, at least
+constexpr int kOneBlockTokens = 128;       // up to which one workgroup does all
+
+struct RouteArgs {
+  MoeRouteArgs r;
+  int block_tokens, blocks;
+  int32_t* counts;                         // [blocks][experts]
+};
+
+// Order of floats as that of integers; 0 for what is not chosen.
+__device__ inline uint32_t order_of(float v) {
+  if (!(v > -__builtin_inff())) return 0;                   // (-inf and NaN)
+  v = fminf(v, 3.4028234663852886e38f) + 0.f;               // (+inf counts as the largest; -0 is 0)
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ inline float value_of(uint32_t order) {
+  return __builtin_bit_cast(float, order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
+}
+
+template <typename T>
+__device__ inline float logit(const void* row, int e) {
+  if constexpr (std::is_same<T, float>::value) return ((const float*)row)[e];
+  else return T::widen(((const uint16_t*)row)[e]);
+}
+
+// The experts and weights of one token, by a wave. kLogits: a lane's.
+template <typename T, int kLogits>
+__device__ inline void choose(const MoeRouteArgs& a, int64_t token) {
+  const int lane = threadIdx.x & 63;
+  const char* row = (const char*)a.logits + token * a.logits_stride * (int64_t)(std::is_same<T, float>::value ? 4 : 2);
+  uint32_t order[kLogits];
+#pragma unroll
+  for (int i = 0; i < kLogits; ++i) {
+    const int e = i * 64 + lane;
+    order[i] = e < a.experts ? order_of(logit<T>(row, e)) : 0;
+  }
+  // The best of a lane's own is kept until it is taken.
+  float top = 0.f, total = 0.f;
+  uint32_t mine_order = 0;
+  int mine = -1;
+  for (int k = 0; k < a.top_k; ++k) {
+    uint32_t best = 0;
+    int best_i = 0;
+#pragma unroll
+    for (int i = 0; i < kLogits; ++i)
+      if (order[i] > best) best = order[i], best_i = i;
+    uint64_t key = best ? (uint64_t)best << 32 | (uint32_t)~(best_i * 64 + lane) : 0;
+#pragma unroll
+    for (int mask = 32; mask; mask >>= 1) {
+      const uint64_t there = (uint64_t)__shfl_xor((uint32_t)(key >> 32), mask) << 32 | __shfl_xor((uint32_t)key, mask);
+      key = there > key ? there : key;
+    }
+    const int e = key ? (int)~(uint32_t)key : -1;
+    const uint32_t chosen = (uint32_t)(key >> 32);
+    if (k == 0) {
+      top = key ? value_of(chosen) : 0.f;
+      if (!a.renormalize) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kLogits; ++i)
+          if (order[i]) sum += expf(value_of(order[i]) - top);
+#pragma unroll
+        for (int mask = 32; mask; mask >>= 1) sum += __shfl_xor(sum, mask);
+        total = sum;
+      }
+    }
+    if (e >= 0) {
+      if (a.renormalize) total += expf(value_of(chosen) - top);
+#pragma unroll
+      for (int i = 0; i < kLogits; ++i)
+        if (e == i * 64 + lane) order[i] = 0;
+    }
+    if (lane == k) mine = e, mine_order = chosen;
+  }
+  if (lane < a.top_k) {
+    a.expert_ids[token * a.top_k + lane] = mine;
+    a.expert_weights[token * a.top_k + lane] = mine >= 0 ? expf(value_of(mine_order) - top) / total : 0.f;
+  }
+}
+
+// Lanes that hold the same expert as this one.
+__device__ inline uint64_t same_expert(int e, int bits) {
+  uint64_t same = __ballot(e >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t set = __ballot(e >> b & 1);
+    same &= e >> b & 1 ? set : ~set;
+  }
+  return same;
+}
+
+// Places of the slots of a block's tokens. places: [waves][experts] in LDS; first[e]: the place of the
+// block's first slot of expert e, in LDS.
+template <int kWaves>
+__device__ inline void place(const MoeRouteArgs& a, int64_t first_slot, int slots, int* places, const int* first) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, experts = a.experts;
+  const int share = (int)ceil_div(ceil_div(slots, kWaves), 64) * 64;
+  const int begin = min(wave * share, slots), end = min(begin + share, slots);
+  for (int i = threadIdx.x; i < kWaves * experts; i += kWaves * 64) places[i] = 0;
+  __syncthreads();
+  for (int i = begin + lane; i < end; i += 64) {
+    const int e = a.expert_ids[first_slot + i];
+    if (e >= 0) atomicAdd(&places[wave * experts + e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += kWaves * 64) {
+    int at = first[e];
+    for (int w = 0; w < kWaves; ++w) {
+      const int n = places[w * experts + e];
+      places[w * experts + e] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  const int bits = 32 - __builtin_clz(experts | 1);
+  for (int i = begin; i < end; i += 64) {
+    const int e = i + lane < end ? a.expert_ids[first_slot + i + lane] : -1;
+    const uint64_t same = same_expert(e, bits);
+    const int before = __popcll(same & ((1ull << lane) - 1));
+    int at = 0;
+    if (e >= 0) at = places[wave * experts + e] + before;
+    __builtin_amdgcn_wave_barrier();
+    if (e >= 0) {
+      if (before == 0) places[wave * experts + e] = at + __popcll(same);
+      a.rows[at] = (int32_t)(first_slot + i + lane);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Turns the counts of all experts into the place of the first slot of each, in LDS, by one wave, 64
+// experts at a time; returns how many slots there are (in that wave).
+__device__ inline int first_places(int* count, int experts) {
+  const int lane = threadIdx.x & 63;
+  int at = 0;
+  for (int e0 = 0; e0 < experts; e0 += 64) {
+    const int e = e0 + lane, n = e < experts ? count[e] : 0;
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int v = __shfl_up(sum, d);
+      if (lane >= d) sum += v;
+    }
+    if (e < experts) count[e] = at + sum - n;
+    at += __shfl(sum, 63);
+  }
+  return at;
+}
+
+// kAll: one workgroup does all. Else only the choices and the counts of a block.
+template <typename T, int kLogits, bool kAll>
+__global__ __launch_bounds__(kAll ? 1024 : 256) void moe_route_kernel(RouteArgs args) {
+  constexpr int kWaves = kAll ? 16 : 4;
+  const MoeRouteArgs& a = args.r;
+  extern __shared__ int memory[];
+  int* const count = memory;                 // [experts], then (kAll) places [waves][experts]
+  const int wave = threadIdx.x >> 6, experts = a.experts;
+  const int64_t first = (int64_t)blockIdx.x * args.block_tokens;
+  const int64_t last = min(first + args.block_tokens, a.tokens);
+  for (int64_t token = first + wave; token < last; token += kWaves) choose<T, kLogits>(a, token);
+  for (int e = threadIdx.x; e < experts; e += kWaves * 64) count[e] = 0;
+  __syncthreads();                           // (the choices are read below, by other waves of the workgroup)
+  const int64_t first_slot = first * a.top_k;
+  const int64_t slots = (last - first) * a.top_k;
+  for (int64_t i = threadIdx.x; i < slots; i += kWaves * 64) {
+    const int e = a.expert_ids[first_slot + i];
+    if (e >= 0) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  if constexpr (!kAll) {
+    for (int e = threadIdx.x; e < experts; e += kWaves * 64) args.counts[(int64_t)blockIdx.x * experts + e] = count[e];
+  } else {
+    __shared__ int all;
+    if (wave == 0) {
+      const int n = first_places(count, experts);
+      if (threadIdx.x == 0) all = n;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += kWaves * 64) a.offsets[e] = count[e];
+    if (threadIdx.x == 0) a.offsets[experts] = all;
+    for (int64_t i = all + threadIdx.x; i < slots; i += kWaves * 64) a.rows[i] = -1;
+    place<kWaves>(a, 0, (int)slots, count + experts, count);
+  }
+}
+
+// Second launch: a block's slots to their places.
+__global__ __launch_bounds__(256) void moe_route_place_kernel(RouteArgs args) {
+  constexpr int kWaves = 4;
+  const MoeRouteArgs& a = args.r;
+  extern __shared__ int memory[];
+  const int experts = a.experts;
+  int* const first = memory;                 // [experts]: of all, then of the block
+  int* const before = memory + experts;      // [experts]: counts of the blocks before; then places [waves][experts]
+  __shared__ int all;
+  for (int e = threadIdx.x; e < experts; e += 256) {
+    int mine = 0, total = 0;
+    for (int b = 0; b < args.blocks; ++b) {
+      const int n = args.counts[(int64_t)b * experts + e];
+      if (b < (int)blockIdx.x) mine += n;
+      total += n;
+    }
+    first[e] = total;
+    before[e] = mine;
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int n = first_places(first, experts);
+    if (threadIdx.x == 0) all = n;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int e = threadIdx.x; e < experts; e += 256) a.offsets[e] = first[e];
+    if (threadIdx.x == 0) a.offsets[experts] = all;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += 256) first[e] += before[e];
+  const int64_t slots = a.tokens * a.top_k;
+  for (int64_t i = all + (int64_t)blockIdx.x * 256 + threadIdx.x; i < slots; i += (int64_t)args.blocks * 256) a.rows[i] = -1;
+  __syncthreads();
+  const int64_t first_token = (int64_t)blockIdx.x * args.block_tokens;
+  const int64_t tokens = min((int64_t)args.block_tokens, a.tokens - first_token);
+  place<kWaves>(a, first_token * a.top_k, (int)(tokens * a.top_k), before, first);
+}
+
+template <typename T, int kLogits>
+int launch_choose(const RouteArgs& args, hipStream_t s) {
+  const int experts = args.r.experts;
+  if (args.blocks == 1)
+    hipLaunchKernelGGL((moe_route_kernel<T, kLogits, true>), dim3(1), dim3(1024), (1 + 16) * experts * 4, s, args);
+  else
+    hipLaunchKernelGGL((moe_route_kernel<T, kLogits, false>), dim3((unsigned)args.blocks), dim3(256), experts * 4, s, args);
+  return check_hip(hipGetLastError(), "moe_route launch");
+}
+
+template <typename T>
+int launch_type(const RouteArgs& args, hipStream_t s) {
+  const int experts = args.r.experts;
+  if (experts <= 64) return launch_choose<T, 1>(args, s);
+  if (experts <= 128) return launch_choose<T, 2>(args, s);
+  if (experts <= 256) return launch_choose<T, 4>(args, s);
+  return launch_choose<T, kMostExperts / 64>(args, s);
+}
+
+// Blocks of tokens of a call that has the workspace.
+int64_t route_blocks(int64_t tokens, int64_t* block_tokens) {
+  *block_tokens = tokens;
+  if (tokens <= kOneBlockTokens) return 1;
+  *block_tokens = ceil_div(ceil_div(tokens, kMostBlocks), kBlockTokens) * kBlockTokens;
+  return ceil_div(tokens, *block_tokens);
+}
+
+}  // namespace
+
+uint64_t moe_route_workspace(int64_t tokens, int experts) {
+  int64_t block_tokens;
+  const int64_t blocks = route_blocks(tokens, &block_tokens);
+  return blocks > 1 ? (uint64_t)blocks * experts * 4 : 0;
+}
+
+int launch_moe_route(const MoeRouteArgs& a, hipStream_t s) {
+  RouteArgs args{a, 0, 1, (int32_t*)a.workspace};
+  int64_t block_tokens, blocks = route_blocks(a.tokens, &block_tokens);
+  if (blocks > 1 && a.workspace_bytes < moe_route_workspace(a.tokens, a.experts)) blocks = 1, block_tokens = a.tokens;
+  args.block_tokens = (int)block_tokens;
+  args.blocks = (int)blocks;
+  int st = a.type == 3 ? launch_type<float>(args, s) : a.type == 2 ? launch_type<BF16>(args, s) : launch_type<F16>(args, s);
+  if (st || blocks == 1) return st;
+  // (the wave's places begin where the counts of the blocks before were)
+  hipLaunchKernelGGL(moe_route_place_kernel, dim3((unsigned)blocks), dim3(256), (1 + 4) * a.experts * 4, s, args);
+  return check_hip(hipGetLastError(), "moe_route launch");
+}
+
+}  // namespace uk
