@@ -6,10 +6,11 @@
 // and the codes need neither the sum of squares nor its root: largest value and sum of
 // squares come out of one reduction, and a row is read once.
 //
-// A row stays in the registers of the threads that share it: one wave up to 1024 elements, 256
-// threads up to 8192, 1024 threads up to 65536. What bounds them is memory.
+// A row stays in the registers of the threads that share it. What bounds them is memory.
 #include "uk_common.h"
 #include "uk_kv4.h"
+
+#include <type_traits>
 
 namespace uk {
 namespace {
@@ -22,8 +23,7 @@ typedef uint32_t code_bits_t __attribute__((ext_vector_type(2), aligned(1)));
 constexpr int kWidth = 8;      // elements a thread holds side by side
 
 // Elements [at, at + 8) of a row of `dim`, zeros past its end.
-template <typename T>
-__device__ inline void load8(const uint16_t* row, int at, int dim, float* x) {
+__device__ inline u32x4 load8(const uint16_t* row, int at, int dim) {
   u32x4 w = {0, 0, 0, 0};
   if (at + kWidth <= dim) {
     w = *(const row_bits_t*)(row + at);
@@ -32,82 +32,92 @@ __device__ inline void load8(const uint16_t* row, int at, int dim, float* x) {
     for (int i = 0; i < kWidth; ++i)
       if (at + i < dim) w[i / 2] |= (uint32_t)row[at + i] << (i % 2 * 16);
   }
+  return w;
+}
+__device__ inline void store8(uint16_t* row, int at, int dim, u32x4 w) {
+  if (at + kWidth <= dim) {
+    *(row_bits_t*)(row + at) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i)
+      if (at + i < dim) row[at + i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+  }
+}
+template <typename T>
+__device__ inline void widen8(u32x4 w, float* x) {
   widen4<T>(u32x2{w.x, w.y}, x);
   widen4<T>(u32x2{w.z, w.w}, x + 4);
 }
 
-// What a row's reductions give.
-struct RowSums {
-  double squares;
-  float top;             // largest size
-  float bad;             // 0, or NaN where a value is not finite
+// The larger size; NaN where one is NaN.
+__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+struct Larger {
+  __device__ float operator()(float a, float b) const { return larger(a, b); }
+  __device__ double operator()(double a, double b) const { return a > b ? a : b; }
 };
-
-__device__ inline RowSums join(RowSums a, RowSums b) {
-  return {a.squares + b.squares, fmaxf(a.top, b.top), a.bad + b.bad};
-}
-struct RowSizes {
-  float top, large;      // largest size, and that of what it is made of
-  float bad;
+struct Sum {
+  __device__ double operator()(double a, double b) const { return a + b; }
 };
-__device__ inline RowSizes join(RowSizes a, RowSizes b) {
-  return {fmaxf(a.top, b.top), fmaxf(a.large, b.large), a.bad + b.bad};
-}
-__device__ inline double join(double a, double b) { return fmax(a, b); }
+constexpr float kMostFloat = 3.4028234663852886e38f;
 
-__device__ inline RowSums other(RowSums v, int mask) {
-  return {__shfl_xor(v.squares, mask), __shfl_xor(v.top, mask), __shfl_xor(v.bad, mask)};
-}
-__device__ inline RowSizes other(RowSizes v, int mask) {
-  return {__shfl_xor(v.top, mask), __shfl_xor(v.large, mask), __shfl_xor(v.bad, mask)};
-}
-__device__ inline double other(double v, int mask) { return __shfl_xor(v, mask); }
-
-// The joint value of the kThreads threads of a row, the same in all of them, added in a fixed
-// order. `shared`: one value for each wave of the row; a barrier on entry for those of a
-// workgroup, so that it may be used again.
-template <int kThreads, typename V>
-__device__ inline V over_row(V v, V* shared) {
-#pragma unroll
-  for (int mask = 1; mask < 64; mask *= 2) v = join(v, other(v, mask));
-  if constexpr (kThreads > 64) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = shared[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / 64; ++w) v = join(v, shared[w]);
+// The values of a lane and its partner in one step of a reduction over a wave, in an order that both
+// have (of the last two steps).
+template <int kStep>
+__device__ inline void partners(uint32_t v, uint32_t* a, uint32_t* b) {
+  if constexpr (kStep < 4) {
+    constexpr int control = kStep == 0 ? 0xB1 : kStep == 1 ? 0x4E : kStep == 2 ? 0x141 : 0x140;
+    *a = v;
+    *b = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, control, 0xF, 0xF, true);
+  } else if constexpr (kStep == 4) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    *a = (uint32_t)p[0], *b = (uint32_t)p[1];
+  } else {
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    *a = (uint32_t)p[0], *b = (uint32_t)p[1];
   }
-  return v;
+}
+template <int kStep, typename F>
+__device__ inline float joined(float v, F f) {
+  uint32_t a, b;
+  partners<kStep>(__builtin_bit_cast(uint32_t, v), &a, &b);
+  return f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+template <int kStep, typename F>
+__device__ inline double joined(double v, F f) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  uint32_t a, b, c, d;
+  partners<kStep>((uint32_t)u, &a, &b);
+  partners<kStep>((uint32_t)(u >> 32), &c, &d);
+  return f(__builtin_bit_cast(double, (uint64_t)c << 32 | a), __builtin_bit_cast(double, (uint64_t)d << 32 | b));
+}
+template <typename V, typename F>
+__device__ inline V over_wave(V v, F f) {
+  v = joined<0>(v, f);
+  v = joined<1>(v, f);
+  v = joined<2>(v, f);
+  v = joined<3>(v, f);
+  v = joined<4>(v, f);
+  return joined<5>(v, f);
 }
 
-// The codes of 8 values t that stand for `exact(i)`, whose largest size in the row is `top`.
-// f32 gives 127 t / top with an error below kSlack; where that leaves open which side of the border
-// between two codes a value lies on, the 64-bit quotient decides: a product of two values of 16 bits
-// over another that is not on a border lies 2^-26 of itself away from it at least.
-template <typename Exact>
-__device__ inline u32x2 codes8(const float* t, float inverse, double top, float slack, Exact exact) {
-  int q[kWidth];
-  float nearest = 1.f;
+// 127 y / top of 8 values as codes: t times `inverse` is added to 1.5 * 2^23 with one rounding, which
+// leaves the code in the last byte; `far` grows to the largest distance from a code.
+__device__ inline u32x2 codes8(const float* t, float inverse, float* far) {
+  constexpr float kShift = 12582912.f;
+  uint32_t b[kWidth];
 #pragma unroll
   for (int i = 0; i < kWidth; ++i) {
-    const float v = t[i] * inverse, r = __builtin_rintf(v);
-    nearest = fminf(nearest, 0.5f - fabsf(v - r));
-    q[i] = (int)r;
-  }
-  if (nearest <= slack) {
-#pragma unroll
-    for (int i = 0; i < kWidth; ++i) {
-      const float v = t[i] * inverse;
-      // (a value that f32 does not hold may be NaN here)
-      if (!(0.5f - fabsf(v - __builtin_rintf(v)) > slack)) q[i] = (int)__builtin_rint(exact(i) * 127.0 / top);
-    }
+    const float moved = __builtin_fmaf(t[i], inverse, kShift), q = moved - kShift;
+    *far = fmaxf(*far, fabsf(__builtin_fmaf(t[i], inverse, -q)));
+    b[i] = __builtin_bit_cast(uint32_t, moved);
   }
   u32x2 w;
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    w[h] = (uint32_t)(q[4 * h] & 0xFF) | (uint32_t)(q[4 * h + 1] & 0xFF) << 8 | (uint32_t)(q[4 * h + 2] & 0xFF) << 16 |
-           (uint32_t)q[4 * h + 3] << 24;
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t lo = __builtin_amdgcn_perm(b[4 * h + 1], b[4 * h], 0x0C0C0400);
+    const uint32_t hi = __builtin_amdgcn_perm(b[4 * h + 3], b[4 * h + 2], 0x04000C0C);
+    w[h] = lo | hi;
+  }
   return w;
 }
 
@@ -121,107 +131,182 @@ __device__ inline void store_codes8(int8_t* row, int at, int dim, u32x2 w) {
   }
 }
 
-// A product of two values of 16 bits is exact in f32, 127 / top and its product with t are each
-// rounded once: below 127 * 2^-23 together, and the subtraction's rounding.
+// The code of a value in 64 bits, which lies between a and a + 1 in size: of a product of two values of 16 bits,
+// over another, both sides are exact.
+__device__ inline uint32_t code_between(double y, double top, float a) {
+  const double size = fabs(y) * 127.0, border = ((double)a + 0.5) * top;
+  const int q = (int)a + (size > border || (size == border && ((int)a & 1)));
+  return (uint32_t)(y < 0.0 ? -q : q) & 0xFF;
+}
+
+// f32 gives 127 t / top with an error below this (127 / top and its product with t are each rounded
+// once, below 127 * 2^-23 together): where a value lies nearer than that to the border between two
+// codes, 64 bits decide.
 constexpr float kSlack = 1.f / 32768;
-// Below this a quotient by the largest value could overflow f32: all of the row in 64 bits.
-constexpr float kTiny = 1e-30f;
+
+// Codes of 8 exact values.
+__device__ inline u32x2 exact_codes8(const float* t, float inverse, float top) {
+  float far = 0.f;
+  u32x2 w = codes8(t, inverse, &far);
+  if (far >= 0.5f - kSlack) {
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) {
+      const float v = fabsf(t[i] * inverse), a = floorf(v);
+      if (fabsf(v - a - 0.5f) <= 2 * kSlack) {
+        asm volatile("");      // (a branch of its own: worked out for all 8, it takes 30 registers more)
+        w[i / 4] = (w[i / 4] & ~(0xFFu << (i % 4 * 8))) | code_between(t[i], top, a) << (i % 4 * 8);
+      }
+    }
+  }
+  return w;
+}
+
+// Rows whose largest value lies below this are worked on 2^100 times as large: 127 / top would overflow.
+constexpr float kTiny = 1e-30f, kTinyScale = 1.2676506002282294e30f;
+
+template <int kReps>
+__device__ inline float scaled_if_tiny(float (&t)[kReps][kWidth], float top) {
+  if (!(top < kTiny)) return top;
+#pragma unroll
+  for (int r = 0; r < kReps; ++r)
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) t[r][i] *= kTinyScale;
+  return top * kTinyScale;
+}
+
+template <int kThreads>
+constexpr int kBlockOf = kThreads < 256 ? 256 : kThreads;
 
 // ---------------------------------------------------------------------------
 // rms_norm_quantize
 // ---------------------------------------------------------------------------
 
-template <typename T, int kThreads, int kReps>
-__global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void rms_norm_quantize_kernel(RmsNormQuantizeArgs a) {
-  constexpr int kBlock = kThreads < 256 ? 256 : kThreads, kRows = kBlock / kThreads;
-  __shared__ RowSums shared[kBlock / 64];
+// Which row of its workgroup's a wave has a part of.
+template <int kThreads>
+__device__ inline int row_of_wave() {
+  return kThreads < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads) : 0;
+}
+
+// Rows of a launch are dealt to its workgroups in turn, kRows at a time; while a row is worked on, the next
+// one of its threads is on its way.
+
+// kOne: one addend without a weight.
+template <typename T, bool kOne, int kThreads, int kReps>
+__global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(RmsNormQuantizeArgs a) {
+  constexpr int kRows = kBlockOf<kThreads> / kThreads, kWaves = kThreads / 64;
+  __shared__ double shared_squares[kWaves];
+  __shared__ float shared_top[kWaves];
   const int thread = threadIdx.x % kThreads, dim = a.dim;
-  for (int64_t token = (int64_t)blockIdx.x * kRows + threadIdx.x / kThreads; token < a.tokens;
-       token += (int64_t)gridDim.x * kRows) {
-    const uint16_t* x = (const uint16_t*)a.x + token * a.x_stride0;
-    const uint16_t* residual = a.residual ? (const uint16_t*)a.residual + token * a.residual_stride : nullptr;
-    uint16_t* sum_out = a.sum_out ? (uint16_t*)a.sum_out + token * a.sum_out_stride : nullptr;
-    const float* factors = a.factors ? a.factors + token * a.factors_stride : nullptr;
-    float t[kReps][kWidth];
-    RowSums sums = {0.0, 0.f, 0.f};
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t token = (int64_t)blockIdx.x * kRows + row_of_wave<kThreads>();
+  u32x4 next_added[kOne ? kReps : 1], next_bits[kReps];
+  auto load_row = [&](int64_t of) {
+    const uint16_t* x = (const uint16_t*)a.x + of * a.x_stride0;
+    const uint16_t* residual = a.residual ? (const uint16_t*)a.residual + of * a.residual_stride : nullptr;
 #pragma unroll
     for (int r = 0; r < kReps; ++r) {
       const int at = (r * kThreads + thread) * kWidth;
+      if constexpr (kOne) next_added[r] = at < dim ? load8(x, at, dim) : u32x4{0, 0, 0, 0};
+      next_bits[r] = residual && at < dim ? load8(residual, at, dim) : u32x4{0, 0, 0, 0};
+    }
+  };
+  if (token < a.tokens) load_row(token);
+  for (; token < a.tokens; token += step) {
+    u32x4 added[kOne ? kReps : 1], bits[kReps];
 #pragma unroll
-      for (int i = 0; i < kWidth; ++i) t[r][i] = 0.f;
-      if (at >= dim) continue;
-      float h[kWidth] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (residual) load8<T>(residual, at, dim, h);
-      if (a.addends == 1 && !factors) {
+    for (int r = 0; r < kReps; ++r) {
+      if constexpr (kOne) added[r] = next_added[r];
+      bits[r] = next_bits[r];
+    }
+    if (token + step < a.tokens) load_row(token + step);
+    // The sum, rounded to its type.
+#pragma unroll
+    for (int r = 0; r < kReps; ++r) {
+      const int at = (r * kThreads + thread) * kWidth;
+      float h[kWidth];
+      __builtin_amdgcn_sched_barrier(0);      // (one after the other, in the same registers)
+      widen8<T>(bits[r], h);
+      if constexpr (kOne) {
         float v[kWidth];
-        load8<T>(x, at, dim, v);
+        widen8<T>(added[r], v);
 #pragma unroll
         for (int i = 0; i < kWidth; ++i) h[i] += v[i];
-      } else {
+      } else if (at < dim) {
         // (several addends in 64 bits, so that their order cannot show in the sum's rounding)
+        const uint16_t* x = (const uint16_t*)a.x + token * a.x_stride0;
+        const float* factors = a.factors ? a.factors + token * a.factors_stride : nullptr;
         double wide[kWidth];
 #pragma unroll
         for (int i = 0; i < kWidth; ++i) wide[i] = h[i];
-#pragma unroll 4
+#pragma unroll 8
         for (int j = 0; j < a.addends; ++j) {
           const float factor = factors ? factors[j] : 1.f;
           float v[kWidth];
-          load8<T>(x + j * a.x_stride1, at, dim, v);
+          widen8<T>(load8(x + j * a.x_stride1, at, dim), v);
           // (what a slot without an expert holds, NaN too, changes nothing)
 #pragma unroll
-          for (int i = 0; i < kWidth; ++i)
-            wide[i] = fma((double)factor, factor == 0.f ? 0.0 : (double)v[i], wide[i]);
+          for (int i = 0; i < kWidth; ++i) wide[i] = fma((double)factor, (double)(factor == 0.f ? 0.f : v[i]), wide[i]);
         }
 #pragma unroll
         for (int i = 0; i < kWidth; ++i) h[i] = (float)wide[i];
       }
-      // The sum as it is kept.
-      u32x4 bits;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bits[i] = T::narrow2(h[2 * i], h[2 * i + 1]);
-      if (sum_out) {
-        if (at + kWidth <= dim) {
-          *(row_bits_t*)(sum_out + at) = bits;
-        } else {
+      for (int i = 0; i < 4; ++i) bits[r][i] = T::narrow2(h[2 * i], h[2 * i + 1]);
+    }
+    if (a.sum_out) {
+      uint16_t* sum_out = (uint16_t*)a.sum_out + token * a.sum_out_stride;
 #pragma unroll
-          for (int i = 0; i < kWidth; ++i)
-            if (at + i < dim) sum_out[at + i] = (uint16_t)(bits[i / 2] >> (i % 2 * 16));
-        }
-      }
-      widen4<T>(u32x2{bits.x, bits.y}, h);
-      widen4<T>(u32x2{bits.z, bits.w}, h + 4);
-      float w[kWidth] = {1, 1, 1, 1, 1, 1, 1, 1};
-      if (a.weight) load8<T>((const uint16_t*)a.weight, at, dim, w);
-#pragma unroll
-      for (int i = 0; i < kWidth; ++i) {
-        t[r][i] = h[i] * w[i];
-        sums.squares = fma((double)h[i], (double)h[i], sums.squares);
-        sums.top = fmaxf(sums.top, fabsf(t[r][i]));
-        sums.bad = fmaf(t[r][i], 0.f, sums.bad);
-      }
-      // (a sum that is not finite next to a weight of 0)
-      if (a.weight) {
-#pragma unroll
-        for (int i = 0; i < kWidth; ++i) sums.bad = fmaf(h[i], 0.f, sums.bad);
+      for (int r = 0; r < kReps; ++r) {
+        const int at = (r * kThreads + thread) * kWidth;
+        if (at < dim) store8(sum_out, at, dim, bits[r]);
       }
     }
-    sums = over_row<kThreads>(sums, shared + threadIdx.x / kThreads * (kThreads / 64));
-    const bool finite = sums.bad == 0.f;
-    const bool tiny = sums.top < kTiny;
-    const float inverse = finite && !tiny ? 127.f / sums.top : 0.f;
+    float t[kReps][kWidth], top = 0.f;
+    double squares = 0.0;
+#pragma unroll
+    for (int r = 0; r < kReps; ++r) {
+      const int at = (r * kThreads + thread) * kWidth;
+      __builtin_amdgcn_sched_barrier(0);
+      widen8<T>(bits[r], t[r]);
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) squares = fma((double)t[r][i], (double)t[r][i], squares);
+      if (a.weight && at < dim) {
+        float w[kWidth];
+        widen8<T>(load8((const uint16_t*)a.weight, at, dim), w);
+#pragma unroll
+        for (int i = 0; i < kWidth; ++i) t[r][i] *= w[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) top = larger(top, fabsf(t[r][i]));
+    }
+    squares = over_wave(squares, Sum());
+    top = over_wave(top, Larger());
+    if constexpr (kWaves > 1) {
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) shared_squares[threadIdx.x >> 6] = squares, shared_top[threadIdx.x >> 6] = top;
+      __syncthreads();
+      squares = shared_squares[0], top = shared_top[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) {
+        squares += shared_squares[w];
+        top = larger(top, shared_top[w]);
+      }
+    }
+    const bool finite = top <= kMostFloat;
+    const float its_top = scaled_if_tiny<kReps>(t, top), inverse = 127.f / its_top;
     int8_t* q = (int8_t*)a.q + token * a.q_stride;
 #pragma unroll
     for (int r = 0; r < kReps; ++r) {
       const int at = (r * kThreads + thread) * kWidth;
       if (at >= dim) continue;
       u32x2 w = {0, 0};
-      if (finite && sums.top > 0.f)
-        w = codes8(t[r], inverse, sums.top, tiny ? 1.f : kSlack, [&](int i) { return (double)t[r][i]; });
+      __builtin_amdgcn_sched_barrier(0);
+      if (finite && top > 0.f) w = exact_codes8(t[r], inverse, its_top);
       store_codes8(q, at, dim, w);
     }
     if (thread == 0) {
-      const double rate = 1.0 / sqrt(sums.squares / dim + (double)a.eps);
-      a.scale[token] = !finite ? __builtin_nanf("") : sums.top > 0.f ? (float)(sums.top * rate / 127.0) : 0.f;
+      const double rate = 1.0 / sqrt(squares / dim + (double)a.eps);
+      a.scale[token] = !finite ? __builtin_nanf("") : top > 0.f ? (float)(top * rate / 127.0) : 0.f;
     }
   }
 }
@@ -230,114 +315,227 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void rms_norm_quan
 // quantize_rows
 // ---------------------------------------------------------------------------
 
-// silu(g) u, within 2^-21 of itself for sizes up to 2^40 and an exponential that f32 holds (past it: 0).
-__device__ inline float silu_mul_near(float g, float u) {
-  constexpr float kLog2e = 1.44269502162933349609375f, kRest = 1.92596299112661746887e-8f;
-  const float p = -g * kLog2e;
-  const float rest = fmaf(-g, kLog2e, -p) - g * kRest;       // -g log2(e) - p
-  const float e = __builtin_amdgcn_exp2f(p);
-  const float sum = 1.f + (p > 126.f ? __builtin_inff() : fmaf(e, rest * 0.693147180559945f, e));
-  return g * __builtin_amdgcn_rcpf(sum) * u;
-}
-__device__ inline double silu_mul_wide(float g, float u) { return (double)g / (1.0 + exp(-(double)g)) * (double)u; }
-constexpr float kGatedSlack = 1.f / 8192;
-constexpr float kLarge = 1.0995116e12f;      // 2^40
-
-template <typename T, bool kGated, int kThreads, int kReps>
-__global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void quantize_rows_kernel(QuantizeRowsArgs a) {
-  constexpr int kBlock = kThreads < 256 ? 256 : kThreads, kRows = kBlock / kThreads;
-  __shared__ RowSizes shared[kBlock / 64];
-  __shared__ double shared_top[kBlock / 64];
-  const int thread = threadIdx.x % kThreads, cols = a.cols, first_wave = threadIdx.x / kThreads * (kThreads / 64);
-  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kThreads; row < a.rows;
-       row += (int64_t)gridDim.x * kRows) {
-    const uint16_t* x = (const uint16_t*)a.x + row * a.x_stride;
-    const uint16_t* up = kGated ? (const uint16_t*)a.up + row * a.up_stride : nullptr;
-    float t[kReps][kWidth];
-    RowSizes sizes = {0.f, 0.f, 0.f};
+template <typename T, int kThreads, int kReps>
+__global__ __launch_bounds__(kBlockOf<kThreads>) void quantize_rows_kernel(QuantizeRowsArgs a) {
+  constexpr int kRows = kBlockOf<kThreads> / kThreads, kWaves = kThreads / 64;
+  __shared__ float shared_top[kWaves];
+  const int thread = threadIdx.x % kThreads, cols = a.cols;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + row_of_wave<kThreads>();
+  u32x4 next[kReps];
+  auto load_row = [&](int64_t of) {
 #pragma unroll
     for (int r = 0; r < kReps; ++r) {
       const int at = (r * kThreads + thread) * kWidth;
-#pragma unroll
-      for (int i = 0; i < kWidth; ++i) t[r][i] = 0.f;
-      if (at >= cols) continue;
-      load8<T>(x, at, cols, t[r]);
-#pragma unroll
-      for (int i = 0; i < kWidth; ++i) sizes.bad = fmaf(t[r][i], 0.f, sizes.bad);
-      if constexpr (kGated) {
-        float u[kWidth];
-        load8<T>(up, at, cols, u);
-#pragma unroll
-        for (int i = 0; i < kWidth; ++i) {
-          sizes.bad = fmaf(u[i], 0.f, sizes.bad);
-          sizes.large = fmaxf(sizes.large, fmaxf(fabsf(t[r][i]), fabsf(u[i])));
-          t[r][i] = silu_mul_near(t[r][i], u[i]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kWidth; ++i) sizes.top = fmaxf(sizes.top, fabsf(t[r][i]));
+      next[r] = at < cols ? load8((const uint16_t*)a.x + of * a.x_stride, at, cols) : u32x4{0, 0, 0, 0};
     }
-    const float mine = sizes.top;
-    sizes = over_row<kThreads>(sizes, shared + first_wave);
-    const bool finite = sizes.bad == 0.f;
-    // Values so large or small that f32 does not hold what the codes are made of: all in 64 bits.
-    const bool wide = sizes.top < kTiny || (kGated && (sizes.large > kLarge || sizes.top < 1.f / kLarge));
-    double top = sizes.top;
-    auto exact = [&](int r, int i) -> double {
-      if constexpr (kGated) {
-        const int at = (r * kThreads + thread) * kWidth + i;
-        return at < cols ? silu_mul_wide(T::widen(x[at]), T::widen(up[at])) : 0.0;
-      } else {
-        return (double)t[r][i];
-      }
-    };
-    if constexpr (kGated) {
-      // The largest in 64 bits is among those that are near the largest in 32.
-      top = 0.0;
-      const float from = wide ? -1.f : sizes.top * (1.f - 1.f / 262144);
-      if (finite && mine >= from) {
-#pragma unroll 1
-        for (int at = thread * kWidth; at < cols; at += kThreads * kWidth)
-          for (int i = 0; i < kWidth && at + i < cols; ++i) {
-            const float g = T::widen(x[at + i]), u = T::widen(up[at + i]);
-            if (fabsf(silu_mul_near(g, u)) >= from || wide) top = fmax(top, fabs(silu_mul_wide(g, u)));
-          }
-      }
-      top = over_row<kThreads>(top, shared_top + first_wave);
+  };
+  if (row < a.rows) load_row(row);
+  for (; row < a.rows; row += step) {
+    float t[kReps][kWidth], top = 0.f;
+#pragma unroll
+    for (int r = 0; r < kReps; ++r) widen8<T>(next[r], t[r]);
+    if (row + step < a.rows) load_row(row + step);
+#pragma unroll
+    for (int r = 0; r < kReps; ++r)
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) top = larger(top, fabsf(t[r][i]));
+    top = over_wave(top, Larger());
+    if constexpr (kWaves > 1) {
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) shared_top[threadIdx.x >> 6] = top;
+      __syncthreads();
+      top = shared_top[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = larger(top, shared_top[w]);
     }
-    const bool fits = finite && top <= 3.4028234663852886e38;
-    const float inverse = fits && !wide ? 127.f / (float)top : 0.f;
+    const bool finite = top <= kMostFloat;
+    const float its_top = scaled_if_tiny<kReps>(t, top), inverse = 127.f / its_top;
     int8_t* q = (int8_t*)a.q + row * a.q_stride;
 #pragma unroll
     for (int r = 0; r < kReps; ++r) {
       const int at = (r * kThreads + thread) * kWidth;
       if (at >= cols) continue;
       u32x2 w = {0, 0};
-      if (fits && top > 0.0)
-        w = codes8(t[r], inverse, top, wide ? 1.f : kGated ? kGatedSlack : kSlack, [&](int i) { return exact(r, i); });
+      __builtin_amdgcn_sched_barrier(0);      // (one after the other, in the same registers)
+      if (finite && top > 0.f) w = exact_codes8(t[r], inverse, its_top);
       store_codes8(q, at, cols, w);
     }
-    if (thread == 0) a.scale[row] = fits ? (float)(top / 127.0) : __builtin_nanf("");
+    if (thread == 0) a.scale[row] = finite ? (float)(top / 127.0) : __builtin_nanf("");
   }
 }
 
-// Rows of a launch in workgroups of `block` threads, `rows` of them in each. (A grid's threads are
-// counted in 32 bits.)
-unsigned grid_of(int64_t rows, int rows_of_block, int block) {
-  const int64_t blocks = ceil_div(rows, rows_of_block), most = 0xFFFFFFFFll / block;
+__device__ inline uint32_t code_of(double y, double top) { return (uint32_t)(int)__builtin_rint(y * 127.0 / top) & 0xFF; }
+
+// silu(g) u, within 2^-19.1 of itself where an exponential of up to 88 closes the gate (past that
+// nothing is left of it next to sizes up to 2^40):
+//   2^p with p = g * -log2(e), and what p's rounding left out as a factor.
+__device__ inline float silu_mul_near(float g, float u) {
+  constexpr float kLog2e = 1.44269502162933349609375f;
+  const float p = g * -kLog2e, rest = __builtin_fmaf(g, -kLog2e, -p);
+  const float e = __builtin_amdgcn_exp2f(p) * __builtin_fmaf(rest, 0.693147180559945f, 1.f);
+  return g * __builtin_amdgcn_rcpf(1.f + e) * u;
+}
+__device__ inline double silu_mul_wide(float g, float u) { return (double)g / (1.0 + exp(-(double)g)) * (double)u; }
+// 127 times the error of such a value and of the largest of the row.
+constexpr float kGatedSlack = 1.f / 2048;
+constexpr float kLarge = 1.0995116e12f;      // 2^40
+// Eights of a row with a code (or the largest value) that f32 leaves open: about one in 130, whose elements
+// the threads then look at side by side. A row with more of them is worked out in 64 bits as a whole.
+constexpr int kMostOpen = 512;
+
+// All of a row in 64 bits: rows of sizes that f32 does not hold, or with too many open codes.
+template <typename T, int kThreads>
+__device__ inline void gated_row_wide(const uint16_t* x, const uint16_t* up, int8_t* q, float* scale, int cols,
+                                      double* shared) {
+  const int thread = threadIdx.x;
+  double top = 0.0;
+#pragma unroll 1
+  for (int i = thread; i < cols; i += kThreads) {
+    const float g = T::widen(x[i]), u = T::widen(up[i]);
+    const double y = fabs(silu_mul_wide(g, u));
+    const bool finite = fabsf(g) <= kMostFloat && fabsf(u) <= kMostFloat && y <= kMostFloat;
+    top = Larger()(top, finite ? y : (double)__builtin_inff());
+  }
+  top = over_wave(top, Larger());
+  __syncthreads();
+  if ((thread & 63) == 0) shared[thread >> 6] = top;
+  __syncthreads();
+  top = shared[0];
+  for (int w = 1; w < kThreads / 64; ++w) top = Larger()(top, shared[w]);
+  const bool finite = top <= kMostFloat;
+#pragma unroll 1
+  for (int i = thread; i < cols; i += kThreads)
+    q[i] = finite && top > 0.0 ? (int8_t)code_of(silu_mul_wide(T::widen(x[i]), T::widen(up[i])), top) : 0;
+  if (thread == 0) *scale = finite ? (float)(top / 127.0) : __builtin_nanf("");
+}
+
+template <typename T, int kThreads, int kReps>
+__global__ __launch_bounds__(kThreads) void quantize_gated_rows_kernel(QuantizeRowsArgs a) {
+  constexpr int kWaves = kThreads / 64;
+  constexpr bool kAnySize = std::is_same<T, BF16>::value;      // (f16 has none above 2^40)
+  __shared__ float shared_top[kWaves], shared_large[kWaves];
+  __shared__ double shared_wide[kWaves];
+  __shared__ int open_count[2], open[2][kMostOpen];      // candidates for the largest, open codes
+  const int thread = threadIdx.x, cols = a.cols;
+  u32x4 gates[kReps], ups[kReps];
+  auto load_row = [&](int64_t of) {
+    const uint16_t* x = (const uint16_t*)a.x + of * a.x_stride;
+    const uint16_t* up = (const uint16_t*)a.up + of * a.up_stride;
+#pragma unroll
+    for (int r = 0; r < kReps; ++r) {
+      const int at = (r * kThreads + thread) * kWidth;
+      gates[r] = at < cols ? load8(x, at, cols) : u32x4{0, 0, 0, 0};
+      ups[r] = at < cols ? load8(up, at, cols) : u32x4{0, 0, 0, 0};
+    }
+  };
+  constexpr bool kAhead = kReps <= 2;
+  if (kAhead && (int64_t)blockIdx.x < a.rows) load_row(blockIdx.x);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if constexpr (!kAhead) load_row(row);
+    const uint16_t* x = (const uint16_t*)a.x + row * a.x_stride;
+    const uint16_t* up = (const uint16_t*)a.up + row * a.up_stride;
+    int8_t* q = (int8_t*)a.q + row * a.q_stride;
+    float t[kReps][kWidth], mine[kReps], top = 0.f, large = 0.f;
+#pragma unroll
+    for (int r = 0; r < kReps; ++r) {
+      float g[kWidth], u[kWidth];
+      __builtin_amdgcn_sched_barrier(0);      // (one after the other, in the same registers)
+      widen8<T>(gates[r], g);
+      widen8<T>(ups[r], u);
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) {
+        t[r][i] = silu_mul_near(g[i], u[i]);
+        if constexpr (kAnySize) large = fmaxf(fmaxf(large, fabsf(g[i])), fabsf(u[i]));
+      }
+      // (a gate or factor that is not finite gives a product that is not either)
+      mine[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) mine[r] = larger(mine[r], fabsf(t[r][i]));
+      top = larger(top, mine[r]);
+    }
+    if (kAhead && row + gridDim.x < a.rows) load_row(row + gridDim.x);
+    top = over_wave(top, Larger());
+    if constexpr (kAnySize) large = over_wave(large, Larger());
+    if ((thread & 63) == 0) shared_top[thread >> 6] = top, shared_large[thread >> 6] = large;
+    if (thread < 2) open_count[thread] = 0;
+    __syncthreads();
+    top = shared_top[0], large = shared_large[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+      top = larger(top, shared_top[w]);
+      if constexpr (kAnySize) large = larger(large, shared_large[w]);
+    }
+    bool wide = !(top <= kLarge * kLarge) || top < 1.f / kLarge || (kAnySize && !(large <= kLarge));
+    const float from = top * (1.f - 1.f / 131072), inverse = 127.f / top;
+    if (!wide) {
+#pragma unroll
+      for (int r = 0; r < kReps; ++r) {
+        const int at = (r * kThreads + thread) * kWidth;
+        float far = 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+        const u32x2 w = codes8(t[r], inverse, &far);
+        if (at < cols) store_codes8(q, at, cols, w);
+        if (mine[r] >= from) {
+          const int n = atomicAdd(&open_count[0], 1);
+          if (n < kMostOpen) open[0][n] = at;
+        }
+        if (far >= 0.5f - kGatedSlack) {
+          const int n = atomicAdd(&open_count[1], 1);
+          if (n < kMostOpen) open[1][n] = at;
+        }
+      }
+      __syncthreads();           // (the codes are stored, the lists are complete)
+      wide = open_count[0] > kMostOpen || open_count[1] > kMostOpen;
+    }
+    if (wide) {
+      gated_row_wide<T, kThreads>(x, up, q, &a.scale[row], cols, shared_wide);
+    } else {
+      // One wave has the largest in 64 bits, which is among those near the largest in 32, then all the open codes.
+      if (thread < 64) {
+        double exact = 0.0;
+        for (int n = thread; n < open_count[0] * kWidth; n += 64) {
+          const int i = open[0][n / kWidth] + n % kWidth;
+          if (i >= cols) continue;
+          const float g = T::widen(x[i]), u = T::widen(up[i]);
+          if (fabsf(silu_mul_near(g, u)) >= from) exact = Larger()(exact, fabs(silu_mul_wide(g, u)));
+        }
+        exact = over_wave(exact, Larger());
+        if (thread == 0) shared_wide[0] = exact, a.scale[row] = (float)(exact / 127.0);
+      }
+      __syncthreads();
+      const double exact = shared_wide[0];
+      for (int n = thread; n < open_count[1] * kWidth; n += kThreads) {
+        const int i = open[1][n / kWidth] + n % kWidth;
+        if (i >= cols) continue;
+        const float g = T::widen(x[i]), u = T::widen(up[i]), v = silu_mul_near(g, u) * inverse;
+        if (fabsf(v - __builtin_rintf(v)) >= 0.5f - 1.02f * kGatedSlack)
+          q[i] = (int8_t)code_of(silu_mul_wide(g, u), exact);
+      }
+    }
+    __syncthreads();             // (the lists are used up)
+  }
+}
+
+// Workgroups of `block` threads for so many rows, `rows_of_block` in each at a time: at most `waves` of them on
+// a vector unit, whether resident or not; they take the rows in turn.
+unsigned grid_of(int64_t rows, int rows_of_block, int block, int waves) {
+  const int64_t blocks = ceil_div(rows, (int64_t)rows_of_block), most = (int64_t)device_cu_count() * waves * 256 / block;
   return (unsigned)(blocks < most ? blocks : most);
 }
 
-// Calls launch(threads, reps) with the shape that holds a row of `dim` elements.
+// Calls launch(threads, reps) with the first of the shapes (threads that share a row, times 8 elements of
+// each) that holds a row of `dim` elements and is not left out by `from`.
 template <typename Launch>
-int with_row_shape(int64_t dim, Launch launch) {
-#define UK_ROW_SHAPE(threads, reps) \
-  if (dim <= (threads) * (reps) * kWidth) return launch(std::integral_constant<int, threads>(), std::integral_constant<int, reps>())
+int with_row_shape(int64_t dim, int64_t from, Launch launch) {
+#define UK_ROW_SHAPE(threads, reps)                                     \
+  if (dim <= (threads) * (reps) * kWidth && (threads) * (reps) >= from) \
+  return launch(std::integral_constant<int, threads>(), std::integral_constant<int, reps>())
   UK_ROW_SHAPE(64, 1);
   UK_ROW_SHAPE(64, 2);
   UK_ROW_SHAPE(256, 1);
   UK_ROW_SHAPE(256, 2);
-  UK_ROW_SHAPE(256, 4);
+  UK_ROW_SHAPE(512, 2);
   UK_ROW_SHAPE(1024, 2);
   UK_ROW_SHAPE(1024, 4);
   UK_ROW_SHAPE(1024, 8);
@@ -348,31 +546,34 @@ int with_row_shape(int64_t dim, Launch launch) {
 }  // namespace
 
 int launch_rms_norm_quantize(const RmsNormQuantizeArgs& a, hipStream_t s) {
-  return with_row_shape(a.dim, [&](auto threads, auto reps) {
-    constexpr int kThreads = decltype(threads)::value, kReps = decltype(reps)::value;
-    constexpr int kBlock = kThreads < 256 ? 256 : kThreads;
-    const dim3 grid(grid_of(a.tokens, kBlock / kThreads, kBlock));
-    if (a.bf16)
-      hipLaunchKernelGGL((rms_norm_quantize_kernel<BF16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+  return with_row_shape(a.dim, 0, [&](auto threads, auto reps) {
+    constexpr int kThreads = decltype(threads)::value, kReps = decltype(reps)::value, kBlock = kBlockOf<kThreads>;
+    const dim3 grid(grid_of(a.tokens, kBlock / kThreads, kBlock, 8));
+    const bool one = a.addends == 1 && !a.factors;
+    if (a.bf16 && one)
+      hipLaunchKernelGGL((rms_norm_quantize_kernel<BF16, true, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+    else if (a.bf16)
+      hipLaunchKernelGGL((rms_norm_quantize_kernel<BF16, false, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+    else if (one)
+      hipLaunchKernelGGL((rms_norm_quantize_kernel<F16, true, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
     else
-      hipLaunchKernelGGL((rms_norm_quantize_kernel<F16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+      hipLaunchKernelGGL((rms_norm_quantize_kernel<F16, false, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
     return check_hip(hipGetLastError(), "rms_norm_quantize launch");
   });
 }
 
 int launch_quantize_rows(const QuantizeRowsArgs& a, hipStream_t s) {
-  return with_row_shape(a.cols, [&](auto threads, auto reps) {
-    constexpr int kThreads = decltype(threads)::value, kReps = decltype(reps)::value;
-    constexpr int kBlock = kThreads < 256 ? 256 : kThreads;
-    const dim3 grid(grid_of(a.rows, kBlock / kThreads, kBlock));
-    if (a.bf16 && a.up)
-      hipLaunchKernelGGL((quantize_rows_kernel<BF16, true, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-    else if (a.bf16)
-      hipLaunchKernelGGL((quantize_rows_kernel<BF16, false, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-    else if (a.up)
-      hipLaunchKernelGGL((quantize_rows_kernel<F16, true, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-    else
-      hipLaunchKernelGGL((quantize_rows_kernel<F16, false, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+  // (gated rows always have a whole workgroup)
+  return with_row_shape(a.cols, a.up ? 256 : 0, [&](auto threads, auto reps) {
+    constexpr int kThreads = decltype(threads)::value, kReps = decltype(reps)::value, kBlock = kBlockOf<kThreads>;
+    const dim3 grid(grid_of(a.rows, kBlock / kThreads, kBlock, a.up ? 4 : 8));
+    if (!a.up) {
+      if (a.bf16) hipLaunchKernelGGL((quantize_rows_kernel<BF16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+      else hipLaunchKernelGGL((quantize_rows_kernel<F16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+    } else if constexpr (kThreads >= 256) {
+      if (a.bf16) hipLaunchKernelGGL((quantize_gated_rows_kernel<BF16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+      else hipLaunchKernelGGL((quantize_gated_rows_kernel<F16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+    }
     return check_hip(hipGetLastError(), "quantize_rows launch");
   });
 }
