@@ -1,9 +1,8 @@
 // Each token's experts and their weights from its logits, and the tokens' slots in the order of
 // their experts (include/iree_amd_uk.h).
 //
-// A wave chooses for a token: its lanes hold the logits, and top_k times the largest of all lanes is
-// taken, as one 64-bit key of the value and, below it, the number of the expert counted down, so that
-// of equal values the lowest expert wins. The slots are then sorted by expert the way one digit of
+// A wave chooses for a token: its lanes hold the logits as integers of the same order, and top_k times the
+// largest is taken from the lowest expert that has it. The slots are then sorted by expert the way one digit of
 // a radix sort is: blocks of consecutive tokens count their slots of every expert, and a slot's place
 // is its expert's first place, plus the counts of the blocks and waves before, plus the lanes before it
 // with the same expert. The order of no addition decides anything: the lists are the same on every call.
@@ -21,7 +20,8 @@ using namespace kv4;
 
 constexpr int kMostExperts = 512;
 constexpr int kMostBlocks = 256;           // blocks of tokens
-constexpr int kBlockTokens = 64;           // of one, at least
+constexpr int kBlockTokens = 16;           // of one, at least
+constexpr int kBlockWaves = 8;
 constexpr int kOneBlockTokens = 128;       // up to which one workgroup does all
 
 struct RouteArgs {
@@ -47,6 +47,19 @@ __device__ inline float logit(const void* row, int e) {
   else return T::widen(((const uint16_t*)row)[e]);
 }
 
+__device__ inline uint32_t largest_of_wave(uint32_t v) {
+  auto with = [&](uint32_t o) { v = o > v ? o : v; };
+  with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));       // lane ^ 1, ^ 2, mirrors of 8 and 16
+  with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));
+  with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true));
+  with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, true));
+  const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = p[0] > p[1] ? p[0] : p[1];
+  const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = q[0] > q[1] ? q[0] : q[1];
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+
 // The experts and weights of one token, by a wave. kLogits: a lane's.
 template <typename T, int kLogits>
 __device__ inline void choose(const MoeRouteArgs& a, int64_t token) {
@@ -58,26 +71,17 @@ __device__ inline void choose(const MoeRouteArgs& a, int64_t token) {
     const int e = i * 64 + lane;
     order[i] = e < a.experts ? order_of(logit<T>(row, e)) : 0;
   }
-  // The best of a lane's own is kept until it is taken.
-  float top = 0.f, total = 0.f;
-  uint32_t mine_order = 0;
+  float top = 0.f, total = 0.f, mine_logit = 0.f;
   int mine = -1;
   for (int k = 0; k < a.top_k; ++k) {
-    uint32_t best = 0;
-    int best_i = 0;
+    uint32_t best = order[0];
 #pragma unroll
-    for (int i = 0; i < kLogits; ++i)
-      if (order[i] > best) best = order[i], best_i = i;
-    uint64_t key = best ? (uint64_t)best << 32 | (uint32_t)~(best_i * 64 + lane) : 0;
-#pragma unroll
-    for (int mask = 32; mask; mask >>= 1) {
-      const uint64_t there = (uint64_t)__shfl_xor((uint32_t)(key >> 32), mask) << 32 | __shfl_xor((uint32_t)key, mask);
-      key = there > key ? there : key;
-    }
-    const int e = key ? (int)~(uint32_t)key : -1;
-    const uint32_t chosen = (uint32_t)(key >> 32);
+    for (int i = 1; i < kLogits; ++i) best = order[i] > best ? order[i] : best;
+    best = largest_of_wave(best);
+    if (best == 0) break;
+    const float its_logit = value_of(best);
     if (k == 0) {
-      top = key ? value_of(chosen) : 0.f;
+      top = its_logit;
       if (!a.renormalize) {
         float sum = 0.f;
 #pragma unroll
@@ -88,17 +92,22 @@ __device__ inline void choose(const MoeRouteArgs& a, int64_t token) {
         total = sum;
       }
     }
-    if (e >= 0) {
-      if (a.renormalize) total += expf(value_of(chosen) - top);
+    if (a.renormalize) total += expf(its_logit - top);
+    bool taken = false;
 #pragma unroll
-      for (int i = 0; i < kLogits; ++i)
-        if (e == i * 64 + lane) order[i] = 0;
+    for (int i = 0; i < kLogits; ++i) {
+      const uint64_t has = taken ? 0 : __ballot(order[i] == best);
+      if (has) {
+        const int l = __builtin_ctzll(has);
+        if (lane == l) order[i] = 0;
+        if (lane == k) mine = i * 64 + l, mine_logit = its_logit;
+        taken = true;
+      }
     }
-    if (lane == k) mine = e, mine_order = chosen;
   }
   if (lane < a.top_k) {
     a.expert_ids[token * a.top_k + lane] = mine;
-    a.expert_weights[token * a.top_k + lane] = mine >= 0 ? expf(value_of(mine_order) - top) / total : 0.f;
+    a.expert_weights[token * a.top_k + lane] = mine >= 0 ? expf(mine_logit - top) / total : 0.f;
   }
 }
 
@@ -172,8 +181,8 @@ __device__ inline int first_places(int* count, int experts) {
 
 // kAll: one workgroup does all. Else only the choices and the counts of a block.
 template <typename T, int kLogits, bool kAll>
-__global__ __launch_bounds__(kAll ? 1024 : 256) void moe_route_kernel(RouteArgs args) {
-  constexpr int kWaves = kAll ? 16 : 4;
+__global__ __launch_bounds__(kAll ? 1024 : kBlockWaves * 64) void moe_route_kernel(RouteArgs args) {
+  constexpr int kWaves = kAll ? 16 : kBlockWaves;
   const MoeRouteArgs& a = args.r;
   extern __shared__ int memory[];
   int* const count = memory;                 // [experts], then (kAll) places [waves][experts]
@@ -207,23 +216,29 @@ __global__ __launch_bounds__(kAll ? 1024 : 256) void moe_route_kernel(RouteArgs 
 }
 
 // Second launch: a block's slots to their places.
-__global__ __launch_bounds__(256) void moe_route_place_kernel(RouteArgs args) {
-  constexpr int kWaves = 4;
+__global__ __launch_bounds__(kBlockWaves * 64) void moe_route_place_kernel(RouteArgs args) {
+  constexpr int kWaves = kBlockWaves, kThreads = kWaves * 64;
   const MoeRouteArgs& a = args.r;
   extern __shared__ int memory[];
   const int experts = a.experts;
   int* const first = memory;                 // [experts]: of all, then of the block
   int* const before = memory + experts;      // [experts]: counts of the blocks before; then places [waves][experts]
   __shared__ int all;
-  for (int e = threadIdx.x; e < experts; e += 256) {
+  for (int e = threadIdx.x; e < experts; e += kThreads) first[e] = before[e] = 0;
+  __syncthreads();
+  // (experts side by side, and as many shares of the blocks as there are threads for)
+  const int width = experts <= 64 ? 64 : experts <= 128 ? 128 : experts <= 256 ? 256 : 512;
+  const int shares = kThreads / width, e = threadIdx.x % width;
+  if (e < experts) {
     int mine = 0, total = 0;
-    for (int b = 0; b < args.blocks; ++b) {
+#pragma unroll 8
+    for (int b = threadIdx.x / width; b < args.blocks; b += shares) {
       const int n = args.counts[(int64_t)b * experts + e];
-      if (b < (int)blockIdx.x) mine += n;
+      mine += b < (int)blockIdx.x ? n : 0;
       total += n;
     }
-    first[e] = total;
-    before[e] = mine;
+    atomicAdd(&first[e], total);
+    atomicAdd(&before[e], mine);
   }
   __syncthreads();
   if (threadIdx.x < 64) {
@@ -232,13 +247,14 @@ __global__ __launch_bounds__(256) void moe_route_place_kernel(RouteArgs args) {
   }
   __syncthreads();
   if (blockIdx.x == 0) {
-    for (int e = threadIdx.x; e < experts; e += 256) a.offsets[e] = first[e];
+    for (int e = threadIdx.x; e < experts; e += kThreads) a.offsets[e] = first[e];
     if (threadIdx.x == 0) a.offsets[experts] = all;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < experts; e += 256) first[e] += before[e];
+  for (int e = threadIdx.x; e < experts; e += kThreads) first[e] += before[e];
   const int64_t slots = a.tokens * a.top_k;
-  for (int64_t i = all + (int64_t)blockIdx.x * 256 + threadIdx.x; i < slots; i += (int64_t)args.blocks * 256) a.rows[i] = -1;
+  for (int64_t i = all + (int64_t)blockIdx.x * kThreads + threadIdx.x; i < slots; i += (int64_t)args.blocks * kThreads)
+    a.rows[i] = -1;
   __syncthreads();
   const int64_t first_token = (int64_t)blockIdx.x * args.block_tokens;
   const int64_t tokens = min((int64_t)args.block_tokens, a.tokens - first_token);
@@ -251,7 +267,8 @@ int launch_choose(const RouteArgs& args, hipStream_t s) {
   if (args.blocks == 1)
     hipLaunchKernelGGL((moe_route_kernel<T, kLogits, true>), dim3(1), dim3(1024), (1 + 16) * experts * 4, s, args);
   else
-    hipLaunchKernelGGL((moe_route_kernel<T, kLogits, false>), dim3((unsigned)args.blocks), dim3(256), experts * 4, s, args);
+    hipLaunchKernelGGL((moe_route_kernel<T, kLogits, false>), dim3((unsigned)args.blocks), dim3(kBlockWaves * 64),
+                       experts * 4, s, args);
   return check_hip(hipGetLastError(), "moe_route launch");
 }
 
@@ -288,8 +305,9 @@ int launch_moe_route(const MoeRouteArgs& a, hipStream_t s) {
   args.blocks = (int)blocks;
   int st = a.type == 3 ? launch_type<float>(args, s) : a.type == 2 ? launch_type<BF16>(args, s) : launch_type<F16>(args, s);
   if (st || blocks == 1) return st;
-  // (the wave's places begin where the counts of the blocks before were)
-  hipLaunchKernelGGL(moe_route_place_kernel, dim3((unsigned)blocks), dim3(256), (1 + 4) * a.experts * 4, s, args);
+  // (the waves' places begin where the counts of the blocks before were)
+  hipLaunchKernelGGL(moe_route_place_kernel, dim3((unsigned)blocks), dim3(kBlockWaves * 64),
+                     (1 + kBlockWaves) * a.experts * 4, s, args);
   return check_hip(hipGetLastError(), "moe_route launch");
 }
 
