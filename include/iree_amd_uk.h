@@ -870,19 +870,13 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_quantize_rows(
  * bits, its rows readable up to K rounded up to 16 (what lies past K does not count). rhs
  * is packed as iree_amd_uk_pack does for the right-hand side of a matmul, in tiles of
  * 32 x 16 with padding 0: [N / 32][K / 16][32][16], rhs_stride0 bytes between
- * outer columns; 16-byte aligned. out is row-major with any alignment of its elements.
- *   workspace: partial sums of a long K over few tiles, at least what
- * iree_amd_uk_matmul_w8a8_workspace says, 16-byte aligned; with less, or null, the call
- * runs unsplit: slower, the same bits. The caller's: calls that may overlap, and graphs
- * whose replays may, need one each. */
+ * outer columns; 16-byte aligned. out is row-major with any alignment of its elements. Nothing is
+ * allocated. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_matmul_w8a8(
     const void* lhs, iree_amd_uk_index_t lhs_stride0, const float* lhs_scale, const void* rhs,
     iree_amd_uk_index_t rhs_stride0, const float* rhs_scale, const float* bias, void* out,
     iree_amd_uk_index_t out_stride0, iree_amd_uk_index_t M, iree_amd_uk_index_t N,
-    iree_amd_uk_index_t K, void* workspace, uint64_t workspace_bytes, uint32_t flags, void* stream);
-/* Bytes of workspace such a call uses on the current device (0: none). */
-IREE_AMD_UK_EXPORT int iree_amd_uk_matmul_w8a8_workspace(iree_amd_uk_index_t M, iree_amd_uk_index_t N,
-                                                         iree_amd_uk_index_t K, uint64_t* out_bytes);
+    iree_amd_uk_index_t K, uint32_t flags, void* stream);
 
 /* The top_k experts of each token (top_k up to 64 and `experts`, which is up to 512) by
  * its logits ([tokens][experts], any ROWS_TYPE, logits_stride0 elements apart), the
@@ -895,8 +889,9 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_matmul_w8a8_workspace(iree_amd_uk_index_t M, 
  * expert in their own: rows[tokens * top_k], those of expert e at [offsets[e],
  * offsets[e + 1]), and -1 from offsets[experts] on. The same lists on every call.
  * tokens * top_k lies below 2^31.
- *   workspace: at least what iree_amd_uk_moe_route_workspace says, 16-byte aligned, as
- * above; without it one workgroup does all. */
+ *   workspace: at least what iree_amd_uk_moe_route_workspace says, 16-byte aligned; with
+ * less, or null, one workgroup does all: slower, the same lists. The caller's: calls
+ * that may overlap, and graphs whose replays may, need one each. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_moe_route(
     const void* logits, iree_amd_uk_index_t logits_stride0, int32_t* expert_ids,
     float* expert_weights, int32_t* offsets, int32_t* rows, iree_amd_uk_index_t tokens,
@@ -997,7 +992,7 @@ IREE_AMD_UK_EXPORT const char* iree_amd_uk_last_error(void);
  * "dequant_i4:gemv", "dequant_i4:gemm", "dequant_i4:reassociated",
  * "dequant_i4:reassociated-element-wise", "dequant_i4:element-wise",
  * "attention_kv4:few-rows", "attention_kv4:prompt", each with "-split" behind it when the
- * caches were split over workgroups, "w8a8:few-rows", "w8a8:mfma", "w8a8:mfma-split" ("" before the first call). A static string. No counterpart in the reference, whose
+ * caches were split over workgroups, "w8a8:few-rows", "w8a8:mfma" ("" before the first call). A static string. No counterpart in the reference, whose
  * tile-function choice is visible through iree_uk_mmt4d_info only. */
 IREE_AMD_UK_EXPORT const char* iree_amd_uk_last_kernel_path(void);
 /* Rows and columns of the macro tile of the calling thread's last "mmt4d:mfma"

@@ -51,7 +51,6 @@ from .ukernel import (  # noqa: F401
 from .w8a8 import (  # noqa: F401
     grouped_matmul_w8a8,
     matmul_w8a8,
-    matmul_w8a8_workspace,
     moe_route,
     moe_route_workspace,
     quantize_rows,

@@ -175,9 +175,7 @@ def _declare(lib):
     lib.iree_amd_uk_quantize_rows.restype = C.c_int
     lib.iree_amd_uk_quantize_rows.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i64, u32, vp]
     lib.iree_amd_uk_matmul_w8a8.restype = C.c_int
-    lib.iree_amd_uk_matmul_w8a8.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, i64, i64, i64, i64, vp, C.c_uint64, u32, vp]
-    lib.iree_amd_uk_matmul_w8a8_workspace.restype = C.c_int
-    lib.iree_amd_uk_matmul_w8a8_workspace.argtypes = [i64, i64, i64, C.POINTER(C.c_uint64)]
+    lib.iree_amd_uk_matmul_w8a8.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, i64, i64, i64, i64, u32, vp]
     lib.iree_amd_uk_moe_route.restype = C.c_int
     lib.iree_amd_uk_moe_route.argtypes = [vp, i64, vp, vp, vp, vp, i64, i32, i32, vp, C.c_uint64, u32, vp]
     lib.iree_amd_uk_moe_route_workspace.restype = C.c_int

@@ -1258,7 +1258,7 @@ extern "C" int iree_amd_uk_moe_route_workspace(iree_amd_uk_index_t tokens, int32
 }
 
 // What the two products share: sizes, rows of 8 bits, packed weights of `experts`, the result.
-static int validate_w8a8(const char* what, const W8A8Args& a, int64_t N, int64_t K) {
+static int validate_w8a8(const char* what, int64_t N, int64_t K) {
   if (N < 0 || N > (1 << 24) || K < 0)
     return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: N outside [0, 2^24] or negative K", what);
   if (K > 131071) return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: K above 131071", what);
@@ -1287,32 +1287,19 @@ extern "C" int iree_amd_uk_matmul_w8a8(const void* lhs, iree_amd_uk_index_t lhs_
                                        const void* rhs, iree_amd_uk_index_t rhs_stride0, const float* rhs_scale,
                                        const float* bias, void* out, iree_amd_uk_index_t out_stride0,
                                        iree_amd_uk_index_t M, iree_amd_uk_index_t N, iree_amd_uk_index_t K,
-                                       void* workspace, uint64_t workspace_bytes, uint32_t flags, void* stream) {
+                                       uint32_t flags, void* stream) {
   const char* what = "matmul_w8a8";
   UK_RETURN_IF_ERROR(validate_rows8_flags(what, flags, 0, IREE_AMD_UK_FLAG_ROWS_TYPE_F32));
   W8A8Args a{};
   if (M < 0 || M > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: M outside [0, 2^31)", what);
-  UK_RETURN_IF_ERROR(validate_w8a8(what, a, N, K));
-  UK_RETURN_IF_ERROR(validate_workspace(what, workspace, workspace_bytes));
+  UK_RETURN_IF_ERROR(validate_w8a8(what, N, K));
   if (M == 0 || N == 0) return 0;
   a.lhs = (const char*)lhs, a.lhs_stride = lhs_stride0, a.lhs_rows = M, a.lhs_scale = lhs_scale;
   a.rhs = (const char*)rhs, a.rhs_stride = rhs_stride0, a.rhs_scale = rhs_scale, a.bias = bias;
   a.out = (char*)out, a.out_stride = out_stride0, a.out_rows = M, a.positions = M, a.rows_per_token = 1;
   a.experts = 1, a.N = (int)N, a.K = (int)K, a.type = (int)(flags & IREE_AMD_UK_FLAG_ROWS_TYPE_MASK);
-  a.workspace = workspace, a.workspace_bytes = workspace ? workspace_bytes : 0;
   UK_RETURN_IF_ERROR(validate_w8a8_buffers(what, a));
   return launch_w8a8(a, (hipStream_t)stream);
-}
-
-extern "C" int iree_amd_uk_matmul_w8a8_workspace(iree_amd_uk_index_t M, iree_amd_uk_index_t N, iree_amd_uk_index_t K,
-                                                 uint64_t* out_bytes) {
-  const char* what = "matmul_w8a8_workspace";
-  if (!out_bytes) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: null result", what);
-  *out_bytes = 0;
-  if (M < 0 || M > 0x7FFFFFFF) return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: M outside [0, 2^31)", what);
-  UK_RETURN_IF_ERROR(validate_w8a8(what, W8A8Args{}, N, K));
-  if (M && N && K) *out_bytes = w8a8_workspace(M, N, K);
-  return 0;
 }
 
 extern "C" int iree_amd_uk_grouped_matmul_w8a8(
@@ -1325,7 +1312,7 @@ extern "C" int iree_amd_uk_grouped_matmul_w8a8(
   UK_RETURN_IF_ERROR(validate_rows8_flags(what, flags, IREE_AMD_UK_FLAG_GROUPED_GATHER | IREE_AMD_UK_FLAG_GROUPED_SCATTER,
                                           IREE_AMD_UK_FLAG_ROWS_TYPE_F32));
   W8A8Args a{};
-  UK_RETURN_IF_ERROR(validate_w8a8(what, a, N, K));
+  UK_RETURN_IF_ERROR(validate_w8a8(what, N, K));
   if (lhs_rows < 0 || lhs_rows > 0x7FFFFFFF || out_rows < 0 || out_rows > 0x7FFFFFFF || positions < 0 ||
       positions > 0x7FFFFFFF || experts < 0)
     return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT, "%s: rows, positions or experts outside [0, 2^31)", what);

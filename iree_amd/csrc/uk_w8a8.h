@@ -25,12 +25,17 @@ struct W8A8Args {
   bool gather, scatter;
   int experts, N, K;
   int type;                            // of the result: 1 f16, 2 bf16, 3 f32
-  void* workspace;
-  uint64_t workspace_bytes;
 };
 
 int launch_w8a8(const W8A8Args& a, hipStream_t s);
-uint64_t w8a8_workspace(int64_t M, int64_t N, int64_t K);
+// Macro tiles (uk_w8a8_mfma.hip), by number.
+constexpr int kW8A8Shapes = 5;
+int launch_w8a8_mfma(const W8A8Args& a, int shape, hipStream_t s);
+// Tiles of rows that there can be at most: of every expert that has any, the last is not full.
+inline int64_t w8a8_row_tiles(const W8A8Args& a, int height) {
+  if (!a.offsets) return ceil_div(a.positions, (int64_t)height);
+  return a.positions / height + (a.experts < a.positions ? a.experts : a.positions);
+}
 
 namespace w8a8 {
 

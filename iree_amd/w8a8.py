@@ -54,36 +54,17 @@ def quantize_rows(x, q, scale, rows, cols, flags, *, up=None, x_stride0=None, up
         cols, flags, _stream_on(stream, device)))
 
 
-def matmul_w8a8_workspace(M, N, K):
-    """Bytes of workspace that ``matmul_w8a8`` of these sizes uses (0: none)."""
-    out = C.c_uint64(0)
-    _check(load_library().iree_amd_uk_matmul_w8a8_workspace(M, N, K, C.byref(out)))
-    return out.value
-
-
-@functools.lru_cache(maxsize=4096)
-def _matmul_workspace(device, M, N, K):
-    return matmul_w8a8_workspace(M, N, K)
-
-
 def matmul_w8a8(lhs, rhs_packed, out, lhs_scale, rhs_scale, M, N, K, flags, *, bias=None, lhs_stride0=None,
-                rhs_stride0=None, out_stride0=None, workspace=None, stream=None):
+                rhs_stride0=None, out_stride0=None, stream=None):
     """``out[m][n] = sum_k lhs[m][k] rhs[n][k] * lhs_scale[m] * rhs_scale[n] + bias[n]``. Rows of ``lhs`` lie
-    ``K`` rounded up to 16 apart unless told otherwise. Without a ``workspace`` the call takes one
-    from torch's allocator for its own duration where it uses one."""
+    ``K`` rounded up to 16 apart unless told otherwise."""
     device, wide = _device(), -(-K // 16) * 16
-    at = _tensor(lhs, _I8, "lhs", device)
-    if workspace is None and device >= 0 and min(M, N, K) > 0:
-        nbytes = _matmul_workspace(device, M, N, K)
-        if nbytes:
-            workspace = _workspace(nbytes, stream)
     _check(load_library().iree_amd_uk_matmul_w8a8(
-        at, wide if lhs_stride0 is None else lhs_stride0, _tensor(lhs_scale, _F32, "lhs_scale", device),
-        _tensor(rhs_packed, _I8, "rhs_packed", device), 32 * wide if rhs_stride0 is None else rhs_stride0,
+        _tensor(lhs, _I8, "lhs", device), wide if lhs_stride0 is None else lhs_stride0,
+        _tensor(lhs_scale, _F32, "lhs_scale", device), _tensor(rhs_packed, _I8, "rhs_packed", device), 32 * wide if rhs_stride0 is None else rhs_stride0,
         _tensor(rhs_scale, _F32, "rhs_scale", device), _tensor(bias, _F32, "bias", device),
         _tensor(out, _TYPES.get(flags & F.ROWS_TYPE_MASK), "out", device), N if out_stride0 is None else out_stride0, M, N, K,
-        _tensor(workspace, None, "workspace", device), 0 if workspace is None else workspace.nbytes, flags,
-        _stream_on(stream, device)))
+        flags, _stream_on(stream, device)))
 
 
 def moe_route_workspace(tokens, experts):
@@ -99,7 +80,8 @@ _route_workspace = functools.lru_cache(maxsize=4096)(moe_route_workspace)
 def moe_route(logits, expert_ids, expert_weights, offsets, rows, tokens, experts, top_k, flags, *, logits_stride0=None,
               workspace=None, stream=None):
     """The ``top_k`` experts of each token and their weights, and the slots in the order of their
-    experts: ``rows``, those of expert ``e`` at ``offsets[e]`` to ``offsets[e + 1]``."""
+    experts: ``rows``, those of expert ``e`` at ``offsets[e]`` to ``offsets[e + 1]``. Without a ``workspace``
+    the call takes one from torch's allocator for its own duration where it uses one."""
     device = _device()
     at = _tensor(logits, _TYPES.get(flags & F.ROWS_TYPE_MASK), "logits", device)
     if workspace is None and 0 < tokens < 1 << 31 and 0 < experts <= 512:

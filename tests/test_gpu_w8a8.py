@@ -215,6 +215,25 @@ def test_product(cuda, kind, M, N, K):
     _assert_product(kind, M, N, K, bias=(M + N) % 2 == 0)
 
 
+def test_every_tile_of_the_product(cuda):
+    # (which one a call takes follows from estimates: the sizes differ enough to reach all)
+    found = set()
+    for M, N, K in [(12, 3847, 4430), (70, 64, 1600), (6, 8582, 4829), (3, 200, 333), (30, 7279, 4722), (64, 4096, 1024),
+                    (119, 4221, 4564), (35, 8676, 2697), (2040, 779, 4870), (500, 4096, 1000), (2503, 3137, 4914),
+                    (2459, 3251, 4988), (1869, 8463, 3748), (4100, 4100, 1100), (1439, 8757, 4623), (2048, 14336, 4096)]:
+        gen = torch.Generator(device="cuda").manual_seed(M + N)
+        wide = -(-K // 16) * 16
+        lhs = torch.randint(-127, 128, (M, wide), generator=gen, device="cuda", dtype=torch.int8)
+        w = torch.randint(-127, 128, (N, K), generator=gen, device="cuda", dtype=torch.int8)
+        s, t = (torch.rand(n, generator=gen, device="cuda") + 0.5 for n in (M, N))
+        out = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+        iree_amd.matmul_w8a8(lhs, ref.pack(w.cpu()).cuda(), out, s, t, M, N, K, F.ROWS_TYPE_BF16)
+        found.add(iree_amd.last_macro_tile()[:2])
+        assert iree_amd.last_kernel_path() in ("w8a8:few-rows", "w8a8:mfma")
+        ref.assert_near(out, *ref.product(lhs[:, :K], s, w, t))
+    assert len(found) == 9, found
+
+
 def test_product_without_a_sum(cuda):
     # K = 0: the bias, or zeros
     s, bias = torch.ones(40, device="cuda"), torch.arange(40.0, device="cuda")

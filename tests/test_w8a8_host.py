@@ -58,7 +58,7 @@ def test_rows_refuse(status, changes):
 
 
 MATMUL = dict(lhs=ONE, lhs_stride=112, lhs_scale=ONE, rhs=ONE, rhs_stride=112 * 32, rhs_scale=ONE, bias=ONE, out=ONE,
-              out_stride=70, M=5, N=70, K=100, workspace=None, nbytes=0, flags=T, stream=None)
+              out_stride=70, M=5, N=70, K=100, flags=T, stream=None)
 
 
 @pytest.mark.parametrize("status,changes", [
@@ -68,8 +68,7 @@ MATMUL = dict(lhs=ONE, lhs_stride=112, lhs_scale=ONE, rhs=ONE, rhs_stride=112 * 
     (3, dict(rhs=None)), (3, dict(rhs=EIGHT)), (3, dict(rhs_stride=112 * 32 - 16)), (3, dict(rhs_stride=112 * 32 + 8)),
     (3, dict(rhs_stride=(1 << 24) + 16)), (3, dict(lhs_scale=None)), (3, dict(rhs_scale=None)),
     (3, dict(rhs_scale=C.c_void_p(4098))), (3, dict(bias=ODD)), (3, dict(out=None)), (3, dict(out=ODD)),
-    (3, dict(out_stride=69)), (3, dict(nbytes=64)), (3, dict(workspace=EIGHT, nbytes=64)),
-    (3, dict(flags=F.ROWS_TYPE_F32, out=C.c_void_p(4098))),
+    (3, dict(out_stride=69)), (3, dict(flags=F.ROWS_TYPE_F32, out=C.c_void_p(4098))),
 ])
 def test_product_refuses(status, changes):
     assert _call("matmul_w8a8", MATMUL, **changes) == status
@@ -128,9 +127,6 @@ def test_workspaces():
             iree_amd.moe_route_workspace(tokens, experts)
     lib = iree_amd.load_library()
     assert lib.iree_amd_uk_moe_route_workspace(5, 8, None) == 3
-    assert lib.iree_amd_uk_matmul_w8a8_workspace(5, 8, 16, None) == 3
-    for sizes in ((-1, 8, 8), (8, -1, 8), (8, 8, -1), (1 << 31, 8, 8)):
-        assert lib.iree_amd_uk_matmul_w8a8_workspace(*sizes, C.byref(C.c_uint64())) == 3
 
 
 def test_tensors_are_checked():
