@@ -21,7 +21,8 @@ using namespace kv4;
 constexpr int kMostExperts = 512;
 constexpr int kMostBlocks = 256;           // blocks of tokens
 constexpr int kBlockTokens = 16;           // of one, at least
-constexpr int kBlockWaves = 8;
+constexpr int kWaves = 16;                 // of a workgroup
+constexpr int kHeldSlots = 8192;           // of a block whose choices stay in LDS
 constexpr int kOneBlockTokens = 128;       // up to which one workgroup does all
 
 struct RouteArgs {
@@ -60,54 +61,83 @@ __device__ inline uint32_t largest_of_wave(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
 }
 
-// The experts and weights of one token, by a wave. kLogits: a lane's.
+// The experts and weights of two tokens, by a wave, whose steps wait for nothing of each other; the second may be
+// past the last. kLogits: of a token, a lane's. `ids` (or null): the choices of the block's tokens from `first` on, in LDS.
 template <typename T, int kLogits>
-__device__ inline void choose(const MoeRouteArgs& a, int64_t token) {
+__device__ inline void choose(const MoeRouteArgs& a, const int64_t (&token)[2], int64_t last, int64_t first, int16_t* ids) {
   const int lane = threadIdx.x & 63;
-  const char* row = (const char*)a.logits + token * a.logits_stride * (int64_t)(std::is_same<T, float>::value ? 4 : 2);
-  uint32_t order[kLogits];
+  uint32_t order[2][kLogits];
 #pragma unroll
-  for (int i = 0; i < kLogits; ++i) {
-    const int e = i * 64 + lane;
-    order[i] = e < a.experts ? order_of(logit<T>(row, e)) : 0;
-  }
-  float top = 0.f, total = 0.f, mine_logit = 0.f;
-  int mine = -1;
-  for (int k = 0; k < a.top_k; ++k) {
-    uint32_t best = order[0];
-#pragma unroll
-    for (int i = 1; i < kLogits; ++i) best = order[i] > best ? order[i] : best;
-    best = largest_of_wave(best);
-    if (best == 0) break;
-    const float its_logit = value_of(best);
-    if (k == 0) {
-      top = its_logit;
-      if (!a.renormalize) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < kLogits; ++i)
-          if (order[i]) sum += expf(value_of(order[i]) - top);
-#pragma unroll
-        for (int mask = 32; mask; mask >>= 1) sum += __shfl_xor(sum, mask);
-        total = sum;
-      }
-    }
-    if (a.renormalize) total += expf(its_logit - top);
-    bool taken = false;
+  for (int t = 0; t < 2; ++t) {
+    const char* row = (const char*)a.logits + token[t] * a.logits_stride * (int64_t)(std::is_same<T, float>::value ? 4 : 2);
 #pragma unroll
     for (int i = 0; i < kLogits; ++i) {
-      const uint64_t has = taken ? 0 : __ballot(order[i] == best);
-      if (has) {
-        const int l = __builtin_ctzll(has);
-        if (lane == l) order[i] = 0;
-        if (lane == k) mine = i * 64 + l, mine_logit = its_logit;
-        taken = true;
-      }
+      const int e = i * 64 + lane;
+      order[t][i] = e < a.experts && token[t] < last ? order_of(logit<T>(row, e)) : 0;
     }
   }
-  if (lane < a.top_k) {
-    a.expert_ids[token * a.top_k + lane] = mine;
-    a.expert_weights[token * a.top_k + lane] = mine >= 0 ? expf(mine_logit - top) / total : 0.f;
+  float total[2] = {0.f, 0.f}, top[2] = {0.f, 0.f}, mine_logit[2] = {0.f, 0.f};
+  int mine[2] = {-1, -1};
+  if (!a.renormalize) {
+    // (the sum's exponentials before any is taken)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t best = order[t][0];
+#pragma unroll
+      for (int i = 1; i < kLogits; ++i) best = order[t][i] > best ? order[t][i] : best;
+      top[t] = value_of(largest_of_wave(best));
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kLogits; ++i)
+        if (order[t][i]) sum += expf(value_of(order[t][i]) - top[t]);
+#pragma unroll
+      for (int mask = 32; mask; mask >>= 1) sum += __shfl_xor(sum, mask);
+      total[t] = sum;
+    }
+  }
+  for (int k = 0; k < a.top_k; ++k) {
+    uint32_t best[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      best[t] = order[t][0];
+#pragma unroll
+      for (int i = 1; i < kLogits; ++i) best[t] = order[t][i] > best[t] ? order[t][i] : best[t];
+    }
+    best[0] = largest_of_wave(best[0]);
+    best[1] = largest_of_wave(best[1]);
+    if (!(best[0] | best[1])) break;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float its_logit = value_of(best[t]);
+      if (k == 0) top[t] = its_logit;
+      int e = best[t] ? -1 : -2;            // (-2: none is left)
+#pragma unroll
+      for (int i = 0; i < kLogits; ++i) {
+        const uint64_t has = __ballot(order[t][i] == best[t]);
+        if (e == -1 && has) {
+          const int l = __builtin_ctzll(has);
+          e = i * 64 + l;
+          if (lane == l) order[t][i] = 0;
+        }
+      }
+      if (lane == k && e >= 0) mine[t] = e, mine_logit[t] = its_logit;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    if (token[t] >= last) continue;
+    const float p = lane < a.top_k && mine[t] >= 0 ? expf(mine_logit[t] - top[t]) : 0.f;
+    if (a.renormalize) {
+      float sum = p;
+#pragma unroll
+      for (int mask = 32; mask; mask >>= 1) sum += __shfl_xor(sum, mask);
+      total[t] = sum;
+    }
+    if (lane < a.top_k) {
+      a.expert_ids[token[t] * a.top_k + lane] = mine[t];
+      a.expert_weights[token[t] * a.top_k + lane] = mine[t] >= 0 ? p / total[t] : 0.f;
+      if (ids) ids[(token[t] - first) * a.top_k + lane] = (int16_t)mine[t];
+    }
   }
 }
 
@@ -121,22 +151,32 @@ __device__ inline uint64_t same_expert(int e, int bits) {
   return same;
 }
 
-// Places of the slots of a block's tokens. places: [waves][experts] in LDS; first[e]: the place of the
-// block's first slot of expert e, in LDS.
+// Slots of a block in the waves' shares of it, one after the other.
+struct Share { int begin, end; };
 template <int kWaves>
-__device__ inline void place(const MoeRouteArgs& a, int64_t first_slot, int slots, int* places, const int* first) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, experts = a.experts;
-  const int share = (int)ceil_div(ceil_div(slots, kWaves), 64) * 64;
-  const int begin = min(wave * share, slots), end = min(begin + share, slots);
-  for (int i = threadIdx.x; i < kWaves * experts; i += kWaves * 64) places[i] = 0;
-  __syncthreads();
-  for (int i = begin + lane; i < end; i += 64) {
-    const int e = a.expert_ids[first_slot + i];
-    if (e >= 0) atomicAdd(&places[wave * experts + e], 1);
+__device__ inline Share share_of_wave(int slots) {
+  const int share = (int)ceil_div(ceil_div(slots, kWaves), 64) * 64, begin = min((int)(threadIdx.x >> 6) * share, slots);
+  return {begin, min(begin + share, slots)};
+}
+
+// Counts of the waves' shares, [waves][experts] in LDS, which is zeros. id(i): the expert of slot i of the block.
+template <int kWaves, typename Id>
+__device__ inline void count_shares(Share share, int experts, int* counts, Id id) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int i = share.begin + lane; i < share.end; i += 64) {
+    const int e = id(i);
+    if (e >= 0) atomicAdd(&counts[wave * experts + e], 1);
   }
-  __syncthreads();
+}
+
+// Places of a block's slots: counts become the places of the waves' first slots, of which the block's begin at
+// first[e].
+template <int kWaves, typename Id>
+__device__ inline void place(const MoeRouteArgs& a, int64_t first_slot, Share share, int* places, const int* first, Id id) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, experts = a.experts;
   for (int e = threadIdx.x; e < experts; e += kWaves * 64) {
     int at = first[e];
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const int n = places[w * experts + e];
       places[w * experts + e] = at;
@@ -145,8 +185,8 @@ __device__ inline void place(const MoeRouteArgs& a, int64_t first_slot, int slot
   }
   __syncthreads();
   const int bits = 32 - __builtin_clz(experts | 1);
-  for (int i = begin; i < end; i += 64) {
-    const int e = i + lane < end ? a.expert_ids[first_slot + i + lane] : -1;
+  for (int i = share.begin; i < share.end; i += 64) {
+    const int e = i + lane < share.end ? id(i + lane) : -1;
     const uint64_t same = same_expert(e, bits);
     const int before = __popcll(same & ((1ull << lane) - 1));
     int at = 0;
@@ -181,58 +221,71 @@ __device__ inline int first_places(int* count, int experts) {
 
 // kAll: one workgroup does all. Else only the choices and the counts of a block.
 template <typename T, int kLogits, bool kAll>
-__global__ __launch_bounds__(kAll ? 1024 : kBlockWaves * 64) void moe_route_kernel(RouteArgs args) {
-  constexpr int kWaves = kAll ? 16 : kBlockWaves;
+__global__ __launch_bounds__(kWaves * 64) void moe_route_kernel(RouteArgs args) {
+  constexpr int kThreads = kWaves * 64;
   const MoeRouteArgs& a = args.r;
-  extern __shared__ int memory[];
-  int* const count = memory;                 // [experts], then (kAll) places [waves][experts]
-  const int wave = threadIdx.x >> 6, experts = a.experts;
+  extern __shared__ int memory[];            // counts [waves][experts], (kAll) of all [experts]
+  __shared__ int16_t ids[kHeldSlots];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), experts = a.experts;
   const int64_t first = (int64_t)blockIdx.x * args.block_tokens;
   const int64_t last = min(first + args.block_tokens, a.tokens);
-  for (int64_t token = first + wave; token < last; token += kWaves) choose<T, kLogits>(a, token);
-  for (int e = threadIdx.x; e < experts; e += kWaves * 64) count[e] = 0;
-  __syncthreads();                           // (the choices are read below, by other waves of the workgroup)
   const int64_t first_slot = first * a.top_k;
-  const int64_t slots = (last - first) * a.top_k;
-  for (int64_t i = threadIdx.x; i < slots; i += kWaves * 64) {
-    const int e = a.expert_ids[first_slot + i];
-    if (e >= 0) atomicAdd(&count[e], 1);
-  }
+  const int slots = (int)((last - first) * a.top_k);
+  const bool held = slots <= kHeldSlots;     // (without its workspace one block may have any number of tokens)
+  for (int i = threadIdx.x; i < kWaves * experts; i += kThreads) memory[i] = 0;
+  for (int64_t token = first + wave; token < last; token += 2 * kWaves)
+    choose<T, kLogits>(a, {token, token + kWaves}, last, first, held ? ids : nullptr);
+  __syncthreads();                           // (the choices are read below, by other waves of the workgroup)
+  const Share share = share_of_wave<kWaves>(slots);
+  auto id = [&](int i) { return held ? (int)ids[i] : a.expert_ids[first_slot + i]; };
+  count_shares<kWaves>(share, experts, memory, id);
   __syncthreads();
-  if constexpr (!kAll) {
-    for (int e = threadIdx.x; e < experts; e += kWaves * 64) args.counts[(int64_t)blockIdx.x * experts + e] = count[e];
-  } else {
+  int* const count = memory + kWaves * experts;
+  for (int e = threadIdx.x; e < experts; e += kThreads) {
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum += memory[w * experts + e];
+    if constexpr (kAll) count[e] = sum;
+    else args.counts[(int64_t)blockIdx.x * experts + e] = sum;
+  }
+  if constexpr (kAll) {
     __shared__ int all;
+    __syncthreads();
     if (wave == 0) {
       const int n = first_places(count, experts);
       if (threadIdx.x == 0) all = n;
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += kWaves * 64) a.offsets[e] = count[e];
+    for (int e = threadIdx.x; e < experts; e += kThreads) a.offsets[e] = count[e];
     if (threadIdx.x == 0) a.offsets[experts] = all;
-    for (int64_t i = all + threadIdx.x; i < slots; i += kWaves * 64) a.rows[i] = -1;
-    place<kWaves>(a, 0, (int)slots, count + experts, count);
+    for (int64_t i = all + threadIdx.x; i < slots; i += kThreads) a.rows[i] = -1;
+    place<kWaves>(a, 0, share, memory, count, id);
   }
 }
 
 // Second launch: a block's slots to their places.
-__global__ __launch_bounds__(kBlockWaves * 64) void moe_route_place_kernel(RouteArgs args) {
-  constexpr int kWaves = kBlockWaves, kThreads = kWaves * 64;
+__global__ __launch_bounds__(kWaves * 64) void moe_route_place_kernel(RouteArgs args) {
+  constexpr int kThreads = kWaves * 64;
   const MoeRouteArgs& a = args.r;
-  extern __shared__ int memory[];
+  extern __shared__ int memory[];            // counts [waves][experts], then of all and of the blocks before
   const int experts = a.experts;
-  int* const first = memory;                 // [experts]: of all, then of the block
-  int* const before = memory + experts;      // [experts]: counts of the blocks before; then places [waves][experts]
+  int* const first = memory + kWaves * experts;
+  int* const before = first + experts;
   __shared__ int all;
-  for (int e = threadIdx.x; e < experts; e += kThreads) first[e] = before[e] = 0;
+  for (int i = threadIdx.x; i < (kWaves + 2) * experts; i += kThreads) memory[i] = 0;
+  const int64_t first_token = (int64_t)blockIdx.x * args.block_tokens, first_slot = first_token * a.top_k;
+  const int slots = (int)(min((int64_t)args.block_tokens, a.tokens - first_token) * a.top_k);
+  const Share share = share_of_wave<kWaves>(slots);
+  auto id = [&](int i) { return a.expert_ids[first_slot + i]; };
   __syncthreads();
-  // (experts side by side, and as many shares of the blocks as there are threads for)
+  count_shares<kWaves>(share, experts, memory, id);
+  // (experts side by side, and as many parts of the blocks as there are threads for)
   const int width = experts <= 64 ? 64 : experts <= 128 ? 128 : experts <= 256 ? 256 : 512;
-  const int shares = kThreads / width, e = threadIdx.x % width;
+  const int parts = kThreads / width, e = threadIdx.x % width;
   if (e < experts) {
     int mine = 0, total = 0;
 #pragma unroll 8
-    for (int b = threadIdx.x / width; b < args.blocks; b += shares) {
+    for (int b = threadIdx.x / width; b < args.blocks; b += parts) {
       const int n = args.counts[(int64_t)b * experts + e];
       mine += b < (int)blockIdx.x ? n : 0;
       total += n;
@@ -247,28 +300,26 @@ __global__ __launch_bounds__(kBlockWaves * 64) void moe_route_place_kernel(Route
   }
   __syncthreads();
   if (blockIdx.x == 0) {
-    for (int e = threadIdx.x; e < experts; e += kThreads) a.offsets[e] = first[e];
+    for (int i = threadIdx.x; i < experts; i += kThreads) a.offsets[i] = first[i];
     if (threadIdx.x == 0) a.offsets[experts] = all;
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < experts; e += kThreads) first[e] += before[e];
-  const int64_t slots = a.tokens * a.top_k;
-  for (int64_t i = all + (int64_t)blockIdx.x * kThreads + threadIdx.x; i < slots; i += (int64_t)args.blocks * kThreads)
+  for (int64_t i = all + (int64_t)blockIdx.x * kThreads + threadIdx.x; i < a.tokens * a.top_k;
+       i += (int64_t)args.blocks * kThreads)
     a.rows[i] = -1;
   __syncthreads();
-  const int64_t first_token = (int64_t)blockIdx.x * args.block_tokens;
-  const int64_t tokens = min((int64_t)args.block_tokens, a.tokens - first_token);
-  place<kWaves>(a, first_token * a.top_k, (int)(tokens * a.top_k), before, first);
+  for (int i = threadIdx.x; i < experts; i += kThreads) first[i] += before[i];
+  __syncthreads();
+  place<kWaves>(a, first_slot, share, memory, first, id);
 }
 
 template <typename T, int kLogits>
 int launch_choose(const RouteArgs& args, hipStream_t s) {
   const int experts = args.r.experts;
   if (args.blocks == 1)
-    hipLaunchKernelGGL((moe_route_kernel<T, kLogits, true>), dim3(1), dim3(1024), (1 + 16) * experts * 4, s, args);
+    hipLaunchKernelGGL((moe_route_kernel<T, kLogits, true>), dim3(1), dim3(kWaves * 64), (kWaves + 1) * experts * 4, s, args);
   else
-    hipLaunchKernelGGL((moe_route_kernel<T, kLogits, false>), dim3((unsigned)args.blocks), dim3(kBlockWaves * 64),
-                       experts * 4, s, args);
+    hipLaunchKernelGGL((moe_route_kernel<T, kLogits, false>), dim3((unsigned)args.blocks), dim3(kWaves * 64),
+                       kWaves * experts * 4, s, args);
   return check_hip(hipGetLastError(), "moe_route launch");
 }
 
@@ -305,9 +356,7 @@ int launch_moe_route(const MoeRouteArgs& a, hipStream_t s) {
   args.blocks = (int)blocks;
   int st = a.type == 3 ? launch_type<float>(args, s) : a.type == 2 ? launch_type<BF16>(args, s) : launch_type<F16>(args, s);
   if (st || blocks == 1) return st;
-  // (the waves' places begin where the counts of the blocks before were)
-  hipLaunchKernelGGL(moe_route_place_kernel, dim3((unsigned)blocks), dim3(kBlockWaves * 64),
-                     (1 + kBlockWaves) * a.experts * 4, s, args);
+  hipLaunchKernelGGL(moe_route_place_kernel, dim3((unsigned)blocks), dim3(kWaves * 64), (kWaves + 2) * a.experts * 4, s, args);
   return check_hip(hipGetLastError(), "moe_route launch");
 }
 
