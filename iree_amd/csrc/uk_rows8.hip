@@ -491,7 +491,20 @@ __global__ __launch_bounds__(kThreads) void quantize_gated_rows_kernel(QuantizeR
     if (wide) {
       gated_row_wide<T, kThreads>(x, up, q, &a.scale[row], cols, shared_wide);
     } else {
-      // One wave has the largest in 64 bits, which is among those near the largest in 32, then all the open codes.
+      // One wave has the largest in 64 bits, which is among those near the largest in 32; the others meanwhile
+      // work out the first values with an open code, and then all the codes.
+      const int items = open_count[1] * kWidth;
+      auto item = [&](int n, int* i, double* y) {
+        *i = open[1][n / kWidth] + n % kWidth;
+        if (*i >= cols) return false;
+        const float g = T::widen(x[*i]), u = T::widen(up[*i]), v = silu_mul_near(g, u) * inverse;
+        if (fabsf(v - __builtin_rintf(v)) < 0.5f - 1.02f * kGatedSlack) return false;
+        *y = silu_mul_wide(g, u);
+        return true;
+      };
+      int first_i = 0;
+      double first_y = 0.0;
+      bool first_is_open = false;
       if (thread < 64) {
         double exact = 0.0;
         for (int n = thread; n < open_count[0] * kWidth; n += 64) {
@@ -502,15 +515,16 @@ __global__ __launch_bounds__(kThreads) void quantize_gated_rows_kernel(QuantizeR
         }
         exact = over_wave(exact, Larger());
         if (thread == 0) shared_wide[0] = exact, a.scale[row] = (float)(exact / 127.0);
+      } else if (thread - 64 < items) {
+        first_is_open = item(thread - 64, &first_i, &first_y);
       }
       __syncthreads();
       const double exact = shared_wide[0];
-      for (int n = thread; n < open_count[1] * kWidth; n += kThreads) {
-        const int i = open[1][n / kWidth] + n % kWidth;
-        if (i >= cols) continue;
-        const float g = T::widen(x[i]), u = T::widen(up[i]), v = silu_mul_near(g, u) * inverse;
-        if (fabsf(v - __builtin_rintf(v)) >= 0.5f - 1.02f * kGatedSlack)
-          q[i] = (int8_t)code_of(silu_mul_wide(g, u), exact);
+      if (first_is_open) q[first_i] = (int8_t)code_of(first_y, exact);
+      for (int n = kThreads - 64 + thread; n < items; n += kThreads) {
+        int i;
+        double y;
+        if (item(n, &i, &y)) q[i] = (int8_t)code_of(y, exact);
       }
     }
     __syncthreads();             // (the lists are used up)
