@@ -826,7 +826,8 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_copy_pages(void* pool, iree_amd_uk_index_t pa
  * multiplied from it, reads as NaN. q has the bits of the formula in 64 bits
  * (products of two values of 16 bits are in it as far as f32 holds them).
  * Rows lie `stride0` elements apart at any alignment of their elements; rows of 8 bits
- * that the products read, 16-byte aligned and whole 16s apart.
+ * that the products read, 16-byte aligned and whole 16s apart. A call with a size of 0
+ * writes nothing (moe_route of no tokens: offsets).
  *===------------------------------------------------------------------------===*/
 #define IREE_AMD_UK_FLAG_ROWS_TYPE_MASK 0xFF
 #define IREE_AMD_UK_FLAG_ROWS_TYPE_F16 0x01
@@ -995,7 +996,7 @@ IREE_AMD_UK_EXPORT const char* iree_amd_uk_last_error(void);
  * caches were split over workgroups, "w8a8:few-rows", "w8a8:mfma" ("" before the first call). A static string. No counterpart in the reference, whose
  * tile-function choice is visible through iree_uk_mmt4d_info only. */
 IREE_AMD_UK_EXPORT const char* iree_amd_uk_last_kernel_path(void);
-/* Rows and columns of the macro tile of the calling thread's last "mmt4d:mfma"
+/* Rows and columns of the macro tile of the calling thread's last "mmt4d:mfma" or "w8a8:..."
  * launch, and the number of slices of K (1: not split); zeros before the first.
  * For tests and callers that tune, as the above. */
 IREE_AMD_UK_EXPORT void iree_amd_uk_last_macro_tile(int32_t* rows, int32_t* cols, int32_t* k_slices);

@@ -64,7 +64,7 @@ __device__ __forceinline__ RowTile find_row_tile(const W8A8Args& a, int64_t tile
       begin = begin < 0 ? 0 : begin;
       end = end > most ? most : end;
     }
-    const int tiles = end > begin ? (int)((uint32_t)(end - begin + height - 1) / (uint32_t)height) : 0;
+    const int tiles = end > begin ? (int)(((uint32_t)(end - begin) + height - 1) / (uint32_t)height) : 0;
     int sum = tiles;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {

@@ -6,6 +6,9 @@
 // feed the matrix cores (packed tiles are in operand order); rows, which lie one after the other,
 // come through the wave's own part of LDS, a quad of lanes fetching the 64 bytes of one row. The sums
 // are integers, so the order of their additions cannot show.
+//
+// One row against 4096 -> 14336 is a stream of 58.7 MB of weights: 11.0 us, 5.4 TB/s (a pass that only reads 117 MB
+// reaches 6.7).
 #include "uk_w8a8.h"
 
 #include <cmath>

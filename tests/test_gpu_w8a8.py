@@ -511,3 +511,83 @@ def test_two_captured_layers_on_two_streams(cuda):
             assert all(torch.equal(a, b) for a, b in zip(layer.results(), want))
         layers[0].run()                      # the program's own work in between
         assert all(torch.equal(a, b) for a, b in zip(layers[0].results(), eager[0]))
+
+
+def _far_rows(rows, stride, K, at):
+    """An otherwise empty matrix of 8 bits with rows at `at`, and those rows."""
+    lhs = torch.zeros(rows, stride, dtype=torch.int8, device="cuda")
+    mine = ref.rows8(_gen(rows), len(at), K)
+    lhs[torch.tensor(at, device="cuda"), :K] = mine.cuda()
+    return lhs, mine
+
+
+@pytest.mark.parametrize("tokens", [24, 500])
+def test_rows_gathered_from_almost_4_gib(cuda, tokens):
+    rows, stride, K, N = 1044000, 4112, 80, 48                 # 4.293e9 bytes
+    at = [0, 522300, rows - 1, rows - 2, 5]
+    lhs, mine = _far_rows(rows, stride, K, at)
+    gen = _gen(1)
+    w, w_scale = ref.rows8(gen, 2, N, K), ref.scales(gen, 2, N)
+    scale = torch.ones(rows, device="cuda")
+    which = torch.arange(tokens) % len(at)
+    half = tokens // 3
+    out = torch.zeros(tokens, N, device="cuda")
+    iree_amd.grouped_matmul_w8a8(lhs, ref.pack(w).cuda(), out, scale, w_scale.cuda(),
+                                 torch.tensor([0, half, tokens], dtype=torch.int32).cuda(), tokens, 2, N, K,
+                                 F.ROWS_TYPE_F32 | F.GROUPED_GATHER, lhs_rows=rows,
+                                 rows=torch.tensor(at, dtype=torch.int32)[which].cuda(), lhs_stride0=stride)
+    for e, part in ((0, slice(0, half)), (1, slice(half, tokens))):
+        p, _ = ref.product(mine[which[part]], torch.ones(len(which[part])), w[e], w_scale[e])
+        ref.assert_near(out[part].cpu(), p, p)
+
+
+def test_a_matrix_of_more_than_4_gib(cuda):
+    rows, stride, K, N = 2200000, 2064, 40, 32                 # 4.5e9 bytes
+    at = [0, 1, 1099999, rows - 1]
+    lhs, mine = _far_rows(rows, stride, K, at)
+    gen = _gen(2)
+    w, w_scale = ref.rows8(gen, N, K), ref.scales(gen, N)
+    out = torch.full((rows, N), 3.0, dtype=torch.float16, device="cuda")
+    iree_amd.matmul_w8a8(lhs, ref.pack(w).cuda(), out, torch.ones(rows, device="cuda"), w_scale.cuda(), rows, N, K,
+                         F.ROWS_TYPE_F16, lhs_stride0=stride)
+    ref.assert_near(out[torch.tensor(at, device="cuda")].cpu(), *ref.product(mine, torch.ones(4), w, w_scale))
+    out[torch.tensor(at, device="cuda")] = 0
+    assert not out.any()
+
+
+@pytest.mark.parametrize("tokens", [3, 400])
+def test_weights_of_more_than_4_gib(cuda, tokens):
+    experts, N, K = 512, 4096, 2304                            # 4.8e9 bytes
+    packed = torch.zeros(experts, N // 32, K // 16, 32, 16, dtype=torch.int8, device="cuda")
+    gen = _gen(3)
+    w, w_scale = ref.rows8(gen, N, K), ref.scales(gen, N)
+    packed[experts - 1] = ref.pack(w).cuda()
+    scale = torch.zeros(experts, N, device="cuda")
+    scale[experts - 1] = w_scale.cuda()
+    lhs, lhs_scale = ref.rows8(gen, tokens, K), ref.scales(gen, tokens)
+    offsets = torch.zeros(experts + 1, dtype=torch.int32, device="cuda")
+    offsets[experts] = tokens
+    out = torch.zeros(tokens, N, device="cuda")
+    iree_amd.grouped_matmul_w8a8(lhs.cuda(), packed, out, lhs_scale.cuda(), scale, offsets, tokens, experts, N, K,
+                                 F.ROWS_TYPE_F32, lhs_rows=tokens)
+    p, _ = ref.product(lhs, lhs_scale, w, w_scale)
+    ref.assert_near(out.cpu(), p, p)
+
+
+def test_a_call_on_another_stream(cuda):
+    gen, M, N, K = _gen(6), 70, 96, 200
+    lhs, lhs_scale, w, w_scale = _product_case(gen, M, N, K)
+    args = [t.cuda() for t in (lhs, ref.pack(w), lhs_scale, w_scale)]
+    out = torch.zeros(M, N, device="cuda")
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    iree_amd.matmul_w8a8(args[0], args[1], out, args[2], args[3], M, N, K, F.ROWS_TYPE_F32, stream=stream)
+    logits = torch.randn(500, 64, generator=gen)
+    on = logits.cuda()
+    ids, weights = torch.zeros(500, 4, dtype=torch.int32, device="cuda"), torch.zeros(500, 4, device="cuda")
+    offsets, rows = torch.zeros(65, dtype=torch.int32, device="cuda"), torch.zeros(2000, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    iree_amd.moe_route(on, ids, weights, offsets, rows, 500, 64, 4, F.ROWS_TYPE_F32, stream=stream)
+    stream.synchronize()
+    ref.assert_near(out.cpu(), *ref.product(lhs[:, :K], lhs_scale, w, w_scale))
+    _assert_route([t.cpu() for t in (ids, weights, offsets, rows)], logits, 4, False)
