@@ -106,6 +106,17 @@ __device__ inline V over_wave(V v, F f) {
   return joined<5>(v, f);
 }
 
+// The joint value of the kWaves (4, 8 or 16) waves of a row, each of which has left its own in LDS.
+template <int kWaves, typename V, typename F>
+__device__ inline V over_waves(const V* shared, F f) {
+  V v = shared[threadIdx.x & (kWaves - 1)];
+  v = joined<0>(v, f);
+  v = joined<1>(v, f);
+  if constexpr (kWaves > 4) v = joined<2>(v, f);
+  if constexpr (kWaves > 8) v = joined<3>(v, f);
+  return v;
+}
+
 // 127 y / top of 8 values as codes: t times `inverse` is added to 1.5 * 2^23 with one rounding, which
 // leaves the code in the last byte; `far` grows to the largest distance from a code.
 __device__ inline u32x2 codes8(const float* t, float inverse, float* far) {
@@ -291,12 +302,8 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(R
       __syncthreads();
       if ((threadIdx.x & 63) == 0) shared_squares[threadIdx.x >> 6] = squares, shared_top[threadIdx.x >> 6] = top;
       __syncthreads();
-      squares = shared_squares[0], top = shared_top[0];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) {
-        squares += shared_squares[w];
-        top = larger(top, shared_top[w]);
-      }
+      squares = over_waves<kWaves>(shared_squares, Sum());
+      top = over_waves<kWaves>(shared_top, Larger());
     }
     const bool finite = top <= kMostFloat;
     const float its_top = scaled_if_tiny<kReps>(t, top), inverse = 127.f / its_top;
@@ -351,9 +358,7 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void quantize_rows_kernel(Quant
       __syncthreads();
       if ((threadIdx.x & 63) == 0) shared_top[threadIdx.x >> 6] = top;
       __syncthreads();
-      top = shared_top[0];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = larger(top, shared_top[w]);
+      top = over_waves<kWaves>(shared_top, Larger());
     }
     const bool finite = top <= kMostFloat;
     const float its_top = scaled_if_tiny<kReps>(t, top), inverse = 127.f / its_top;
@@ -420,10 +425,10 @@ template <typename T, int kThreads, int kReps>
 __global__ __launch_bounds__(kThreads) void quantize_gated_rows_kernel(QuantizeRowsArgs a) {
   constexpr int kWaves = kThreads / 64;
   constexpr bool kAnySize = std::is_same<T, BF16>::value;      // (f16 has none above 2^40)
-  __shared__ float shared_top[kWaves], shared_large[kWaves];
+  __shared__ float shared_top[kWaves];
   __shared__ double shared_wide[kWaves];
   __shared__ int open_count[2], open[2][kMostOpen];      // candidates for the largest, open codes
-  const int thread = threadIdx.x, cols = a.cols;
+  const int thread = threadIdx.x, first_thread = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63), cols = a.cols;
   u32x4 gates[kReps], ups[kReps];
   auto load_row = [&](int64_t of) {
     const uint16_t* x = (const uint16_t*)a.x + of * a.x_stride;
@@ -445,6 +450,10 @@ __global__ __launch_bounds__(kThreads) void quantize_gated_rows_kernel(QuantizeR
     float t[kReps][kWidth], mine[kReps], top = 0.f, large = 0.f;
 #pragma unroll
     for (int r = 0; r < kReps; ++r) {
+      mine[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) t[r][i] = 0.f;
+      if ((r * kThreads + first_thread) * kWidth >= cols) continue;      // (a wave behind the row's end)
       float g[kWidth], u[kWidth];
       __builtin_amdgcn_sched_barrier(0);      // (one after the other, in the same registers)
       widen8<T>(gates[r], g);
@@ -455,29 +464,25 @@ __global__ __launch_bounds__(kThreads) void quantize_gated_rows_kernel(QuantizeR
         if constexpr (kAnySize) large = fmaxf(fmaxf(large, fabsf(g[i])), fabsf(u[i]));
       }
       // (a gate or factor that is not finite gives a product that is not either)
-      mine[r] = 0.f;
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) mine[r] = larger(mine[r], fabsf(t[r][i]));
       top = larger(top, mine[r]);
     }
     if (kAhead && row + gridDim.x < a.rows) load_row(row + gridDim.x);
+    // (sizes that f32 does not see through count as not finite here)
+    if (kAnySize && !(large <= kLarge)) top = __builtin_nanf("");
     top = over_wave(top, Larger());
-    if constexpr (kAnySize) large = over_wave(large, Larger());
-    if ((thread & 63) == 0) shared_top[thread >> 6] = top, shared_large[thread >> 6] = large;
+    if ((thread & 63) == 0) shared_top[thread >> 6] = top;
     if (thread < 2) open_count[thread] = 0;
     __syncthreads();
-    top = shared_top[0], large = shared_large[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-      top = larger(top, shared_top[w]);
-      if constexpr (kAnySize) large = larger(large, shared_large[w]);
-    }
-    bool wide = !(top <= kLarge * kLarge) || top < 1.f / kLarge || (kAnySize && !(large <= kLarge));
+    top = over_waves<kWaves>(shared_top, Larger());
+    bool wide = !(top <= kLarge * kLarge) || top < 1.f / kLarge;
     const float from = top * (1.f - 1.f / 131072), inverse = 127.f / top;
     if (!wide) {
 #pragma unroll
       for (int r = 0; r < kReps; ++r) {
         const int at = (r * kThreads + thread) * kWidth;
+        if ((r * kThreads + first_thread) * kWidth >= cols) continue;
         float far = 0.f;
         __builtin_amdgcn_sched_barrier(0);
         const u32x2 w = codes8(t[r], inverse, &far);
