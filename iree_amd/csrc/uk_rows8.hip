@@ -228,6 +228,19 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(R
     }
   };
   if (token < a.tokens) load_row(token);
+  // (the weight, too, is on its way before it is needed, and for all rows of a workgroup, where there is room for it)
+  constexpr bool kHeld = kReps <= 2;
+  u32x4 weight[kHeld ? kReps : 1];
+  auto load_weight = [&](int r) {
+    const int at = (r * kThreads + thread) * kWidth;
+    return at < dim ? load8((const uint16_t*)a.weight, at, dim) : u32x4{0, 0, 0, 0};
+  };
+  if constexpr (kHeld) {
+    if (a.weight) {
+#pragma unroll
+      for (int r = 0; r < kReps; ++r) weight[r] = load_weight(r);
+    }
+  }
   for (; token < a.tokens; token += step) {
     u32x4 added[kOne ? kReps : 1], bits[kReps];
 #pragma unroll
@@ -282,14 +295,14 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(R
     double squares = 0.0;
 #pragma unroll
     for (int r = 0; r < kReps; ++r) {
-      const int at = (r * kThreads + thread) * kWidth;
       __builtin_amdgcn_sched_barrier(0);
       widen8<T>(bits[r], t[r]);
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) squares = fma((double)t[r][i], (double)t[r][i], squares);
-      if (a.weight && at < dim) {
+      if (a.weight) {
         float w[kWidth];
-        widen8<T>(load8((const uint16_t*)a.weight, at, dim), w);
+        if constexpr (kHeld) widen8<T>(weight[r], w);
+        else widen8<T>(load_weight(r), w);
 #pragma unroll
         for (int i = 0; i < kWidth; ++i) t[r][i] *= w[i];
       }
