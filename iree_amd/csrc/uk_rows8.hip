@@ -8,11 +8,11 @@
 //
 // A row stays in the registers of the threads that share it: a wave has up to 1024 elements, 256 threads
 // up to 4096, 512 up to 8192, 1024 the longer ones (4096 elements, 4099 rows of bf16: a wave 47 us, two 35, four 28,
-// eight 27). Norms of 4099 x 4096 bf16, 117 MB, take 23.5 us on the device (5.0 TB/s, 10 of them vector
-// instructions), eight weighted addends of 2048 x 4096, 176 MB, 37 us (4.8 TB/s, 16 of them vector
-// instructions: the sums in 64 bits), one row 3.2; the gate of 2048 x 14336, 147 MB, 38.7: 25 of them vector
-// instructions, which the one workgroup of a compute unit does not hide behind its barriers (two of 512
-// threads with twice the elements each: 50 us, more registers than two have room for).
+// eight 27, before the weight was held and the next row on its way). Norms of 4099 x 4096 bf16, 117 MB, take 25.1 us, 22.8 on
+// the device (5.1 TB/s, 11 of them vector instructions), eight weighted addends of 2048 x 4096, 176 MB, 36.1 and
+// 34.6 (16 of them vector instructions: the sums in 64 bits), one row 3.2; the gate of 2048 x 14336,
+// 147 MB, 36.0: 20 of them vector instructions, which the one workgroup of a compute unit does not hide behind its
+// barriers (two of 512 threads with twice the elements each: 50 us, more registers than two have room for).
 #include "uk_common.h"
 #include "uk_kv4.h"
 

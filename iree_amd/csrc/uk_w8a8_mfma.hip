@@ -17,7 +17,7 @@
 // the tiles, in panels of a few tiles of rows, so that the operands its tiles share are in its L2.
 //
 // 4096^3 with bf16 results 58.7 us (2.34 POP/s, one round of 128 x 256, two to a compute unit; 59.6 on 256 x 256), by
-// expert 4096 tokens x 8 of 64 experts, 4096 -> 3584, 549 us: 1.75 POP/s, 2.0 with the rows that fill the last
+// expert 4096 tokens x 8 of 64 experts, 4096 -> 3584, 544 to 555 us: 1.75 POP/s, 2.0 with the rows that fill the last
 // tile of each expert, which is what several rounds sustain (2048 x 14336 x 4096 116 us, 2.07 POP/s). A last tile of
 // 256 rows worked on at half its height where that suffices took 550 us and is not kept. 500 x 4096 x
 // 14336 takes 38.8 us on 256 workgroups of 64 x 128, whose 2.75 MB of operands each come in at 71 GB/s.
