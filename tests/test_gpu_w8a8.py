@@ -591,3 +591,43 @@ def test_a_call_on_another_stream(cuda):
     stream.synchronize()
     ref.assert_near(out.cpu(), *ref.product(lhs[:, :K], lhs_scale, w, w_scale))
     _assert_route([t.cpu() for t in (ids, weights, offsets, rows)], logits, 4, False)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 70, 100), (300, 513, 640), (1, 1000, 2048)])
+def test_product_on_what_pack_makes_and_beside_the_integer_one(cuda, M, N, K):
+    gen = _gen(M)
+    lhs, w = ref.rows8(gen, M, K) // 8, ref.rows8(gen, N, K)
+    high, wide = -(-N // 32), -(-K // 16)
+    packed = torch.full((high, wide, 32, 16), 7, dtype=torch.int8, device="cuda")
+    iree_amd.pack(w.cuda(), packed, N, K, high, wide, 32, 16, 0, F.PACK_TYPE_I8I8)
+    assert torch.equal(packed.cpu(), ref.pack(w))
+    rows = torch.zeros(M, wide * 16, dtype=torch.int8)
+    rows[:, :K] = lhs
+    one = torch.ones(max(M, N), device="cuda")
+    out = torch.zeros(M, N, device="cuda")
+    iree_amd.matmul_w8a8(rows.cuda(), packed, out, one, one, M, N, K, F.ROWS_TYPE_F32)
+    whole = torch.zeros(M, high * 32, dtype=torch.int32, device="cuda")
+    iree_amd.matmul_data_tiled(lhs.cuda(), w.T.contiguous().cuda(), whole.view(-1)[:M * N], M, N, K, F.MMT4D_TYPE_S8S8S32)
+    assert torch.equal(out, whole.view(-1)[:M * N].view(M, N).float())        # (sums below 2^24)
+
+
+@pytest.mark.parametrize("counts", [[3, 0, 17], [200, 90, 0]])
+def test_grouped_product_takes_strides(cuda, counts):
+    gen, N, K, positions = _gen(12), 70, 100, sum(counts)
+    lhs, lhs_scale, w, _ = _product_case(gen, positions, 1, K)
+    w, w_scale = ref.rows8(gen, 3, N, K), ref.scales(gen, 3, N)
+    big = torch.full((positions, 144), 99, dtype=torch.int8)
+    big[:, 16:128] = lhs
+    spread = torch.full((3, 4 * 3648), 55, dtype=torch.int8)               # outer columns 3648 bytes apart, four's room
+    packed = ref.pack(w).view(3, 3, 3584)
+    for c in range(3):
+        spread[:, c * 3648:c * 3648 + 3584] = packed[:, c]
+    offsets = torch.tensor([0] + counts).cumsum(0).int()
+    out = torch.full((positions, 75), 5.0, dtype=torch.bfloat16, device="cuda")
+    iree_amd.grouped_matmul_w8a8(big.cuda().view(-1)[16:], spread.cuda(), out.view(-1)[2:], lhs_scale.cuda(), w_scale.cuda(),
+                                 offsets.cuda(), positions, 3, N, K, F.ROWS_TYPE_BF16, lhs_rows=positions, lhs_stride0=144,
+                                 rhs_stride0=3648, rhs_expert_stride=4 * 3648, out_stride0=75)
+    p = torch.stack([v for _, v in ref.grouped(lhs[:, :K], lhs_scale, w, w_scale, offsets, torch.arange(positions), False,
+                                               False, 1, positions)])
+    ref.assert_near(out.cpu()[:, 2:72], p, p)
+    assert (out[:, :2] == 5).all() and (out[:, 72:] == 5).all()
