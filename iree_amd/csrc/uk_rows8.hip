@@ -6,7 +6,7 @@
 // and the codes need neither the sum of squares nor its root: largest value and sum of
 // squares come out of one reduction, and a row is read once.
 //
-// A row stays in the registers of the threads that share it: a wave has up to 1024 elements, 256 threads
+// A row stays in the registers of the threads that share it: 16 lanes have up to 128 elements, a wave up to 1024, 256 threads
 // up to 4096, 512 up to 8192, 1024 the longer ones (4096 elements, 4099 rows of bf16: a wave 47 us, two 35, four 28,
 // eight 27, before the weight was held and the next row on its way). Norms of 4099 x 4096 bf16, 117 MB, take 25.1 us, 22.8 on
 // the device (5.1 TB/s, 11 of them vector instructions), eight weighted addends of 2048 x 4096, 176 MB, 36.1 and
@@ -96,22 +96,27 @@ __device__ inline double joined(double v, F f) {
   partners<kStep>((uint32_t)(u >> 32), &c, &d);
   return f(__builtin_bit_cast(double, (uint64_t)c << 32 | a), __builtin_bit_cast(double, (uint64_t)d << 32 | b));
 }
-template <typename V, typename F>
-__device__ inline V over_wave(V v, F f) {
+// Over the lanes of a wave, or its groups of 16 lanes.
+template <int kLanes, typename V, typename F>
+__device__ inline V over_lanes(V v, F f) {
+  static_assert(kLanes == 16 || kLanes == 64, "a group of lanes");
   v = joined<0>(v, f);
   v = joined<1>(v, f);
   v = joined<2>(v, f);
   v = joined<3>(v, f);
-  v = joined<4>(v, f);
-  return joined<5>(v, f);
+  if constexpr (kLanes == 64) {
+    v = joined<4>(v, f);
+    v = joined<5>(v, f);
+  }
+  return v;
 }
 
-// The joint value of the kWaves (4, 8 or 16) waves of a row, each of which has left its own in LDS.
+// The joint value of the kWaves (2, 4, 8 or 16) waves of a row, each of which has left its own in LDS.
 template <int kWaves, typename V, typename F>
 __device__ inline V over_waves(const V* shared, F f) {
   V v = shared[threadIdx.x & (kWaves - 1)];
   v = joined<0>(v, f);
-  v = joined<1>(v, f);
+  if constexpr (kWaves > 2) v = joined<1>(v, f);
   if constexpr (kWaves > 4) v = joined<2>(v, f);
   if constexpr (kWaves > 8) v = joined<3>(v, f);
   return v;
@@ -201,7 +206,9 @@ constexpr int kBlockOf = kThreads < 256 ? 256 : kThreads;
 // Which row of its workgroup's a wave has a part of.
 template <int kThreads>
 __device__ inline int row_of_wave() {
-  return kThreads < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads) : 0;
+  if constexpr (kThreads >= 256) return 0;
+  else if constexpr (kThreads >= 64) return __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+  else return threadIdx.x / kThreads;
 }
 
 // Rows of a launch are dealt to its workgroups in turn, kRows at a time; while a row is worked on, the next
@@ -210,7 +217,7 @@ __device__ inline int row_of_wave() {
 // kOne: one addend without a weight.
 template <typename T, bool kOne, int kThreads, int kReps>
 __global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(RmsNormQuantizeArgs a) {
-  constexpr int kRows = kBlockOf<kThreads> / kThreads, kWaves = kThreads / 64;
+  constexpr int kRows = kBlockOf<kThreads> / kThreads, kLanes = kThreads < 64 ? kThreads : 64, kWaves = kThreads / kLanes;
   __shared__ double shared_squares[kWaves];
   __shared__ float shared_top[kWaves];
   const int thread = threadIdx.x % kThreads, dim = a.dim;
@@ -227,7 +234,9 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(R
       next_bits[r] = residual && at < dim ? load8(residual, at, dim) : u32x4{0, 0, 0, 0};
     }
   };
-  if (token < a.tokens) load_row(token);
+  // (longer rows leave no room for a second one)
+  constexpr bool kAhead = kReps <= 2;
+  if (kAhead && token < a.tokens) load_row(token);
   // (the weight, too, is on its way before it is needed, and for all rows of a workgroup, where there is room for it)
   constexpr bool kHeld = kReps <= 2;
   u32x4 weight[kHeld ? kReps : 1];
@@ -242,13 +251,14 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(R
     }
   }
   for (; token < a.tokens; token += step) {
+    if constexpr (!kAhead) load_row(token);
     u32x4 added[kOne ? kReps : 1], bits[kReps];
 #pragma unroll
     for (int r = 0; r < kReps; ++r) {
       if constexpr (kOne) added[r] = next_added[r];
       bits[r] = next_bits[r];
     }
-    if (token + step < a.tokens) load_row(token + step);
+    if (kAhead && token + step < a.tokens) load_row(token + step);
     // The sum, rounded to its type.
 #pragma unroll
     for (int r = 0; r < kReps; ++r) {
@@ -309,8 +319,8 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(R
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) top = larger(top, fabsf(t[r][i]));
     }
-    squares = over_wave(squares, Sum());
-    top = over_wave(top, Larger());
+    squares = over_lanes<kLanes>(squares, Sum());
+    top = over_lanes<kLanes>(top, Larger());
     if constexpr (kWaves > 1) {
       __syncthreads();
       if ((threadIdx.x & 63) == 0) shared_squares[threadIdx.x >> 6] = squares, shared_top[threadIdx.x >> 6] = top;
@@ -343,7 +353,7 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(R
 
 template <typename T, int kThreads, int kReps>
 __global__ __launch_bounds__(kBlockOf<kThreads>) void quantize_rows_kernel(QuantizeRowsArgs a) {
-  constexpr int kRows = kBlockOf<kThreads> / kThreads, kWaves = kThreads / 64;
+  constexpr int kRows = kBlockOf<kThreads> / kThreads, kLanes = kThreads < 64 ? kThreads : 64, kWaves = kThreads / kLanes;
   __shared__ float shared_top[kWaves];
   const int thread = threadIdx.x % kThreads, cols = a.cols;
   const int64_t step = (int64_t)gridDim.x * kRows;
@@ -366,7 +376,7 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void quantize_rows_kernel(Quant
     for (int r = 0; r < kReps; ++r)
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) top = larger(top, fabsf(t[r][i]));
-    top = over_wave(top, Larger());
+    top = over_lanes<kLanes>(top, Larger());
     if constexpr (kWaves > 1) {
       __syncthreads();
       if ((threadIdx.x & 63) == 0) shared_top[threadIdx.x >> 6] = top;
@@ -421,7 +431,7 @@ __device__ inline void gated_row_wide(const uint16_t* x, const uint16_t* up, int
     const bool finite = fabsf(g) <= kMostFloat && fabsf(u) <= kMostFloat && y <= kMostFloat;
     top = Larger()(top, finite ? y : (double)__builtin_inff());
   }
-  top = over_wave(top, Larger());
+  top = over_lanes<64>(top, Larger());
   __syncthreads();
   if ((thread & 63) == 0) shared[thread >> 6] = top;
   __syncthreads();
@@ -484,11 +494,11 @@ __global__ __launch_bounds__(kThreads) void quantize_gated_rows_kernel(QuantizeR
     if (kAhead && row + gridDim.x < a.rows) load_row(row + gridDim.x);
     // (sizes that f32 does not see through count as not finite here)
     if (kAnySize && !(large <= kLarge)) top = __builtin_nanf("");
-    top = over_wave(top, Larger());
+    top = over_lanes<64>(top, Larger());
     if ((thread & 63) == 0) shared_top[thread >> 6] = top;
     if (thread < 2) open_count[thread] = 0;
     __syncthreads();
-    top = over_waves<kWaves>(shared_top, Larger());
+    if constexpr (kWaves > 1) top = over_waves<kWaves>(shared_top, Larger());
     bool wide = !(top <= kLarge * kLarge) || top < 1.f / kLarge;
     const float from = top * (1.f - 1.f / 131072), inverse = 127.f / top;
     if (!wide) {
@@ -537,7 +547,7 @@ __global__ __launch_bounds__(kThreads) void quantize_gated_rows_kernel(QuantizeR
           const float g = T::widen(x[i]), u = T::widen(up[i]);
           if (fabsf(silu_mul_near(g, u)) >= from) exact = Larger()(exact, fabs(silu_mul_wide(g, u)));
         }
-        exact = over_wave(exact, Larger());
+        exact = over_lanes<64>(exact, Larger());
         if (thread == 0) shared_wide[0] = exact, a.scale[row] = (float)(exact / 127.0);
       } else if (thread - 64 < items) {
         first_is_open = item(thread - 64, &first_i, &first_y);
@@ -563,12 +573,14 @@ unsigned grid_of(int64_t rows, int rows_of_block, int block, int waves) {
 }
 
 // Calls launch(threads, reps) with the first of the shapes (threads that share a row, times 8 elements of
-// each) that holds a row of `dim` elements and is not left out by `from`.
+// each) that holds a row of `dim` elements.
+#define UK_ROW_SHAPE(threads, reps) \
+  if (dim <= (threads) * (reps) * kWidth) return launch(std::integral_constant<int, threads>(), std::integral_constant<int, reps>())
+constexpr const char* kTooLong = "rows of more than 65536 elements";
+// (norms of 2^24 elements of bf16: rows of 64 with 16 threads 37 us, with a wave 118)
 template <typename Launch>
-int with_row_shape(int64_t dim, int64_t from, Launch launch) {
-#define UK_ROW_SHAPE(threads, reps)                                     \
-  if (dim <= (threads) * (reps) * kWidth && (threads) * (reps) >= from) \
-  return launch(std::integral_constant<int, threads>(), std::integral_constant<int, reps>())
+int with_row_shape(int64_t dim, Launch launch) {
+  UK_ROW_SHAPE(16, 1);
   UK_ROW_SHAPE(64, 1);
   UK_ROW_SHAPE(64, 2);
   UK_ROW_SHAPE(256, 1);
@@ -577,41 +589,69 @@ int with_row_shape(int64_t dim, int64_t from, Launch launch) {
   UK_ROW_SHAPE(1024, 2);
   UK_ROW_SHAPE(1024, 4);
   UK_ROW_SHAPE(1024, 8);
-#undef UK_ROW_SHAPE
-  return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "rows of more than 65536 elements");
+  return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, kTooLong);
 }
+// (more waves where each row needs more loads: four addends of 2048 x 8192 28.9 us, with 512 threads 37.7)
+template <typename Launch>
+int with_row_shape_of_addends(int64_t dim, Launch launch) {
+  UK_ROW_SHAPE(16, 1);
+  UK_ROW_SHAPE(64, 1);
+  UK_ROW_SHAPE(64, 2);
+  UK_ROW_SHAPE(256, 1);
+  UK_ROW_SHAPE(256, 2);
+  UK_ROW_SHAPE(1024, 1);
+  UK_ROW_SHAPE(1024, 2);
+  UK_ROW_SHAPE(1024, 4);
+  UK_ROW_SHAPE(1024, 8);
+  return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, kTooLong);
+}
+// (gated rows have a workgroup each: 2^24 elements in rows of 64 with one wave 181 us, with four 460)
+template <typename Launch>
+int with_gated_row_shape(int64_t dim, Launch launch) {
+  UK_ROW_SHAPE(64, 1);
+  UK_ROW_SHAPE(64, 2);
+  UK_ROW_SHAPE(128, 2);
+  UK_ROW_SHAPE(256, 2);
+  UK_ROW_SHAPE(512, 2);
+  UK_ROW_SHAPE(1024, 2);
+  UK_ROW_SHAPE(1024, 4);
+  UK_ROW_SHAPE(1024, 8);
+  return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, kTooLong);
+}
+#undef UK_ROW_SHAPE
 
 }  // namespace
 
-int launch_rms_norm_quantize(const RmsNormQuantizeArgs& a, hipStream_t s) {
-  return with_row_shape(a.dim, 0, [&](auto threads, auto reps) {
+template <bool kOne>
+static int launch_norm(const RmsNormQuantizeArgs& a, hipStream_t s) {
+  auto launch = [&](auto threads, auto reps) {
     constexpr int kThreads = decltype(threads)::value, kReps = decltype(reps)::value, kBlock = kBlockOf<kThreads>;
     const dim3 grid(grid_of(a.tokens, kBlock / kThreads, kBlock, 8));
-    const bool one = a.addends == 1 && !a.factors;
-    if (a.bf16 && one)
-      hipLaunchKernelGGL((rms_norm_quantize_kernel<BF16, true, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-    else if (a.bf16)
-      hipLaunchKernelGGL((rms_norm_quantize_kernel<BF16, false, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-    else if (one)
-      hipLaunchKernelGGL((rms_norm_quantize_kernel<F16, true, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-    else
-      hipLaunchKernelGGL((rms_norm_quantize_kernel<F16, false, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+    if (a.bf16) hipLaunchKernelGGL((rms_norm_quantize_kernel<BF16, kOne, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+    else hipLaunchKernelGGL((rms_norm_quantize_kernel<F16, kOne, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
     return check_hip(hipGetLastError(), "rms_norm_quantize launch");
-  });
+  };
+  if constexpr (kOne) return with_row_shape(a.dim, launch);
+  else return with_row_shape_of_addends(a.dim, launch);
+}
+int launch_rms_norm_quantize(const RmsNormQuantizeArgs& a, hipStream_t s) {
+  return a.addends == 1 && !a.factors ? launch_norm<true>(a, s) : launch_norm<false>(a, s);
 }
 
 int launch_quantize_rows(const QuantizeRowsArgs& a, hipStream_t s) {
-  // (gated rows always have a whole workgroup)
-  return with_row_shape(a.cols, a.up ? 256 : 0, [&](auto threads, auto reps) {
+  if (a.up)
+    return with_gated_row_shape(a.cols, [&](auto threads, auto reps) {
+      constexpr int kThreads = decltype(threads)::value, kReps = decltype(reps)::value;
+      const dim3 grid(grid_of(a.rows, 1, kThreads, 4)), block(kThreads);
+      if (a.bf16) hipLaunchKernelGGL((quantize_gated_rows_kernel<BF16, kThreads, kReps>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((quantize_gated_rows_kernel<F16, kThreads, kReps>), grid, block, 0, s, a);
+      return check_hip(hipGetLastError(), "quantize_rows launch");
+    });
+  return with_row_shape(a.cols, [&](auto threads, auto reps) {
     constexpr int kThreads = decltype(threads)::value, kReps = decltype(reps)::value, kBlock = kBlockOf<kThreads>;
-    const dim3 grid(grid_of(a.rows, kBlock / kThreads, kBlock, a.up ? 4 : 8));
-    if (!a.up) {
-      if (a.bf16) hipLaunchKernelGGL((quantize_rows_kernel<BF16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-      else hipLaunchKernelGGL((quantize_rows_kernel<F16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-    } else if constexpr (kThreads >= 256) {
-      if (a.bf16) hipLaunchKernelGGL((quantize_gated_rows_kernel<BF16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-      else hipLaunchKernelGGL((quantize_gated_rows_kernel<F16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
-    }
+    const dim3 grid(grid_of(a.rows, kBlock / kThreads, kBlock, 8));
+    if (a.bf16) hipLaunchKernelGGL((quantize_rows_kernel<BF16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
+    else hipLaunchKernelGGL((quantize_rows_kernel<F16, kThreads, kReps>), grid, dim3(kBlock), 0, s, a);
     return check_hip(hipGetLastError(), "quantize_rows launch");
   });
 }

@@ -44,7 +44,7 @@ def _assert_norm(got, x, residual, weight, factors, eps=2.0**-20):
     assert ((got[2].double() - scale).abs().nan_to_num(0) <= (1.001 * 2.0**-24) * scale.abs().nan_to_num(0)).all()
 
 
-DIMS = [1, 7, 8, 9, 64, 333, 512, 513, 1024, 1025, 2048, 2050, 4096, 4099, 8192, 8200, 16384, 16390, 32768, 65529, 65536]
+DIMS = [1, 7, 8, 9, 16, 64, 121, 128, 129, 333, 512, 513, 1024, 1025, 2048, 2049, 2050, 4096, 4099, 8192, 8200, 16384, 16390, 32768, 65529, 65536]
 
 
 @pytest.mark.parametrize("dim", DIMS)
@@ -631,3 +631,19 @@ def test_grouped_product_takes_strides(cuda, counts):
                                                False, 1, positions)])
     ref.assert_near(out.cpu()[:, 2:72], p, p)
     assert (out[:, :2] == 5).all() and (out[:, 72:] == 5).all()
+
+
+@pytest.mark.parametrize("cols", [24, 100, 128, 600, 1030])
+def test_many_short_rows(cuda, cols):
+    # (more rows than there are workgroups: each takes several in turn)
+    gen, rows = _gen(cols), 70001 if cols < 200 else 20001
+    x, up = _rows(gen, "bf16", rows, cols), _rows(gen, "bf16", rows, cols)
+    x[17] = 0
+    x[rows - 1, 3] = math.nan
+    x[rows - 3] = 1e35
+    x[rows // 2] = -500
+    _assert_rows(_quantize(x, None, "bf16"), x, None)
+    _assert_rows(_quantize(x, up, "bf16"), x, up)
+    _assert_norm(_norm(x[:, None], "bf16", up, up[0]), x[:, None], up, up[0], None)
+    both = torch.stack((x, up), 1)
+    _assert_norm(_norm(both, "bf16"), both, None, None, None)
