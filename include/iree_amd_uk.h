@@ -846,8 +846,9 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_copy_pages(void* pool, iree_amd_uk_index_t pa
  * addend_weights[token][j] (addend_weights_stride0 apart; null: 1), and an addend whose
  * weight is 0 changes nothing, whatever it holds: a layer's own output, or those of a
  * token's experts with their weights. One addend without a weight is added in f32,
- * others in 64 bits, in order; h is rounded to the rows' type T (F16 or BF16) and written
- * to sum_out unless that is null. residual and weight may be null (0, and 1). sum_out
+ * others in 64 bits, in order, and their sum is rounded to f32; from f32 h is rounded to
+ * the rows' type T (F16 or BF16), so that a sum within f32's rounding of the middle
+ * between two values of T may go to the farther one. h is written to sum_out unless that is null. residual and weight may be null (0, and 1). sum_out
  * may be residual's own buffer, or with one addend x's, with the same stride; other
  * buffers must not overlap. dim up to 65536. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_rms_norm_quantize(
