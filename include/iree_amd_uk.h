@@ -824,7 +824,7 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_copy_pages(void* pool, iree_amd_uk_index_t pa
  * scale 0, where all of y is 0. A row with a value that is not finite, or whose largest
  * size f32 does not hold, gets zeros and the scale NaN: all of it, and of what is
  * multiplied from it, reads as NaN. q has the bits of the formula in 64 bits
- * (products of two values of 16 bits are in it as far as f32 holds them).
+ * (of rms_norm_quantize, of its products in f32).
  * Rows lie `stride0` elements apart at any alignment of their elements; rows of 8 bits
  * that the products read, 16-byte aligned and whole 16s apart. A call with a size of 0
  * writes nothing (moe_route of no tokens: offsets).
@@ -841,7 +841,10 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_copy_pages(void* pool, iree_amd_uk_index_t pa
 
 /* The residual's addition, RMS norm and 8 bits, in one pass:
  *   h = T(residual + sum_j w_j x_j),  y = h / sqrt(mean(h^2) + eps) * weight
- * and y's row of 8 bits. x is [tokens][addends][dim], x_stride0 elements between
+ * and y's row of 8 bits. The sizes that f32 has to hold are those of h * weight, before the
+ * norm's factor: a row whose largest product does not fit gets zeros and the scale NaN, also
+ * where y would fit; products below 2^-126 lose bits, and a row of which nothing is left
+ * counts as 0. A scale beyond f32 is infinite. x is [tokens][addends][dim], x_stride0 elements between
  * tokens and x_stride1 between a token's addends (one where addends = 1); w_j is
  * addend_weights[token][j] (addend_weights_stride0 apart; null: 1), and an addend whose
  * weight is 0 changes nothing, whatever it holds: a layer's own output, or those of a

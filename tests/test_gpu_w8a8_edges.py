@@ -1,5 +1,7 @@
 """The layer in 8-bit integers on the device where its definitions are easily missed: roundings, sizes
 of values at the ends of f32, sizes of tensors next to the limits."""
+import math
+
 import pytest
 import torch
 
@@ -21,3 +23,63 @@ def test_a_sum_of_several_addends_is_rounded_to_f32_and_then_to_its_type(cuda, k
     q, scale = torch.zeros(tokens, dim, dtype=torch.int8, device="cuda"), torch.zeros(tokens, device="cuda")
     iree_amd.rms_norm_quantize(x, q, scale, tokens, dim, FLAGS[kind], sum_out=out, addends=3, addend_weights=weights.cuda())
     assert torch.equal(out.cpu(), want[:, None].expand(tokens, dim))
+
+
+def _normed(h, weight, eps):
+    """(q, scale f64) of the normed rows: of their products with the weight in f32, which 64 bits hold from there on."""
+    t = (h.float() if weight is None else h.float() * weight.float()).double()
+    top = t.abs().amax(-1)
+    fine = top <= torch.finfo(torch.float32).max
+    q = torch.where((fine & (top > 0))[:, None], torch.round(t * 127 / torch.where(top > 0, top, 1.0)[:, None]), 0.0)
+    scale = torch.where(top == 0, 0.0, top / torch.sqrt(h.double().square().mean(-1) + eps) / 127)
+    return q.nan_to_num(0.0).to(torch.int8), torch.where(fine, scale, math.nan)
+
+
+def _assert_normed(x, weight, eps, addends=1, keep=True):
+    """Of rows x [tokens][dim], which are the sums."""
+    tokens, dim = x.shape
+    given = x if addends == 1 else torch.stack([x] + [torch.zeros_like(x)] * (addends - 1), 1)
+    q, scale = torch.full((tokens, dim), 99, dtype=torch.int8, device="cuda"), torch.full((tokens,), -1.0, device="cuda")
+    out = torch.zeros_like(x).cuda() if keep else None
+    iree_amd.rms_norm_quantize(given.cuda(), q, scale, tokens, dim, FLAGS["bf16"], weight=weight.cuda(), eps=eps, sum_out=out,
+                               addends=addends)
+    want_q, want = _normed(x, weight, eps)
+    if keep:
+        assert torch.equal(out.cpu().nan_to_num(7), x.nan_to_num(7))
+    q, scale = q.cpu(), scale.cpu()
+    assert torch.equal(q, want_q), (q != want_q).any(-1).nonzero()
+    assert torch.equal(torch.isnan(scale), torch.isnan(want)), scale
+    # 64 bits, rounded once to 32: by 2^-24 of it, below 2^-126 by 2^-150, from 2^128 - 2^103 on to infinity
+    beyond = want >= 2.0**128 - 2.0**103
+    assert torch.isinf(scale[beyond]).all()
+    off = torch.where(beyond, 0.0, scale.double() - want).abs().nan_to_num(0)
+    assert (off <= 1.001 * 2.0**-24 * want.nan_to_num(0) + 1.001 * 2.0**-150).all()
+
+
+@pytest.mark.parametrize("dim", [40, 600, 1000, 4096, 8000, 16384, 30000, 65536])
+def test_norms_of_products_at_the_ends_of_f32(cuda, dim):
+    gen = torch.Generator().manual_seed(dim)
+    x = torch.randn(11, dim, generator=gen)
+    x[0] *= 1e30
+    x[1] *= 1e-25
+    x[2] = 0
+    x[2, 7] = 1e-4                            # one value: the norm makes it sqrt(dim)
+    x[3, 5] = math.inf
+    x[4] *= 1e37
+    x[5] = 0
+    x[6] *= 1e-38                             # (subnormal ones among them)
+    x[7, dim - 1] = math.nan
+    x[8] = torch.randint(-127, 128, (dim,), generator=gen) * 2.0**90      # halves between two codes
+    x[8, 0] = 127 * 2.0**91
+    x = x.bfloat16()
+    for size in (1.0, 1e10, 1e-20, 2e38, 1e-30):
+        weight = (size * (1 + torch.rand(dim, generator=gen) / 2)).bfloat16()
+        if size == 1e10:
+            weight = (2.0**31 * torch.ones(dim)).bfloat16()               # (keeps the halves of row 8)
+        _assert_normed(x, weight, 0.0)
+        _assert_normed(x, weight, 1e-6, keep=False)
+        _assert_normed(x, weight, 0.0, addends=2, keep=False)
+    _assert_normed(x, torch.zeros(dim).bfloat16(), 1e-6)
+    weight = torch.ones(dim).bfloat16()
+    weight[3] = math.inf
+    _assert_normed(x, weight, 1e-6)
