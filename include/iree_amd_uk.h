@@ -876,7 +876,7 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_quantize_rows(
  * is packed as iree_amd_uk_pack does for the right-hand side of a matmul, in tiles of
  * 32 x 16 with padding 0: [N / 32][K / 16][32][16], rhs_stride0 bytes between
  * outer columns; 16-byte aligned. out is row-major with any alignment of its elements. Nothing is
- * allocated. */
+ * allocated. Results of 2^24 tiles of 256 x 256 and more are refused. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_matmul_w8a8(
     const void* lhs, iree_amd_uk_index_t lhs_stride0, const float* lhs_scale, const void* rhs,
     iree_amd_uk_index_t rhs_stride0, const float* rhs_scale, const float* bias, void* out,

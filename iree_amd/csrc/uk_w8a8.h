@@ -30,11 +30,16 @@ struct W8A8Args {
 int launch_w8a8(const W8A8Args& a, hipStream_t s);
 // Macro tiles (uk_w8a8_mfma.hip), by number.
 constexpr int kW8A8Shapes = 5;
+constexpr int kW8A8MfmaThreads = 256;
 int launch_w8a8_mfma(const W8A8Args& a, int shape, hipStream_t s);
 // Tiles of rows that there can be at most: of every expert that has any, the last is not full.
 inline int64_t w8a8_row_tiles(const W8A8Args& a, int height) {
   if (!a.offsets) return ceil_div(a.positions, (int64_t)height);
   return a.positions / height + (a.experts < a.positions ? a.experts : a.positions);
+}
+// Workgroups of a call on tiles of that size.
+inline int64_t w8a8_workgroups(const W8A8Args& a, int height, int width) {
+  return w8a8_row_tiles(a, height) * ceil_div((int64_t)a.N, (int64_t)width);
 }
 
 namespace w8a8 {

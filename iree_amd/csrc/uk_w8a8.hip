@@ -226,13 +226,10 @@ int launch_few_rows(const W8A8Args& a, int v, hipStream_t s) {
     default: kernel = w8a8_few_rows_kernel<4, 4, 2, 2>; break;
   }
   const int64_t tiles_n = ceil_div((int64_t)a.N, (int64_t)kTile[v].cols);
-  const int64_t blocks = w8a8_row_tiles(a, kTile[v].rows) * tiles_n;
-  // (a grid's threads are counted in 32 bits)
-  if (blocks > 0xFFFFFFFFll / (kWaves * 64))
-    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "w8a8: too many tiles for one call");
   note_kernel_path("w8a8:few-rows");
   note_macro_tile(kTile[v].rows, kTile[v].cols, 1);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kWaves * 64), 0, s, a, (int)tiles_n);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)w8a8_workgroups(a, kTile[v].rows, kTile[v].cols)), dim3(kWaves * 64), 0,
+                     s, a, (int)tiles_n);
   return check_hip(hipGetLastError(), "w8a8 launch");
 }
 
@@ -240,12 +237,16 @@ int launch_few_rows(const W8A8Args& a, int v, hipStream_t s) {
 
 int launch_w8a8(const W8A8Args& a, hipStream_t s) {
   const int cus = device_cu_count();
-  int best = 0;
+  int best = -1;
   double least = INFINITY;
   for (int v = 0; v < kTiles; ++v) {
+    // (a grid's threads are counted in 32 bits)
+    const int64_t most = 0xFFFFFFFFll / (v < kFewRowsTiles ? kWaves * 64 : kW8A8MfmaThreads);
+    if (w8a8_workgroups(a, kTile[v].rows, kTile[v].cols) > most) continue;
     const double us = estimate_us(a, kTile[v], cus);
     if (us < least) least = us, best = v;
   }
+  if (best < 0) return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "w8a8: too many tiles for one call");
   return best < kFewRowsTiles ? launch_few_rows(a, best, s) : launch_w8a8_mfma(a, best - kFewRowsTiles, s);
 }
 

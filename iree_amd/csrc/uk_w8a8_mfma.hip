@@ -360,7 +360,7 @@ __device__ __forceinline__ void w8a8_mfma_body(const MfmaTileArgs& args) {
 }
 
 template <int WM, int WN, int kRing, int kOcc>
-__global__ __launch_bounds__(256, kOcc) void w8a8_mfma_kernel(MfmaTileArgs args) {
+__global__ __launch_bounds__(kW8A8MfmaThreads, kOcc) void w8a8_mfma_kernel(MfmaTileArgs args) {
   w8a8_mfma_body<WM, WN, kRing>(args);
 }
 
@@ -377,13 +377,9 @@ int launch_tile(const W8A8Args& a, hipStream_t s) {
     set_on.mark(dev);
   }
   const MfmaTileArgs args{a, (int)ceil_div((int64_t)a.N, (int64_t)WN * 32), WM < WN ? 8 : 4};
-  const int64_t blocks = w8a8_row_tiles(a, WM * 32) * args.tiles_n;
-  // (a grid's threads are counted in 32 bits)
-  if (blocks > 0xFFFFFFFFll / 256)
-    return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "w8a8: too many tiles for one call");
   note_kernel_path("w8a8:mfma");
   note_macro_tile(WM * 32, WN * 32, 1);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds_bytes, s, args);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)w8a8_workgroups(a, WM * 32, WN * 32)), dim3(kW8A8MfmaThreads), lds_bytes, s, args);
   return check_hip(hipGetLastError(), "w8a8 launch");
 }
 

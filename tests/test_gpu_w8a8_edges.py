@@ -83,3 +83,26 @@ def test_norms_of_products_at_the_ends_of_f32(cuda, dim):
     weight = torch.ones(dim).bfloat16()
     weight[3] = math.inf
     _assert_normed(x, weight, 1e-6)
+
+
+def test_a_list_whose_small_tiles_no_grid_holds(cuda):
+    # (few channels and a long sum: the estimate alone takes 16 x 16, of which there can be 2^23 and more)
+    positions, N, K, experts = 143191276, 1, 8646, 8
+    gen = torch.Generator().manual_seed(1)
+    lhs, wide = ref.rows8(gen, 5, K), -(-K // 16) * 16
+    rows8 = torch.zeros(5, wide, dtype=torch.int8)
+    rows8[:, :K] = lhs
+    w, w_scale, lhs_scale = ref.rows8(gen, experts, N, K), ref.scales(gen, experts, N), ref.scales(gen, 5)
+    offsets = torch.tensor([0, 3, 3, 40, 41, 41, 90, 100, 150], dtype=torch.int32)
+    rows = torch.zeros(positions, dtype=torch.int32, device="cuda")
+    mine = torch.randint(-1, 6, (150,), generator=gen).int()                 # (some outside)
+    rows[:150] = mine.cuda()
+    out = torch.full((positions, N), 5.0, dtype=torch.float16, device="cuda")
+    iree_amd.grouped_matmul_w8a8(rows8.cuda(), ref.pack(w).cuda(), out, lhs_scale.cuda(), w_scale.cuda(), offsets.cuda(),
+                                 positions, experts, N, K, FLAGS["f16"] | iree_amd.flags.GROUPED_GATHER, lhs_rows=5, rows=rows)
+    found = ref.grouped(lhs, lhs_scale, w, w_scale, offsets, mine, True, False, 1, 150)
+    at, p = torch.tensor([t for t, _ in found]), torch.stack([p for _, p in found])
+    got = out[:200].cpu()
+    ref.assert_near(got[at], p, p)
+    got[at] = 5
+    assert (got == 5).all() and (out[200:] == 5).all()
