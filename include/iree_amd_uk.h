@@ -827,7 +827,7 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_copy_pages(void* pool, iree_amd_uk_index_t pa
  * (of rms_norm_quantize, of its products in f32).
  * Rows lie `stride0` elements apart at any alignment of their elements; rows of 8 bits
  * that the products read, 16-byte aligned and whole 16s apart. A call with a size of 0
- * writes nothing (moe_route of no tokens: offsets).
+ * writes nothing (moe_route of no tokens: offsets; a product with K = 0: the bias, or zeros).
  *===------------------------------------------------------------------------===*/
 #define IREE_AMD_UK_FLAG_ROWS_TYPE_MASK 0xFF
 #define IREE_AMD_UK_FLAG_ROWS_TYPE_F16 0x01

@@ -106,3 +106,17 @@ def test_a_list_whose_small_tiles_no_grid_holds(cuda):
     ref.assert_near(got[at], p, p)
     got[at] = 5
     assert (got == 5).all() and (out[200:] == 5).all()
+
+
+@pytest.mark.parametrize("used", [30, 900])
+@pytest.mark.parametrize("how", [0, iree_amd.flags.GROUPED_GATHER, iree_amd.flags.GROUPED_SCATTER])
+def test_grouped_products_without_a_sum_are_zeros(cuda, how, used):
+    positions, N, experts = used + 20, 70, 3
+    offsets = torch.tensor([0, used // 3, used // 3, used], dtype=torch.int32, device="cuda")
+    rows = torch.arange(positions, dtype=torch.int32, device="cuda")
+    lhs = torch.full((positions, 16), 3, dtype=torch.int8, device="cuda")
+    w = torch.full((experts, 3, 1, 32, 16), 3, dtype=torch.int8, device="cuda")
+    one, out = torch.ones(positions, device="cuda"), torch.full((positions, N), 5.0, device="cuda")
+    iree_amd.grouped_matmul_w8a8(lhs, w, out, one, torch.ones(experts, N, device="cuda"), offsets, positions, experts, N, 0,
+                                 FLAGS["f32"] | how, lhs_rows=positions, rows=rows if how else None)
+    assert not out[:used].any() and (out[used:] == 5).all()
