@@ -895,8 +895,9 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_matmul_w8a8(
  * offsets[e + 1]), and -1 from offsets[experts] on. The same lists on every call.
  * tokens * top_k lies below 2^31.
  *   workspace: at least what iree_amd_uk_moe_route_workspace says, 16-byte aligned; with
- * less, or null, one workgroup does all: slower, the same lists. The caller's: calls
- * that may overlap, and graphs whose replays may, need one each. */
+ * less, or null and 0 bytes, one workgroup does all: slower, the same lists. Null with any
+ * bytes is refused. The caller's: calls that may overlap, and graphs whose replays may,
+ * need one each. */
 IREE_AMD_UK_EXPORT int iree_amd_uk_moe_route(
     const void* logits, iree_amd_uk_index_t logits_stride0, int32_t* expert_ids,
     float* expert_weights, int32_t* offsets, int32_t* rows, iree_amd_uk_index_t tokens,

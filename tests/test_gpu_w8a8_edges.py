@@ -120,3 +120,21 @@ def test_grouped_products_without_a_sum_are_zeros(cuda, how, used):
     iree_amd.grouped_matmul_w8a8(lhs, w, out, one, torch.ones(experts, N, device="cuda"), offsets, positions, experts, N, 0,
                                  FLAGS["f32"] | how, lhs_rows=positions, rows=rows if how else None)
     assert not out[:used].any() and (out[used:] == 5).all()
+
+
+def test_routing_of_many_tokens_with_no_workspace_at_all(cuda):
+    # (the Python function takes one by itself)
+    gen, tokens, experts, top_k = torch.Generator().manual_seed(7), 900, 24, 3
+    logits = torch.randn(tokens, experts, generator=gen)
+    want = ref.route(logits, top_k, True)
+    on = logits.cuda()
+    ids, weights = torch.zeros(tokens, top_k, dtype=torch.int32, device="cuda"), torch.zeros(tokens, top_k, device="cuda")
+    offsets, rows = torch.zeros(experts + 1, dtype=torch.int32, device="cuda"), torch.zeros(tokens * top_k, dtype=torch.int32, device="cuda")
+    lib, flags = iree_amd.load_library(), FLAGS["f32"] | iree_amd.flags.ROUTE_RENORMALIZE
+    call = lambda workspace, nbytes: lib.iree_amd_uk_moe_route(  # noqa: E731
+        on.data_ptr(), experts, ids.data_ptr(), weights.data_ptr(), offsets.data_ptr(), rows.data_ptr(), tokens, experts, top_k,
+        workspace, nbytes, flags, torch.cuda.current_stream().cuda_stream)
+    assert call(None, iree_amd.moe_route_workspace(tokens, experts)) == 3
+    assert not ids.any() and not rows.any()
+    assert call(None, 0) == 0
+    assert torch.equal(ids.cpu(), want[0]) and torch.equal(offsets.cpu(), want[2]) and torch.equal(rows.cpu(), want[3])
