@@ -1335,7 +1335,7 @@ extern "C" int iree_amd_uk_grouped_matmul_w8a8(
                       rhs_expert_stride > (INT64_MAX >> 1) / experts))
     return fail(IREE_AMD_UK_STATUS_INVALID_ARGUMENT,
                 "%s: the experts' weights must lie whole 16 bytes and at least their own size apart", what);
-  if (a.gather && lhs_rows > 1 && lhs_rows * lhs_stride0 >= 0xFFFFFFF0ll)
+  if (a.gather && lhs_rows > 1 && lhs_rows * lhs_stride0 >= 1ll << 32)
     return fail(IREE_AMD_UK_STATUS_UNIMPLEMENTED, "%s: rows to gather from 4 GiB or more", what);
   return launch_w8a8(a, (hipStream_t)stream);
 }

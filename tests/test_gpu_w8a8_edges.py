@@ -138,3 +138,23 @@ def test_routing_of_many_tokens_with_no_workspace_at_all(cuda):
     assert not ids.any() and not rows.any()
     assert call(None, 0) == 0
     assert torch.equal(ids.cpu(), want[0]) and torch.equal(offsets.cpu(), want[2]) and torch.equal(rows.cpu(), want[3])
+
+
+def test_rows_gathered_from_the_last_bytes_below_4_gib(cuda):
+    # 2113665 x 2032 bytes are 2^32 - 16
+    rows, K, N, tokens = 2113665, 2030, 40, 700
+    gen = torch.Generator().manual_seed(3)
+    at = torch.tensor([0, rows - 1, 1056832, rows - 2])
+    mine = ref.rows8(gen, 4, K)
+    lhs = torch.zeros(rows, 2032, dtype=torch.int8, device="cuda")
+    lhs[at.cuda(), :K] = mine.cuda()
+    w, w_scale, scale = ref.rows8(gen, 2, N, K), ref.scales(gen, 2, N), torch.ones(rows, device="cuda")
+    for count in (8, tokens):
+        which = torch.arange(count) % 4
+        out = torch.zeros(count, N, device="cuda")
+        iree_amd.grouped_matmul_w8a8(lhs, ref.pack(w).cuda(), out, scale, w_scale.cuda(),
+                                     torch.tensor([0, count // 2, count], dtype=torch.int32).cuda(), count, 2, N, K,
+                                     FLAGS["f32"] | iree_amd.flags.GROUPED_GATHER, lhs_rows=rows, rows=at[which].int().cuda())
+        for e, part in ((0, slice(0, count // 2)), (1, slice(count // 2, count))):
+            p, _ = ref.product(mine[which[part]], torch.ones(len(which[part])), w[e], w_scale[e])
+            ref.assert_near(out[part].cpu(), p, p)
