@@ -871,7 +871,9 @@ IREE_AMD_UK_EXPORT int iree_amd_uk_quantize_rows(
 
 /* out[m][n] = T((sum_k lhs[m][k] rhs[n][k]) lhs_scale[m] rhs_scale[n] + bias[n])
  * with exact 32-bit integer sums (K up to 131071), scales and bias in f32, T the type in
- * the flags (F16, BF16 or F32), rounded once; bias may be null. lhs is row-major, of 8
+ * the flags (F16, BF16 or F32). The sum, the sum times lhs_scale, and that times rhs_scale
+ * plus bias are each rounded to f32, the last from there to T: where the sum times lhs_scale
+ * passes 2^128 the result is infinite, or NaN next to an rhs_scale of 0. bias may be null. lhs is row-major, of 8
  * bits, its rows readable up to K rounded up to 16 (what lies past K does not count). rhs
  * is packed as iree_amd_uk_pack does for the right-hand side of a matmul, in tiles of
  * 32 x 16 with padding 0: [N / 32][K / 16][32][16], rhs_stride0 bytes between

@@ -158,3 +158,23 @@ def test_rows_gathered_from_the_last_bytes_below_4_gib(cuda):
         for e, part in ((0, slice(0, count // 2)), (1, slice(count // 2, count))):
             p, _ = ref.product(mine[which[part]], torch.ones(len(which[part])), w[e], w_scale[e])
             ref.assert_near(out[part].cpu(), p, p)
+
+
+@pytest.mark.parametrize("M,N,K,path", [(3, 70, 100, "w8a8:few-rows"), (5534, 71, 36, "w8a8:mfma")])
+def test_products_round_the_sum_times_the_row_scale_to_f32(cuda, M, N, K, path):
+    gen = torch.Generator().manual_seed(M)
+    lhs, wide = ref.rows8(gen, M, K), -(-K // 16) * 16
+    rows8 = torch.zeros(M, wide, dtype=torch.int8)
+    rows8[:, :K] = lhs
+    w = ref.rows8(gen, N, K)
+    w[3] = 0                                  # (sums of 0)
+    lhs_scale, w_scale = ref.scales(gen, M) * 1e38, ref.scales(gen, N) * 1e-30
+    lhs_scale[1::3] = 2.0**-140               # (subnormal: the products with whole numbers are exact)
+    w_scale[::7], w_scale[2] = 1e5, 0
+    out = torch.zeros(M, N, device="cuda")
+    iree_amd.matmul_w8a8(rows8.cuda(), ref.pack(w).cuda(), out, lhs_scale.cuda(), w_scale.cuda(), M, N, K, FLAGS["f32"])
+    assert iree_amd.last_kernel_path() == path
+    first = ((lhs.double() @ w.double().T).float() * lhs_scale[:, None]).double()
+    want = (first * w_scale.double()).float()              # (64 bits hold the product: rounded once)
+    assert torch.isinf(want).any() and torch.isnan(want).any() and (want == 0).any()
+    assert torch.equal(out.cpu().nan_to_num(7), want.nan_to_num(7)) and torch.equal(torch.isnan(out.cpu()), torch.isnan(want))
