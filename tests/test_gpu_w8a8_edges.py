@@ -178,3 +178,89 @@ def test_products_round_the_sum_times_the_row_scale_to_f32(cuda, M, N, K, path):
     want = (first * w_scale.double()).float()              # (64 bits hold the product: rounded once)
     assert torch.isinf(want).any() and torch.isnan(want).any() and (want == 0).any()
     assert torch.equal(out.cpu().nan_to_num(7), want.nan_to_num(7)) and torch.equal(torch.isnan(out.cpu()), torch.isnan(want))
+
+
+@pytest.mark.parametrize("tokens,experts,top_k,whole", [(6001, 40, 4, False), (600001, 16, 4, True), (150000, 300, 64, True)])
+def test_routing_of_more_slots_than_a_workgroup_holds(cuda, tokens, experts, top_k, whole):
+    # (above 8192 slots a workgroup reads its choices back from memory: with a workspace from 4 or more such blocks, or in one)
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    logits = torch.randn(tokens, experts, generator=gen, device="cuda") + torch.randn(experts, generator=gen, device="cuda")
+    logits[5] = -math.inf
+    logits[tokens - 3, 3:] = math.nan
+    ids, weights = torch.zeros(tokens, top_k, dtype=torch.int32, device="cuda"), torch.zeros(tokens, top_k, device="cuda")
+    offsets, rows = torch.zeros(experts + 1, dtype=torch.int32, device="cuda"), torch.zeros(tokens * top_k, dtype=torch.int32, device="cuda")
+    iree_amd.moe_route(logits, ids, weights, offsets, rows, tokens, experts, top_k, FLAGS["f32"] | iree_amd.flags.ROUTE_RENORMALIZE,
+                       workspace=None if whole else torch.zeros(16, dtype=torch.uint8, device="cuda"))
+    values, want = torch.sort(logits.nan_to_num(nan=-math.inf, neginf=-math.inf), dim=-1, descending=True, stable=True)
+    want = torch.where(values[:, :top_k] > -math.inf, want[:, :top_k], -1)
+    assert torch.equal(ids.long(), want)
+    slots = torch.where(want < 0, experts, want).flatten()
+    counts = torch.bincount(slots, minlength=experts + 1)
+    assert torch.equal(offsets[1:].long(), counts[:experts].cumsum(0)) and offsets[0] == 0
+    order = torch.sort(slots, stable=True).indices
+    order[int(offsets[-1]):] = -1
+    assert torch.equal(rows.long(), order)
+    p = torch.exp(values[:, :top_k].double() - values[:, :1].double().clamp(min=-1e300)) * (want >= 0)
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+    # (differences of logits of at most 16 rounded by 2^-24 of themselves, expf and the division by 2^-23 each, six additions)
+    assert ((weights.double() - p).abs() <= 2.0**-18 * p + 2.0**-30).all()
+
+
+def test_products_captured_before_they_ever_ran(cuda):
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    sizes = [(21, 65, 2055), (33, 1625, 3009), (30, 1473, 33), (8172, 71, 523), (6717, 67, 460), (6694, 989, 451), (8521, 262, 1186),
+             (8925, 444, 1487), (1681, 8719, 5452)]                          # (a tile each)
+    cases, tiles = [], set()
+    for M, N, K in sizes:
+        wide, high = -(-K // 16), -(-N // 32)
+        lhs = torch.randint(-127, 128, (M, wide * 16), generator=gen, device="cuda", dtype=torch.int8)
+        w = torch.randint(-127, 128, (high, wide, 32, 16), generator=gen, device="cuda", dtype=torch.int8)
+        s, t = (torch.rand(n, generator=gen, device="cuda") + 0.5 for n in (M, N))
+        cases.append((lhs, w, torch.zeros(M, N, dtype=torch.bfloat16, device="cuda"), s, t, M, N, K, FLAGS["bf16"]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for case in cases:
+            iree_amd.matmul_w8a8(*case)
+            tiles.add(iree_amd.last_macro_tile()[:2])
+    assert len(tiles) == 9
+    want = None
+    for _ in range(4):
+        for case in cases:
+            case[2].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [case[2].clone() for case in cases]
+        for case in cases:                    # the program's own work in between
+            case[2].zero_()
+            iree_amd.matmul_w8a8(*case)
+        want = [case[2].clone() for case in cases] if want is None else want
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(case[2], b) and b.abs().sum() > 0 for case, b in zip(cases, want))
+
+
+def test_rows_of_more_than_4_gib(cuda):
+    rows, cols = 70001, 32760
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")        # 4.59e9 bytes
+    at = torch.tensor([0, 1, 35000, rows - 2, rows - 1], device="cuda")
+    mine = (torch.randn(5, cols, generator=torch.Generator().manual_seed(1)) * 2).bfloat16()
+    x[at] = mine.cuda()
+    q, scale = torch.full((rows, cols), 9, dtype=torch.int8, device="cuda"), torch.full((rows,), -1.0, device="cuda")
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+    rest[at] = False
+
+    def check(want, want_scale):
+        assert torch.equal(q[at].cpu(), want)
+        assert ((scale[at].cpu().double() - want_scale).abs() <= 1.001 * 2.0**-24 * want_scale).all()
+        assert not scale[rest].any()
+        q[at] = 0
+        assert not q.any()
+        q.fill_(9)
+
+    iree_amd.quantize_rows(x, q, scale, rows, cols, FLAGS["bf16"])
+    check(*ref.codes(mine.double()))
+    iree_amd.quantize_rows(x, q, scale, rows, cols, FLAGS["bf16"], up=x)
+    check(*ref.codes(ref.silu_mul(mine, mine)))
+    iree_amd.rms_norm_quantize(x, q, scale, rows, cols, FLAGS["bf16"], eps=2.0**-20, sum_out=x)
+    check(*ref.norm(mine, None, 2.0**-20))
+    assert torch.equal(x[at].cpu(), mine)
