@@ -196,9 +196,10 @@ static_assert(kTiles == kFewRowsTiles + kW8A8Shapes, "a tile for each kernel");
 // some have more last_two and last_more times how many more. `weights` and `results` are per MB; groups add `grouped` for finding a
 // tile and `empty` per 1000 workgroups of the grid. How the rows are dealt to the experts only the device knows:
 // as if each position's expert were drawn at random, an expert with rows has a tile that is half full.
-// Fitted to the times of every tile on 1305 problems (1 to 16384 rows or tokens, 64 to 16384 channels and K,
-// matrices and groups of 8 to 256 experts): what it picks is 1.2 % from the best on average for one matrix
-// and 1.6 % for groups, in the 95th percentile 7 and 10 %. (Fitted to half of them, on the others 1.6 and 11 %.)
+// Fitted (non-negative least squares, errors relative to the time) to the times of every tile on 1305 problems: 1 to 16384
+// rows or tokens, 64 to 16384 channels and K, matrices and groups of 8 to 256 experts. On the 1340 others of
+// profiles/w8a8_tiles.txt what it picks is 1.0 % from the best tile on average for one matrix and 1.9 % for groups, in the 95th
+// percentile 8 and 11 %. (Of the floor the best tile itself may be far: 1.3 to 4 times, by the same record.)
 double estimate_us(const W8A8Args& a, const Tile& t, int cus) {
   const double P = (double)a.positions, width = (double)ceil_div((int64_t)a.N, (int64_t)t.cols);
   double experts = 1.0, row_tiles = (double)ceil_div(a.positions, (int64_t)t.rows), us = t.call;
