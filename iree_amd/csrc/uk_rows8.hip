@@ -13,7 +13,8 @@
 // the device (5.1 TB/s, 11 of them vector instructions), eight weighted addends of 2048 x 4096, 176 MB, 36.1 and
 // 34.6 (16 of them vector instructions: the sums in 64 bits), one row 3.2; the gate of 2048 x 14336,
 // 147 MB, 36.0: 20 of them vector instructions, which the one workgroup of a compute unit does not hide behind its
-// barriers (two of 512 threads with twice the elements each: 50 us, more registers than two have room for).
+// barriers (two of 512 threads with twice the elements each: 50 us, more registers than two have room for). Rows above
+// 16384 spill: norms of 512 x 32768 37.7 us, of 256 x 65536 94, the gate of 1024 x 28672 42.0, all of 117 or 147 MB.
 #include "uk_common.h"
 #include "uk_kv4.h"
 
@@ -235,7 +236,8 @@ __global__ __launch_bounds__(kBlockOf<kThreads>) void rms_norm_quantize_kernel(R
       next_bits[r] = residual && at < dim ? load8(residual, at, dim) : u32x4{0, 0, 0, 0};
     }
   };
-  // (longer rows leave no room for a second one)
+  // (rows above 16384, of 32 or 64 elements a thread, spill registers without a second row as well: 34 to 36 and 234 to 258
+  // with one addend, 74 to 76 and more with several)
   constexpr bool kAhead = kReps <= 2;
   if (kAhead && token < a.tokens) load_row(token);
   // (the weight, too, is on its way before it is needed, and for all rows of a workgroup, where there is room for it)
